@@ -600,6 +600,64 @@ int mvb_row_norm_rope_kv_write(int dtype, void* q, int64_t q_row_stride, void* k
                                void* v_cache, int64_t num_slots, int num_tokens, int num_q_heads, int num_kv_heads, int head_dim,
                                int kv_in_place, int32_t* dev_status, void* stream);
 
+/*
+ * A paged cache of one layer's keys and values in 4 bits, and rotation in all its forms.
+ *
+ * mvb_kv4_cache: codes uint8 [num_blocks, num_kv_heads, block_size, head_dim / 2]; affine bf16 [num_blocks, num_kv_heads, block_size,
+ *   head_dim / 64, 2], for each group of 64 channels of a row its (scale, minimum): code c stands for minimum + scale * c, with scale =
+ *   bf16((greatest - least) * fp32(1/15)) and c = round((x - least) / scale) held to 0..15.  head_dim 64, 128 or 256; block_size a multiple
+ *   of 64; 16-byte aligned; slots below 2^31.  Channel 8 L + e lies in bits 4 (e / 2) + 16 (e % 2) of a 32-bit word: word (D / 32) (L % 4) +
+ *   L / 4 of a row of keys, word (D / 64) (L % 8) + L / 8 of a row of values.  Values are finite, with a spread inside a group that is too.
+ * mvb_rotary: the first rotary_dim (even) channels of every head of q [num_tokens, num_q_heads, head_dim] and k turned by the angles of
+ *   cos_sin fp32 [max_pos, rotary_dim] (cosines, then sines): pairs (2i, 2i + 1) if interleaved, else (i, i + rotary_dim / 2); the others
+ *   carried along.  *_out the same as q and k (in place) or apart from them.  dtype as elsewhere; num_q_heads or num_kv_heads 0: without.
+ *   A position outside the table is reported and its token left unturned.
+ * mvb_rotary_kv4_write: bf16; q turned into q_out (may be q; num_q_heads 0: none), k turned and quantised, v quantised, into slot
+ *   slot_mapping[token] (-1: not cached); k_in_place: k is turned in place too.  cos_sin NULL: nothing is turned.  rotary_dim a multiple
+ *   of 16.  A slot given twice in one call: either token's row.
+ * mvb_kv4_gather: the cached rows of sequence b, tokens 0 .. cu_seqlens_k[b + 1] - cu_seqlens_k[b], as dense bf16 rows k_out, v_out
+ *   [num_rows, num_kv_heads, head_dim] from row cu_seqlens_k[b] on; rows behind the last sequence stay as they are; a block id outside the
+ *   pool is reported and reads as zeros.
+ * mvb_decode_attn4: one query token per sequence over its cache_seqlens cached tokens, as mvb_decode_attn_capped; num_q_heads <= 8 *
+ *   num_kv_heads.  spans (NULL: all tokens): int32 [num_seqs, num_kv_heads, budget], the 64-token spans that a head's queries read, each once;
+ *   entries below 0 are skipped (not with a window).  A sequence of no tokens, or none that is read, gives zeros.  workspace of
+ *   mvb_decode_attn4_workspace_bytes, 256-byte aligned, zeroed once by the caller and left zeroed where it has to be; calls that share it
+ *   must not overlap.
+ * mvb_kv4_summarise: bounds of the keys of the spans that a step's tokens were written to: summaries bf16 [num_blocks, num_kv_heads,
+ *   block_size / 64, 2, head_dim], least and greatest key per channel over the span's rows up to the step's last one.  The tokens of a
+ *   sequence stand next to each other, in order.
+ * mvb_kv4_select: per sequence and KV head the `budget` (>= 2) spans with the greatest sum over the group's heads and the channels of
+ *   max(q least, q greatest), the first and the last span always among them, of equal sums the lower index; ascending, -1 behind them.
+ */
+typedef struct mvb_kv4_cache {
+  void* k_codes;
+  void* k_affine;
+  void* v_codes;
+  void* v_affine;
+  int64_t num_blocks;
+  int32_t block_size, num_kv_heads, head_dim;
+} mvb_kv4_cache;
+
+int mvb_rotary(const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride, void* q_out, int64_t q_out_row_stride, void* k_out,
+               int64_t k_out_row_stride, const int64_t* positions, const float* cos_sin, int64_t max_pos, int num_tokens, int num_q_heads,
+               int num_kv_heads, int head_dim, int rotary_dim, int interleaved, int dtype, int32_t* dev_status, void* stream);
+int mvb_rotary_kv4_write(const void* q, int64_t q_row_stride, void* q_out, int64_t q_out_row_stride, void* k, int64_t k_row_stride,
+                         const void* v, int64_t v_row_stride, const int64_t* positions, const float* cos_sin, int64_t max_pos,
+                         int rotary_dim, int interleaved, const int32_t* slot_mapping, const mvb_kv4_cache* cache, int num_tokens,
+                         int num_q_heads, int k_in_place, int32_t* dev_status, void* stream);
+int mvb_kv4_gather(const mvb_kv4_cache* cache, const int32_t* cu_seqlens_k, const int32_t* block_table, int64_t table_stride,
+                   int table_width, int num_seqs, int num_rows, void* k_out, void* v_out, int32_t* dev_status, void* stream);
+size_t mvb_decode_attn4_workspace_bytes(int max_seqs, int num_q_heads, int num_kv_heads, int head_dim);
+int mvb_decode_attn4(const void* q, int64_t q_row_stride, const mvb_kv4_cache* cache, const int32_t* cache_seqlens,
+                     const int32_t* block_table, int64_t table_stride, int table_width, const int32_t* spans, int budget, int num_seqs,
+                     int num_q_heads, float scale, int window_left, float softcap, float out_scale, void* out, int64_t out_row_stride,
+                     void* workspace, size_t workspace_bytes, int32_t* dev_status, void* stream);
+int mvb_kv4_summarise(const mvb_kv4_cache* cache, const int32_t* slot_mapping, int num_tokens, void* summaries, int32_t* dev_status,
+                      void* stream);
+int mvb_kv4_select(const void* q, int64_t q_row_stride, const void* summaries, int64_t num_blocks, int block_size,
+                   const int32_t* cache_seqlens, const int32_t* block_table, int64_t table_stride, int table_width, int num_seqs,
+                   int num_q_heads, int num_kv_heads, int head_dim, int budget, int32_t* spans, int32_t* dev_status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

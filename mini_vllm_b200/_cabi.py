@@ -17,6 +17,12 @@ class AttnExtras(C.Structure):
     _fields_ = [("sinks", vp), ("slopes", vp), ("head_gate", vp), ("head_gate_row_stride", i64), ("keep_first", i32)]
 
 
+class KV4Cache(C.Structure):
+    """``mvb_kv4_cache``"""
+    _fields_ = [("k_codes", vp), ("k_affine", vp), ("v_codes", vp), ("v_affine", vp), ("num_blocks", i64), ("block_size", i32),
+                ("num_kv_heads", i32), ("head_dim", i32)]
+
+
 # name -> (restype, argtypes); mirrors include/mini_vllm_b200.h exactly
 SIGNATURES = {
     "mvb_abi_version": (i32, []),
@@ -104,6 +110,13 @@ SIGNATURES = {
     "mvb_gated_group_norm": (i32, [i32, vp, i64, vp, i64, vp, vp, i64, i32, i32, i32, f32, vp]),
     "mvb_row_norm_rope_kv_write": (i32, [i32, vp, i64, vp, i64, vp, i64, vp, vp, i32, i32, i32, f32, vp, vp, i64, vp, vp, vp, i64, i32,
                                          i32, i32, i32, i32, vp, vp]),
+    "mvb_rotary": (i32, [vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, i64, i32, i32, i32, i32, i32, i32, i32, vp, vp]),
+    "mvb_rotary_kv4_write": (i32, [vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, i64, i32, i32, vp, vp, i32, i32, i32, vp, vp]),
+    "mvb_kv4_gather": (i32, [vp, vp, vp, i64, i32, i32, i32, vp, vp, vp, vp]),
+    "mvb_decode_attn4_workspace_bytes": (sz, [i32, i32, i32, i32]),
+    "mvb_decode_attn4": (i32, [vp, i64, vp, vp, vp, i64, i32, vp, i32, i32, i32, f32, i32, f32, f32, vp, i64, vp, sz, vp, vp]),
+    "mvb_kv4_summarise": (i32, [vp, vp, i32, vp, vp, vp]),
+    "mvb_kv4_select": (i32, [vp, i64, vp, i64, i32, vp, vp, i64, i32, i32, i32, i32, i32, i32, vp, vp, vp]),
 }
 
 _lib = None

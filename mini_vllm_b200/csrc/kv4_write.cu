@@ -1,0 +1,302 @@
+// The way into the 4-bit cache and out of it as dense rows (elementwise passes, bound by memory).
+//
+// Write: q rotated; k rotated, rounded to bf16 and quantised; v quantised.  A lane owns eight neighbouring channels, so a head's row is 8,
+// 16 or 32 neighbouring lanes; a group of 64 channels is eight lanes, which agree on its least and greatest value by three shuffles; the
+// partner of a channel rotated by halves lies with another lane of the row and comes by shuffle.  A warp stays with one token, whose
+// angles a lane then loads once for all of its rows.
+//
+// Gather: the contexts of a ragged step as dense bf16 rows, for the prompt kernel.
+#include "dtype.cuh"
+#include "host_util.cuh"
+#include "kv4.cuh"
+
+#include <type_traits>
+
+namespace mvb {
+
+struct Kv4WriteParams {
+  const __nv_bfloat16* q;
+  __nv_bfloat16* q_out;
+  __nv_bfloat16* k;
+  const __nv_bfloat16* v;
+  int64_t q_stride, qo_stride, k_stride, v_stride;
+  const int64_t* positions;
+  const float* cos_sin;                // nullptr: nothing is rotated
+  int64_t max_pos;
+  const int32_t* slots;                // nullptr: nothing is cached
+  uint8_t *k_codes, *v_codes;
+  uint32_t *k_affine, *v_affine;
+  int64_t num_slots;
+  FastDiv by_block, by_token;
+  int tokens, hq, hkv, block_size, rot, k_in_place;
+  int* dev_status;
+};
+
+// round(t / s) for 0 <= t <= about 15 s, as the correctly rounded quotient rounds: the product with the approximate reciprocal decides
+// unless it lies within 2^-10 of a half, which a division then settles
+__device__ __forceinline__ uint32_t kv4_code(float t, float s, float r) {
+  float f = t * r;
+  const float n = rintf(f);
+  if (fabsf(fabsf(f - n) - 0.5f) < 0x1p-10f) f = __fdiv_rn(t, s);
+  return static_cast<uint32_t>(fminf(rintf(f), 15.f));
+}
+
+template <int D, bool INTER, int ITEMS>
+__global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4WriteParams p) {
+  constexpr int LPH = D / 8, RPW = 32 / LPH;                 // lanes of a row, rows a warp holds at once
+  constexpr uint32_t FULL = 0xffffffffu;
+  const int lane = threadIdx.x & 31, c = lane % LPH, sub = lane / LPH;
+  const uint32_t warp = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const uint32_t t = p.by_token.div(warp);
+  if (t >= static_cast<uint32_t>(p.tokens)) return;          // warp-uniform
+  const int rows = p.hq + 2 * p.hkv;
+  const int row0 = static_cast<int>(warp - t * p.by_token.n) * (RPW * ITEMS) + sub;
+  const int half = p.rot >> 1;
+
+  uint4 x[ITEMS];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int row = row0 + i * RPW;
+    x[i] = make_uint4(0, 0, 0, 0);
+    if (row < rows) {
+      const __nv_bfloat16* src = row < p.hq ? p.q + static_cast<int64_t>(t) * p.q_stride + static_cast<int64_t>(row) * D
+                                 : row < p.hq + p.hkv ? p.k + static_cast<int64_t>(t) * p.k_stride + static_cast<int64_t>(row - p.hq) * D
+                                                      : p.v + static_cast<int64_t>(t) * p.v_stride + static_cast<int64_t>(row - p.hq - p.hkv) * D;
+      x[i] = *reinterpret_cast<const uint4*>(src + c * 8);
+    }
+  }
+  const bool turns = p.cos_sin != nullptr && c * 8 < p.rot;  // this lane's channels are rotated
+  bool ok = true;
+  float cs[8], sn[8];
+  const bool second = !INTER && c * 8 >= half;               // halves: the lane holds the second one of its pairs
+  const int partner = sub * LPH + (turns ? (second ? c - half / 8 : c + half / 8) : c);
+  if (p.cos_sin != nullptr) {
+    const int64_t pos = p.positions[t];
+    ok = pos >= 0 && pos < p.max_pos;
+    if (!ok && lane == 0) report(p.dev_status, kDevBadPosition, t);
+    if (turns && ok) {
+      const float* tab = p.cos_sin + pos * p.rot + (INTER ? c * 4 : (second ? c * 8 - half : c * 8));
+#pragma unroll
+      for (int e = 0; e < (INTER ? 4 : 8); e += 4) {
+        *reinterpret_cast<float4*>(cs + e) = __ldg(reinterpret_cast<const float4*>(tab + e));
+        *reinterpret_cast<float4*>(sn + e) = __ldg(reinterpret_cast<const float4*>(tab + half + e));
+      }
+    }
+  }
+  int64_t slot = p.slots != nullptr ? p.slots[t] : -1;
+  if (slot < -1 || slot >= p.num_slots) {
+    if (lane == 0) report(p.dev_status, kDevBadSlot, t);
+    slot = -1;
+  }
+  const int64_t block = slot >= 0 ? p.by_block.div(static_cast<uint32_t>(slot)) : 0;
+  const int in_block = slot >= 0 ? static_cast<int>(slot - block * p.block_size) : 0;
+
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int row = row0 + i * RPW;
+    const bool is_q = row < p.hq, is_v = row >= p.hq + p.hkv;
+    float y[8];
+    {
+      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+      uint32_t o[4] = {0, 0, 0, 0};
+      if constexpr (!INTER) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = __shfl_sync(FULL, w[e], partner);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { y[2 * e] = bf16_lo(w[e]); y[2 * e + 1] = bf16_hi(w[e]); }
+      if (turns && ok && !is_v) {
+        if constexpr (INTER) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float a = y[2 * e], b = y[2 * e + 1];
+            y[2 * e] = __fsub_rn(__fmul_rn(a, cs[e]), __fmul_rn(b, sn[e]));
+            y[2 * e + 1] = __fadd_rn(__fmul_rn(b, cs[e]), __fmul_rn(a, sn[e]));
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float other = (e & 1) ? bf16_hi(o[e >> 1]) : bf16_lo(o[e >> 1]);
+            const float a = __fmul_rn(y[e], cs[e]), b = __fmul_rn(other, sn[e]);
+            y[e] = second ? __fadd_rn(a, b) : __fsub_rn(a, b);
+          }
+        }
+        x[i] = make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+        const uint32_t r[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { y[2 * e] = bf16_lo(r[e]); y[2 * e + 1] = bf16_hi(r[e]); }
+      }
+    }
+    if (row < rows && is_q) *reinterpret_cast<uint4*>(p.q_out + static_cast<int64_t>(t) * p.qo_stride + static_cast<int64_t>(row) * D + c * 8) = x[i];
+    if (row < rows && !is_q && !is_v && p.k_in_place && turns && ok)
+      *reinterpret_cast<uint4*>(p.k + static_cast<int64_t>(t) * p.k_stride + static_cast<int64_t>(row - p.hq) * D + c * 8) = x[i];
+    if (slot < 0) continue;                                  // warp-uniform
+    // the group's bounds; every lane of the warp takes part (rows of q and rows past the last one for nothing)
+    float lo = fminf(fminf(fminf(y[0], y[1]), fminf(y[2], y[3])), fminf(fminf(y[4], y[5]), fminf(y[6], y[7])));
+    float hi = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
+#pragma unroll
+    for (int off = 1; off < 8; off <<= 1) {
+      lo = fminf(lo, __shfl_xor_sync(FULL, lo, off));
+      hi = fmaxf(hi, __shfl_xor_sync(FULL, hi, off));
+    }
+    if (row >= rows || is_q) continue;
+    const float scale = __bfloat162float(__float2bfloat16_rn(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f)));
+    uint32_t word = 0;
+    if (scale > 0.f) {
+      const bool usual = scale > 0x1p-100f && scale < 0x1p100f;            // (its reciprocal is a normal number)
+      const float r = fast_rcp(scale);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float d = __fsub_rn(y[e], lo);
+        const uint32_t code = usual ? kv4_code(d, scale, r) : static_cast<uint32_t>(fminf(rintf(__fdiv_rn(d, scale)), 15.f));
+        word |= (code & 15u) << kv4_shift(e);
+      }
+    }
+    const int h = row - p.hq - (is_v ? p.hkv : 0);
+    const int64_t at = kv4_row(block, p.hkv, h, p.block_size, in_block);
+    uint32_t* codes = reinterpret_cast<uint32_t*>((is_v ? p.v_codes : p.k_codes) + at * (D / 2));
+    codes[kv4_word<D>(c, !is_v)] = word;
+    if ((c & 7) == 0) (is_v ? p.v_affine : p.k_affine)[at * (D / 64) + (c >> 3)] = pack_bf16(scale, lo);
+  }
+}
+
+struct Kv4GatherParams {
+  const uint32_t *k_codes, *v_codes, *k_affine, *v_affine;
+  __nv_bfloat16 *k_out, *v_out;
+  const int32_t* cu;
+  const int32_t* block_table;
+  int64_t table_stride, num_blocks;
+  FastDiv by_token, by_block;
+  int table_width, num_seqs, rows, hkv, block_size;
+  int* dev_status;
+};
+
+template <int D, int ITEMS>
+__global__ void __launch_bounds__(256) kv4_gather_kernel(const Kv4GatherParams p) {
+  constexpr int LPH = D / 8, RPW = 32 / LPH;
+  const int lane = threadIdx.x & 31, c = lane % LPH, sub = lane / LPH;
+  const uint32_t warp = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const uint32_t t = p.by_token.div(warp);
+  if (t >= static_cast<uint32_t>(p.rows)) return;
+  const int total = p.cu[p.num_seqs];
+  if (static_cast<int>(t) >= total) return;                  // rows behind the last sequence are left as they are
+  const int b = seq_of_row(p.cu, p.num_seqs, t);
+  const int token = static_cast<int>(t) - p.cu[b];
+  const int col = p.by_block.div(token);
+  const int64_t block = col < p.table_width ? p.block_table[b * p.table_stride + col] : -1;
+  const bool ok = block >= 0 && block < p.num_blocks;
+  if (!ok && lane == 0) report(p.dev_status, kDevBadBlock, b);
+  const int in_block = token - col * p.block_size;
+  const int row0 = static_cast<int>(warp - t * p.by_token.n) * (RPW * ITEMS) + sub;
+  uint32_t word[ITEMS], affine[ITEMS];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int row = row0 + i * RPW;
+    word[i] = affine[i] = 0;                                 // a bad block reads as zeros
+    if (row < 2 * p.hkv && ok) {
+      const bool is_v = row >= p.hkv;
+      const int64_t at = kv4_row(block, p.hkv, is_v ? row - p.hkv : row, p.block_size, in_block);
+      word[i] = __ldg((is_v ? p.v_codes : p.k_codes) + at * (D / 8) + kv4_word<D>(c, !is_v));
+      affine[i] = __ldg((is_v ? p.v_affine : p.k_affine) + at * (D / 64) + (c >> 3));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int row = row0 + i * RPW;
+    if (row >= 2 * p.hkv) continue;
+    const bool is_v = row >= p.hkv;
+    float y[8];
+    kv4_values(word[i], affine[i], y);
+    __nv_bfloat16* dst = (is_v ? p.v_out : p.k_out) + (static_cast<int64_t>(t) * p.hkv + (is_v ? row - p.hkv : row)) * D;
+    store_vec<__nv_bfloat16, 8>(dst + c * 8, y);
+  }
+}
+
+template <class F>
+static int by_head_dim(int d, F&& f) {
+  if (d == 64) return f(std::integral_constant<int, 64>{});
+  if (d == 128) return f(std::integral_constant<int, 128>{});
+  return f(std::integral_constant<int, 256>{});
+}
+
+}  // namespace mvb
+
+extern "C" int mvb_rotary_kv4_write(const void* q, int64_t q_row_stride, void* q_out, int64_t q_out_row_stride, void* k,
+                                    int64_t k_row_stride, const void* v, int64_t v_row_stride, const int64_t* positions,
+                                    const float* cos_sin, int64_t max_pos, int rotary_dim, int interleaved, const int32_t* slot_mapping,
+                                    const mvb_kv4_cache* cache, int num_tokens, int num_q_heads, int k_in_place, int32_t* dev_status,
+                                    void* stream) {
+  using namespace mvb;
+  int rc = kv4_check(cache);
+  if (rc != kOk) return rc;
+  if (num_tokens < 0 || num_q_heads < 0) return kInvalidArgument;
+  const int d = cache->head_dim;
+  if (cos_sin != nullptr) {
+    if (!positions || max_pos <= 0 || rotary_dim <= 0) return kInvalidArgument;
+    if (rotary_dim > d || rotary_dim % 16 != 0) return kUnsupportedShape;
+  }
+  if (num_tokens == 0) return kOk;
+  if (!k || !v || !slot_mapping || (num_q_heads > 0 && (!q || !q_out))) return kInvalidArgument;
+  if ((num_q_heads > 0 && (q_row_stride % 8 || q_out_row_stride % 8)) || k_row_stride % 8 || v_row_stride % 8) return kMisaligned;
+  if (!is_aligned(k, 16) || !is_aligned(v, 16) || !is_aligned(cos_sin, 16) || (num_q_heads > 0 && (!is_aligned(q, 16) || !is_aligned(q_out, 16))))
+    return kMisaligned;
+  Kv4WriteParams p;
+  p.q = static_cast<const __nv_bfloat16*>(q); p.q_out = static_cast<__nv_bfloat16*>(q_out);
+  p.k = static_cast<__nv_bfloat16*>(k); p.v = static_cast<const __nv_bfloat16*>(v);
+  p.q_stride = q_row_stride; p.qo_stride = q_out_row_stride; p.k_stride = k_row_stride; p.v_stride = v_row_stride;
+  p.positions = positions; p.cos_sin = cos_sin; p.max_pos = max_pos; p.slots = slot_mapping;
+  p.k_codes = static_cast<uint8_t*>(cache->k_codes); p.v_codes = static_cast<uint8_t*>(cache->v_codes);
+  p.k_affine = static_cast<uint32_t*>(cache->k_affine); p.v_affine = static_cast<uint32_t*>(cache->v_affine);
+  p.num_slots = cache->num_blocks * cache->block_size;
+  p.by_block = FastDiv(static_cast<uint32_t>(cache->block_size));
+  p.tokens = num_tokens; p.hq = num_q_heads; p.hkv = cache->num_kv_heads; p.block_size = cache->block_size;
+  p.rot = cos_sin != nullptr ? rotary_dim : 0; p.k_in_place = k_in_place; p.dev_status = dev_status;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return by_head_dim(d, [&](auto tag) -> int {
+    constexpr int D = decltype(tag)::value;
+    constexpr int RPW = 32 / (D / 8);
+    const int64_t groups = (static_cast<int64_t>(p.hq) + 2 * p.hkv + RPW - 1) / RPW;
+    // four rows in flight per lane once that still leaves every SM its 32 warps
+    const int items = num_tokens * ((groups + 3) / 4) >= static_cast<int64_t>(sm_count()) * 32 ? 4 : 1;
+    const int64_t per_token = (groups + items - 1) / items, warps = per_token * num_tokens;
+    if (warps > 0x7fffffffLL - 8) return kUnsupportedShape;
+    Kv4WriteParams r = p;
+    r.by_token = FastDiv(static_cast<uint32_t>(per_token));
+    const unsigned grid = static_cast<unsigned>((warps + 7) / 8);
+    if (items == 4 && interleaved) kv4_write_kernel<D, true, 4><<<grid, 256, 0, st>>>(r);
+    else if (items == 4) kv4_write_kernel<D, false, 4><<<grid, 256, 0, st>>>(r);
+    else if (interleaved) kv4_write_kernel<D, true, 1><<<grid, 256, 0, st>>>(r);
+    else kv4_write_kernel<D, false, 1><<<grid, 256, 0, st>>>(r);
+    return cudaGetLastError() == cudaSuccess ? kOk : kLaunchFailed;
+  });
+}
+
+extern "C" int mvb_kv4_gather(const mvb_kv4_cache* cache, const int32_t* cu_seqlens_k, const int32_t* block_table, int64_t table_stride,
+                              int table_width, int num_seqs, int num_rows, void* k_out, void* v_out, int32_t* dev_status, void* stream) {
+  using namespace mvb;
+  int rc = kv4_check(cache);
+  if (rc != kOk) return rc;
+  if (num_seqs < 0 || num_rows < 0) return kInvalidArgument;
+  if (num_seqs == 0 || num_rows == 0) return kOk;
+  if (!cu_seqlens_k || !block_table || !k_out || !v_out || table_width <= 0 || table_stride < table_width) return kInvalidArgument;
+  if (!is_aligned(k_out, 16) || !is_aligned(v_out, 16)) return kMisaligned;
+  Kv4GatherParams p;
+  p.k_codes = static_cast<const uint32_t*>(cache->k_codes); p.v_codes = static_cast<const uint32_t*>(cache->v_codes);
+  p.k_affine = static_cast<const uint32_t*>(cache->k_affine); p.v_affine = static_cast<const uint32_t*>(cache->v_affine);
+  p.k_out = static_cast<__nv_bfloat16*>(k_out); p.v_out = static_cast<__nv_bfloat16*>(v_out);
+  p.cu = cu_seqlens_k; p.block_table = block_table; p.table_stride = table_stride; p.num_blocks = cache->num_blocks;
+  p.by_block = FastDiv(static_cast<uint32_t>(cache->block_size));
+  p.table_width = table_width; p.num_seqs = num_seqs; p.rows = num_rows; p.hkv = cache->num_kv_heads; p.block_size = cache->block_size;
+  p.dev_status = dev_status;
+  return by_head_dim(cache->head_dim, [&](auto tag) -> int {
+    constexpr int D = decltype(tag)::value;
+    constexpr int RPW = 32 / (D / 8), ITEMS = 4;
+    const int64_t groups = (2 * static_cast<int64_t>(p.hkv) + RPW - 1) / RPW, per_token = (groups + ITEMS - 1) / ITEMS;
+    const int64_t warps = per_token * num_rows;
+    if (warps > 0x7fffffffLL - 8) return kUnsupportedShape;
+    Kv4GatherParams r = p;
+    r.by_token = FastDiv(static_cast<uint32_t>(per_token));
+    kv4_gather_kernel<D, ITEMS><<<static_cast<unsigned>((warps + 7) / 8), 256, 0, static_cast<cudaStream_t>(stream)>>>(r);
+    return cudaGetLastError() == cudaSuccess ? kOk : kLaunchFailed;
+  });
+}

@@ -1194,3 +1194,261 @@ def moe_gemm(x: torch.Tensor, weight: torch.Tensor, rows: ExpertRows, k: int,
     _cabi.check(rc, "mvb_moe_gemm")
     LaunchCounter.add(1)
     return out
+
+
+# ---- rotation in all its forms, and a paged cache of keys and values in 4 bits ------------------------------------------------------
+def _here(*named: tuple) -> None:
+    """Every (tensor, dtype or None, name) is a tensor of the current device (None: not given)."""
+    device = None
+    for t, dtype, name in named:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor (the kernels have no CPU path)")
+        if dtype is not None and t.dtype != dtype:
+            raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+        if device is None:
+            device = torch.cuda.current_device()
+        if t.device.index != device:
+            raise ValueError(f"{name} is on {t.device}; the current device is cuda:{device}")
+
+
+def _need_rows(t: torch.Tensor | None, name: str) -> None:
+    """[tokens, heads, size] with heads next to each other; only the token stride is free."""
+    if t is not None and t.numel():
+        _heads_contiguous(t, name)
+
+
+def _need_shape(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def rotary(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tensor, cos_sin: torch.Tensor, interleaved: bool = False,
+           q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None, status: torch.Tensor | None = None):
+    """Turns the first ``cos_sin.shape[1]`` channels of every head of ``q [T, Hq, D]`` and ``k [T, Hkv, D]`` (bf16 or fp32; either may be
+    None) by the angles of ``cos_sin`` fp32 ``[positions, rotated channels]`` (cosines, then sines; ``models.layers.rotary`` builds them):
+    pairs ``(2i, 2i + 1)`` if ``interleaved``, else halves.  In place, or into ``q_out`` and ``k_out`` (apart from ``q`` and ``k``)."""
+    one = q if q is not None else k
+    _need_shape(one is not None, "rotary needs q or k")
+    if one.dtype not in _DTYPE:
+        raise TypeError(f"q and k must be bfloat16 or float32, got {one.dtype}")
+    q_out, k_out = q if q_out is None else q_out, k if k_out is None else k_out
+    _here((q, one.dtype, "q"), (k, one.dtype, "k"), (q_out, one.dtype, "q_out"), (k_out, one.dtype, "k_out"),
+          (positions, torch.int64, "positions"), (cos_sin, torch.float32, "cos_sin"), (status, torch.int32, "status"))
+    for t, like, name in ((q, q, "q"), (k, k, "k"), (q_out, q, "q_out"), (k_out, k, "k_out")):
+        _need_rows(t, name)
+        _need_shape(t is None or (t.dim() == 3 and like is not None and t.shape == like.shape), f"{name} must be [tokens, heads, head_dim], as its input")
+    T, _, d = one.shape
+    for t in (q, k):
+        _need_shape(t is None or (t.shape[0] == T and t.shape[2] == d), "q and k must have the same tokens and head size")
+    _need_shape(positions.numel() == T and positions.is_contiguous(), "positions must be one contiguous number per token")
+    _need_shape(cos_sin.dim() == 2 and cos_sin.is_contiguous(), "cos_sin must be [positions, rotated channels], contiguous")
+    heads = [0 if t is None else t.shape[1] for t in (q, k)]
+    stride = lambda t: 0 if t is None else t.stride(0)
+    rc = _cabi.load().mvb_rotary(_ptr(q), stride(q), _ptr(k), stride(k), _ptr(q_out), stride(q_out), _ptr(k_out), stride(k_out),
+                                 _ptr(positions), _ptr(cos_sin), cos_sin.shape[0], T, heads[0], heads[1], d, cos_sin.shape[1],
+                                 1 if interleaved else 0, _DTYPE[one.dtype], _ptr(status), _stream())
+    _cabi.check(rc, "mvb_rotary")
+    LaunchCounter.add(1 if T else 0)
+    return q_out, k_out
+
+
+@dataclass(frozen=True)
+class KV4Cache:
+    """A layer's keys and values in 4 bits: codes uint8 ``[blocks, kv heads, block_size, D / 2]`` and, per 64 channels of a row, bf16
+    (scale, minimum) ``[blocks, kv heads, block_size, D / 64, 2]``; a code stands for ``minimum + scale * code``.  The order of the
+    codes is the kernels' (``mvb_kv4_cache``); ``kv4_gather`` gives the rows back."""
+    k_codes: torch.Tensor
+    k_affine: torch.Tensor
+    v_codes: torch.Tensor
+    v_affine: torch.Tensor
+
+    def __post_init__(self):
+        shape = self.k_codes.shape
+        _need_shape(len(shape) == 4, "codes must be [blocks, kv heads, block_size, head_dim / 2]")
+        affine = (*shape[:3], shape[3] // 32, 2)
+        for t, want, dtype, name in ((self.k_codes, shape, torch.uint8, "k_codes"), (self.v_codes, shape, torch.uint8, "v_codes"),
+                                     (self.k_affine, affine, torch.bfloat16, "k_affine"), (self.v_affine, affine, torch.bfloat16, "v_affine")):
+            if t.dtype != dtype:
+                raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+            _need_shape(tuple(t.shape) == tuple(want) and t.is_contiguous(), f"{name} must be contiguous {tuple(want)}, got {tuple(t.shape)}")
+
+    @classmethod
+    def empty(cls, num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int, device) -> "KV4Cache":
+        codes = lambda: torch.empty(num_blocks, num_kv_heads, block_size, head_dim // 2, dtype=torch.uint8, device=device)
+        affine = lambda: torch.empty(num_blocks, num_kv_heads, block_size, head_dim // 64, 2, dtype=torch.bfloat16, device=device)
+        return cls(codes(), affine(), codes(), affine())
+
+    @staticmethod
+    def token_bytes(num_kv_heads: int, head_dim: int) -> int:
+        """Bytes of one token's key and value in one layer."""
+        return 2 * num_kv_heads * (head_dim // 2 + head_dim // 64 * 4)
+
+    @property
+    def num_blocks(self) -> int:
+        return self.k_codes.shape[0]
+
+    @property
+    def num_kv_heads(self) -> int:
+        return self.k_codes.shape[1]
+
+    @property
+    def block_size(self) -> int:
+        return self.k_codes.shape[2]
+
+    @property
+    def head_dim(self) -> int:
+        return self.k_codes.shape[3] * 2
+
+    def named(self) -> tuple:
+        return ((self.k_codes, torch.uint8, "k_codes"), (self.k_affine, torch.bfloat16, "k_affine"), (self.v_codes, torch.uint8, "v_codes"),
+                (self.v_affine, torch.bfloat16, "v_affine"))
+
+    def struct(self):
+        """The C argument."""
+        return ctypes.byref(_cabi.KV4Cache(_ptr(self.k_codes), _ptr(self.k_affine), _ptr(self.v_codes), _ptr(self.v_affine), self.num_blocks,
+                                           self.block_size, self.num_kv_heads, self.head_dim))
+
+
+def rotary_kv4_write(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor | None, cos_sin: torch.Tensor | None,
+                     slot_mapping: torch.Tensor, cache: KV4Cache, interleaved: bool = False, q_out: torch.Tensor | None = None,
+                     k_in_place: bool = False, status: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Turns ``q`` (in place or into ``q_out``) and ``k`` as ``rotary`` does, and writes ``k`` and ``v`` in 4 bits to their cache slots
+    (-1: none); ``k_in_place``: the turned k also goes back to ``k``.  ``cos_sin`` None: nothing is turned.  bf16; the rotated channels a
+    multiple of 16.  Returns the turned q."""
+    q_out = q if q_out is None else q_out
+    _need_shape(q is not None or q_out is None, "q_out needs q")
+    _here((k, torch.bfloat16, "k"), (v, torch.bfloat16, "v"), (q, torch.bfloat16, "q"), (q_out, torch.bfloat16, "q_out"),
+          (positions if cos_sin is not None else None, torch.int64, "positions"), (cos_sin, torch.float32, "cos_sin"),
+          (slot_mapping, torch.int32, "slot_mapping"), (status, torch.int32, "status"), *cache.named())
+    T, d = k.shape[0], cache.head_dim
+    for t, heads, name in ((k, cache.num_kv_heads, "k"), (v, cache.num_kv_heads, "v"), (q, None, "q"), (q_out, None, "q_out")):
+        if t is not None:
+            _need_rows(t, name)
+            _need_shape(t.dim() == 3 and t.shape[0] == T and t.shape[2] == d and heads in (None, t.shape[1]),
+                        f"{name} must be [tokens, heads, head_dim] as the cache has them, got {tuple(t.shape)}")
+    _need_shape(q is None or q.shape == q_out.shape, "q_out must have the shape of q")
+    _need_shape(slot_mapping.numel() == T and slot_mapping.is_contiguous(), "slot_mapping must be one contiguous number per token")
+    max_pos = rot = 0
+    if cos_sin is not None:
+        _need_shape(positions is not None and positions.numel() == T and positions.is_contiguous(), "positions must be one contiguous number per token")
+        _need_shape(cos_sin.dim() == 2 and cos_sin.is_contiguous(), "cos_sin must be [positions, rotated channels], contiguous")
+        max_pos, rot = cos_sin.shape
+    rc = _cabi.load().mvb_rotary_kv4_write(
+        _ptr(q), 0 if q is None else q.stride(0), _ptr(q_out), 0 if q is None else q_out.stride(0), _ptr(k), k.stride(0), _ptr(v), v.stride(0),
+        _ptr(positions) if cos_sin is not None else None, _ptr(cos_sin), max_pos, rot, 1 if interleaved else 0, _ptr(slot_mapping),
+        cache.struct(), T, 0 if q is None else q.shape[1], 1 if k_in_place else 0, _ptr(status), _stream())
+    _cabi.check(rc, "mvb_rotary_kv4_write")
+    LaunchCounter.add(1 if T else 0)
+    return q_out
+
+
+def _need_table(block_table: torch.Tensor, rows: int) -> None:
+    _need_shape(block_table.dim() == 2 and block_table.stride(1) == 1 and block_table.shape[0] >= rows and block_table.shape[1] > 0,
+                "block_table must be [sequences, blocks] with neighbouring blocks of a sequence next to each other")
+
+
+def kv4_gather(cache: KV4Cache, cu_seqlens_k: torch.Tensor, block_table: torch.Tensor, num_rows: int, k_out: torch.Tensor | None = None,
+               v_out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The cached contexts of a ragged step as dense bf16 rows ``[num_rows, Hkv, D]``, as ``prefill_attn`` reads them: sequence ``b`` from row
+    ``cu_seqlens_k[b]`` on.  ``num_rows`` is the host's count of them; rows behind the last sequence stay as they are."""
+    _here((cu_seqlens_k, torch.int32, "cu_seqlens_k"), (block_table, torch.int32, "block_table"), (k_out, torch.bfloat16, "k_out"),
+          (v_out, torch.bfloat16, "v_out"), (status, torch.int32, "status"), *cache.named())
+    n = cu_seqlens_k.numel() - 1
+    _need_shape(n >= 0 and cu_seqlens_k.is_contiguous(), "cu_seqlens_k must be [sequences + 1], contiguous")
+    _need_table(block_table, n)
+    shape = (num_rows, cache.num_kv_heads, cache.head_dim)
+    k_out, v_out = (torch.empty(shape, dtype=torch.bfloat16, device=cu_seqlens_k.device) if t is None else t for t in (k_out, v_out))
+    for t, name in ((k_out, "k_out"), (v_out, "v_out")):
+        _need_shape(tuple(t.shape) == shape and t.is_contiguous(), f"{name} must be contiguous {shape}")
+    rc = _cabi.load().mvb_kv4_gather(cache.struct(), _ptr(cu_seqlens_k), _ptr(block_table), block_table.stride(0), block_table.shape[1], n,
+                                     num_rows, _ptr(k_out), _ptr(v_out), _ptr(status), _stream())
+    _cabi.check(rc, "mvb_kv4_gather")
+    LaunchCounter.add(1 if n and num_rows else 0)
+    return k_out, v_out
+
+
+def decode4_workspace(max_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int, device) -> torch.Tensor:
+    """Scratch of ``decode_attn4`` for up to ``max_seqs`` sequences; zeroed here once, calls that share it must not overlap on the GPU."""
+    n = _cabi.load().mvb_decode_attn4_workspace_bytes(max_seqs, num_q_heads, num_kv_heads, head_dim)
+    if n == 0:
+        raise ValueError("bad decode workspace shape")
+    return torch.zeros(n, dtype=torch.uint8, device=device)
+
+
+def decode_attn4(q: torch.Tensor, cache: KV4Cache, cache_seqlens: torch.Tensor, block_table: torch.Tensor, scale: float, window_left: int,
+                 workspace: torch.Tensor, spans: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                 status: torch.Tensor | None = None, softcap: float = 0.0, out_scale: float = 1.0) -> torch.Tensor:
+    """``decode_attn`` over a cache in 4 bits: ``q [B, Hq, D]`` bf16, one new token per sequence.  ``spans`` int32 ``[B, Hkv, budget]``
+    (``kv4_select``): only these spans of 64 tokens are read, each listed once, entries below 0 skipped.  No plan is needed."""
+    _here((q, torch.bfloat16, "q"), (cache_seqlens, torch.int32, "cache_seqlens"), (block_table, torch.int32, "block_table"),
+          (workspace, torch.uint8, "workspace"), (spans, torch.int32, "spans"), (out, torch.bfloat16, "out"), (status, torch.int32, "status"),
+          *cache.named())
+    _need_rows(q, "q")
+    B, hq, d = q.shape
+    _need_shape(d == cache.head_dim, f"q has heads of {d}, the cache of {cache.head_dim}")
+    _need_shape(cache_seqlens.numel() >= B and cache_seqlens.is_contiguous(), "cache_seqlens must be one contiguous number per sequence")
+    _need_table(block_table, B)
+    if spans is not None:
+        _need_shape(spans.dim() == 3 and spans.shape[:2] == (B, cache.num_kv_heads) and spans.is_contiguous(),
+                    "spans must be contiguous [sequences, kv heads, budget]")
+    if out is None:
+        out = torch.empty(B, hq, d, dtype=torch.bfloat16, device=q.device)
+    _need_rows(out, "out")
+    _need_shape(out.shape == q.shape, "out must have the shape of q")
+    rc = _cabi.load().mvb_decode_attn4(
+        _ptr(q), q.stride(0), cache.struct(), _ptr(cache_seqlens), _ptr(block_table), block_table.stride(0), block_table.shape[1], _ptr(spans),
+        0 if spans is None else spans.shape[2], B, hq, float(scale), window_left, float(softcap), float(out_scale), _ptr(out), out.stride(0),
+        _ptr(workspace), workspace.numel(), _ptr(status), _stream())
+    _cabi.check(rc, "mvb_decode_attn4")
+    LaunchCounter.add(1 if B else 0)
+    return out
+
+
+def kv4_summaries(cache: KV4Cache) -> torch.Tensor:
+    """Room for the bounds of every span of the cache's keys (written by ``kv4_summarise``, read by ``kv4_select``)."""
+    return torch.zeros(cache.num_blocks, cache.num_kv_heads, cache.block_size // 64, 2, cache.head_dim, dtype=torch.bfloat16,
+                       device=cache.k_codes.device)
+
+
+def _need_summaries(summaries: torch.Tensor, d: int) -> None:
+    _need_shape(summaries.dim() == 5 and summaries.shape[3:] == (2, d) and summaries.is_contiguous(),
+                "summaries must be contiguous [blocks, kv heads, block_size / 64, 2, head_dim]")
+
+
+def kv4_summarise(cache: KV4Cache, slot_mapping: torch.Tensor, summaries: torch.Tensor, status: torch.Tensor | None = None) -> torch.Tensor:
+    """Renews the bounds of the spans that a step has just written to: per channel the least and the greatest key over the span's rows up to
+    the step's last one.  ``slot_mapping`` as for the write, a sequence's tokens next to each other and in order."""
+    _here((slot_mapping, torch.int32, "slot_mapping"), (summaries, torch.bfloat16, "summaries"), (status, torch.int32, "status"), *cache.named())
+    _need_summaries(summaries, cache.head_dim)
+    _need_shape(summaries.shape[:3] == (cache.num_blocks, cache.num_kv_heads, cache.block_size // 64), "summaries must be those of the cache")
+    _need_shape(slot_mapping.is_contiguous(), "slot_mapping must be contiguous")
+    rc = _cabi.load().mvb_kv4_summarise(cache.struct(), _ptr(slot_mapping), slot_mapping.numel(), _ptr(summaries), _ptr(status), _stream())
+    _cabi.check(rc, "mvb_kv4_summarise")
+    LaunchCounter.add(1 if slot_mapping.numel() else 0)
+    return summaries
+
+
+def kv4_select(q: torch.Tensor, summaries: torch.Tensor, cache_seqlens: torch.Tensor, block_table: torch.Tensor, block_size: int, budget: int,
+               out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """The spans of 64 tokens that ``decode_attn4`` should read: int32 ``[B, Hkv, budget]``, ascending, -1 behind them.  Per sequence and KV
+    head the ``budget`` (at least 2) spans with the greatest bound on ``q . k``, added up over the group's heads; the first and the last
+    span are always among them, and of equal bounds the lower index is taken."""
+    _here((q, torch.bfloat16, "q"), (summaries, torch.bfloat16, "summaries"), (cache_seqlens, torch.int32, "cache_seqlens"),
+          (block_table, torch.int32, "block_table"), (out, torch.int32, "out"), (status, torch.int32, "status"))
+    _need_rows(q, "q")
+    B, hq, d = q.shape
+    _need_summaries(summaries, d)
+    blocks, hkv, per_block = summaries.shape[:3]
+    _need_shape(per_block * 64 == block_size, f"summaries have {per_block} spans a block, blocks have {block_size} tokens")
+    _need_shape(cache_seqlens.numel() >= B and cache_seqlens.is_contiguous(), "cache_seqlens must be one contiguous number per sequence")
+    _need_table(block_table, B)
+    if out is None:
+        out = torch.empty(B, hkv, max(budget, 0), dtype=torch.int32, device=q.device)
+    _need_shape(tuple(out.shape) == (B, hkv, budget) and out.is_contiguous(), "out must be contiguous [sequences, kv heads, budget]")
+    rc = _cabi.load().mvb_kv4_select(_ptr(q), q.stride(0), _ptr(summaries), blocks, block_size, _ptr(cache_seqlens), _ptr(block_table),
+                                     block_table.stride(0), block_table.shape[1], B, hq, hkv, d, budget, _ptr(out), _ptr(status), _stream())
+    _cabi.check(rc, "mvb_kv4_select")
+    LaunchCounter.add(1 if B else 0)
+    return out
