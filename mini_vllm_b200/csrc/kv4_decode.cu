@@ -3,6 +3,24 @@
 //     out = sum_t softmax_t(f(q . k_t scale)) v_t        k_t = m + s c per group of 64 channels, v_t likewise; f the score cap, if any
 //
 // over all tokens of the sequence, the last `window_left` + 1 of them, or the tokens of a list of 64-token spans per sequence and KV head.
+//
+// Nothing is unpacked to values.  With the codes themselves as matrix operands (masked halves of a word are fp16 subnormals, kv4.cuh)
+//     q . k_t  = sum over groups of  s_t (q . c_t) + m_t sum(q)
+//     sum_t p_t v_t = sum over t of  (p_t s_t) c_t  +  sum_t p_t m_t        per group
+// so a 32-bit word of eight codes costs five integer instructions for keys (one shift, four ANDs) and six for values (two tokens of a
+// channel have to meet in a register: a byte permutation more), and scales and minima cost a few per token.  q is brought to [2^14, 2^15)
+// by a power of two per head so that fp16 holds every bf16 exactly down to 2^-29 of the greatest; the channels whose codes sit at bits 4-7
+// (16 times as large) have it divided by 16.  Scores, softmax statistics and outputs are fp32; the weights p s are rounded once, to fp16,
+// an eighth of what bf16 weights would lose.  They never overflow: the softmax's reference is the greatest score + log2(scale), which
+// bounds every p s by 1 (scales below 2^-60 count as that).
+//
+// Bound by memory, on paper 4608 bytes against some 450 warp instructions per 32 tokens of a 128-wide head.  Work is tiles of 32 tokens of
+// one (sequence, head), numbered sequence by sequence and head by head, and cut evenly: each CTA takes a contiguous range, each of its
+// warps a contiguous part of that.  A warp streams its tiles through a private ring in shared memory (cp.async, 16 bytes a lane, placed so
+// that the fragment loads meet no bank twice) and needs no other warp until its range is done.  Rows that lie within one warp's range go
+// straight to the output; parts of a row are put together by the CTA, and where a row crosses CTAs by the one that arrives last.  Every
+// CTA works the split out for itself from the lengths (a scan in shared memory), so there is no plan to make, the grid does not depend on
+// data, and nothing ever waits for another CTA.
 #include "dtype.cuh"
 #include "host_util.cuh"
 #include "kv4.cuh"
@@ -11,11 +29,29 @@
 
 namespace mvb {
 
+constexpr int kDecode4MaxGroup = 8;
+constexpr int kDecode4MaxCtas = 160;
+
+template <int D>
+struct Decode4Cfg {
+  static constexpr int TOK = 32;                             // tokens of a tile
+  static constexpr int NW = D == 256 ? 8 : 16;               // warps of a CTA
+  static constexpr int NST = 3;                              // tiles in a warp's ring
+  static constexpr int CODES = TOK * D / 2, AFF = TOK * D / 16;
+  static constexpr int STAGE = 2 * CODES + 2 * AFF;          // key codes, value codes, key affine, value affine
+  static constexpr int RING = NST * STAGE;
+  static constexpr int GRP = D / 64;                         // groups of channels
+  static constexpr int WK = D / 32, WV = D / 64;             // 32-bit words of a lane: of a key, of a value
+  static constexpr size_t SMEM = static_cast<size_t>(NW) * RING;
+};
+
+__host__ __device__ __forceinline__ constexpr int decode4_part(int group, int d) { return group * d + kDecode4MaxGroup; }   // floats of a part
+
 struct Decode4Params {
   const __nv_bfloat16* q;
   __nv_bfloat16* out;
   int64_t q_stride, out_stride;
-  const uint32_t *k_codes, *v_codes, *k_affine, *v_affine;
+  const uint8_t *k_codes, *v_codes, *k_affine, *v_affine;
   const int32_t* seqlens;
   const int32_t* block_table;
   const int32_t* spans;                // [num_seqs, hkv, budget] or nullptr
@@ -23,98 +59,583 @@ struct Decode4Params {
   FastDiv by_block;
   int table_width, num_seqs, hkv, group, block_size, budget, window_left;
   float scale_log2, cap_in, cap_log2, out_scale;
+  float* parts;                        // [CTAs][NW + 2] parts: a warp's first row, then the CTA's first and last
+  int32_t* arrivals;                   // [num_seqs * hkv], zero between launches
   int* dev_status;
 };
 
-constexpr int kDecode4MaxGroup = 8;
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// A block per (KV head, sequence); a warp walks every eighth token of it, a lane holds D / 32 channels.
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float fast_log2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <int N>
+__device__ __forceinline__ void lds_words(uint32_t addr, uint32_t (&w)[N]) {
+  if constexpr (N == 1) {
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
+  } else if constexpr (N == 2) {
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+  } else {
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
+  }
+}
+
+// Where things lie in a stage.  The rows that the lanes of a fragment read together are 0, 3, 4, 7 or 1, 2, 5, 6 of eight (values) and
+// pairs of one even and one odd row (keys), see decode4_row; 16-byte pieces change places with the row so that these meet in no bank.
+template <int D>
+__device__ __forceinline__ uint32_t key_piece(int t, int piece) {           // byte of a row's 16-byte piece
+  return t * (D / 2) + ((D == 256 ? piece ^ (t & 1) : piece) << 4);
+}
+template <int D>
+__device__ __forceinline__ uint32_t value_piece(int t, int piece) {
+  if (D == 256) return t * 128 + ((piece ^ (t & 6)) << 4);
+  if (D == 128) return t * 64 + ((piece ^ ((t >> 1) & 2)) << 4);
+  return (t ^ ((t >> 1) & 2)) * 32 + (piece << 4);
+}
+// the token (of eight) that stands in row r of a fragment
+__device__ __forceinline__ int decode4_row(int r) { return r ^ ((r >> 1) & 1); }
+
+// The tiles of a (sequence, head) row, one after the other.
+template <int TOK>
+struct Decode4Walk {
+  int b, h, i, count, n;               // tile i of `count` of head h of sequence b, which has n tokens
+  __device__ __forceinline__ static int length(const Decode4Params& p, int b) {
+    const int n = p.seqlens[b], most = p.table_width * p.block_size;
+    return min(n, most);
+  }
+  __device__ __forceinline__ static int first_tile(const Decode4Params& p, int n) {
+    return p.window_left >= 0 ? max(0, n - 1 - p.window_left) / TOK : 0;
+  }
+  __device__ __forceinline__ static int tiles(const Decode4Params& p, int n) {
+    if (n <= 0) return 0;
+    if (p.spans != nullptr) return (kKv4Span / TOK) * min(p.budget, (n + kKv4Span - 1) / kKv4Span);
+    return (n + TOK - 1) / TOK - first_tile(p, n);
+  }
+  __device__ __forceinline__ void next(const Decode4Params& p) {
+    if (++i < count) return;
+    i = 0;
+    if (++h < p.hkv) return;
+    h = 0;
+    do {
+      if (++b >= p.num_seqs) { count = 0x7fffffff; n = 0; return; }         // past the last row: nobody reads on
+      n = length(p, b);
+      count = tiles(p, n);
+    } while (count == 0);
+  }
+  // the first token of the tile, -1: none
+  __device__ __forceinline__ int token(const Decode4Params& p) const {
+    if (p.spans == nullptr) return (first_tile(p, n) + i) * TOK;
+    constexpr int per = kKv4Span / TOK;
+    const int span = p.spans[(static_cast<int64_t>(b) * p.hkv + h) * p.budget + i / per];
+    if (span < 0) return -1;
+    if (span > (n - 1) / kKv4Span) return -2;
+    const int t = span * kKv4Span + (i % per) * TOK;
+    return t < n ? t : -1;
+  }
+};
+
 template <int D, bool CAP>
-__global__ void __launch_bounds__(256) kv4_decode_kernel(const Decode4Params p) {
-  constexpr uint32_t FULL = 0xffffffffu;
-  constexpr int W = D / 8, G = kDecode4MaxGroup, CPL = D / 32;
-  extern __shared__ float sh[];                              // [8 warps][G][D + 2]
-  const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int n = p.seqlens[b];
-  float q[G][CPL], o[G][CPL], m[G], l[G];
+__global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(const Decode4Params p) {
+  using C = Decode4Cfg<D>;
+  using Walk = Decode4Walk<C::TOK>;
+  constexpr int NW = C::NW, NT = NW * 32, NST = C::NST, GRP = C::GRP;
+  constexpr uint32_t FULL = 0xffffffffu, LO = 0x000f000fu, HI = 0x00f000f0u;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int scan_s[NW];
+  __shared__ int info_s[NW][NST];                            // first token of the tile in a stage, -1: nothing to read
+  __shared__ int meta_s[NW][2][3];                           // a warp's parts: row (-1: none), the row's first tile and the one behind its last
+  __shared__ int last_s;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c4 = lane & 3;
+  const int G = p.group;
+
+  // ---- the split: a prefix sum of the tile counts in the memory that will be the ring ------------------------------------------------
+  int* prefix = reinterpret_cast<int*>(smem);
+  int running = 0;
+  for (int base = 0; base < p.num_seqs; base += NT) {
+    const int b = base + threadIdx.x;
+    int v = 0;
+    if (b < p.num_seqs) {
+      const int n = p.seqlens[b];
+      if (n > p.table_width * p.block_size) report(p.dev_status, kDevBadLength, b);
+      v = Walk::tiles(p, Walk::length(p, b));
+    }
+    int x = v;
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
-    m[g] = -INFINITY; l[g] = 0.f;
+    for (int off = 1; off < 32; off <<= 1) {
+      const int y = __shfl_up_sync(FULL, x, off);
+      if (lane >= off) x += y;
+    }
+    if (lane == 31) scan_s[warp] = x;
+    __syncthreads();
+    int before = running;
 #pragma unroll
-    for (int e = 0; e < CPL; ++e) {
-      q[g][e] = g < p.group ? __bfloat162float(p.q[b * p.q_stride + (static_cast<int64_t>(h) * p.group + g) * D + lane * CPL + e]) : 0.f;
-      o[g][e] = 0.f;
+    for (int w = 0; w < NW; ++w) {
+      const int s = scan_s[w];
+      before += w < warp ? s : 0;
+      running += s;
+    }
+    if (b < p.num_seqs) prefix[b] = before + x - v;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) prefix[p.num_seqs] = running;
+  const int64_t total = static_cast<int64_t>(running) * p.hkv;
+  // no more CTAs than give every warp a tile: rows of a small call stay on few of them
+  const int64_t ctas = min(static_cast<int64_t>(gridDim.x), (total + NW - 1) / NW);
+  const int cta = blockIdx.x;
+  auto cta_start = [&](int64_t c) -> int { return static_cast<int>(c * total / ctas); };
+  // rows without a token: zeros
+  for (int b = cta; b < p.num_seqs; b += gridDim.x) {
+    if (p.seqlens[b] <= 0) {
+      for (int e = threadIdx.x; e < p.hkv * G * D / 8; e += NT)
+        *reinterpret_cast<uint4*>(p.out + b * p.out_stride + e * 8) = make_uint4(0, 0, 0, 0);
     }
   }
-  const int32_t* list = p.spans != nullptr ? p.spans + (static_cast<int64_t>(b) * p.hkv + h) * p.budget : nullptr;
-  const int first = list == nullptr && p.window_left >= 0 ? max(0, n - 1 - p.window_left) : 0;
-  const int steps = list != nullptr ? p.budget * kKv4Span : n;
-  for (int i = first + warp; i < steps; i += 8) {
-    int t = i;
-    if (list != nullptr) {
-      const int span = list[i / kKv4Span];
-      if (span < 0 || span > (n - 1) / kKv4Span) continue;
-      t = span * kKv4Span + i % kKv4Span;
-      if (t >= n) continue;
-    }
-    const int col = p.by_block.div(t);
-    const int64_t block = col < p.table_width ? p.block_table[b * p.table_stride + col] : -1;
-    if (block < 0 || block >= p.num_blocks) {
-      if (lane == 0) report(p.dev_status, kDevBadBlock, b);
-      continue;
-    }
-    const int64_t row = kv4_row(block, p.hkv, h, p.block_size, t - col * p.block_size);
-    float k[CPL], v[CPL];
-    const int L = lane * CPL / 8, e0 = lane * CPL % 8;
-    const uint32_t kw = p.k_codes[row * W + kv4_word<D>(L, true)], vw = p.v_codes[row * W + kv4_word<D>(L, false)];
-    const uint32_t ka = p.k_affine[row * (D / 64) + L / 8], va = p.v_affine[row * (D / 64) + L / 8];
-#pragma unroll
-    for (int e = 0; e < CPL; ++e) {
-      k[e] = fmaf(kv4_scale(ka), static_cast<float>((kw >> kv4_shift(e0 + e)) & 15u), kv4_min(ka));
-      v[e] = fmaf(kv4_scale(va), static_cast<float>((vw >> kv4_shift(e0 + e)) & 15u), kv4_min(va));
-    }
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      if (g >= p.group) continue;
-      float s = 0.f;
-#pragma unroll
-      for (int e = 0; e < CPL; ++e) s = fmaf(q[g][e], k[e], s);
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(FULL, s, off);
-      const float x = CAP ? p.cap_log2 * tanhf(s * p.cap_in) : s * p.scale_log2;
-      const float nm = fmaxf(m[g], x), a = exp2f(m[g] - nm), w = exp2f(x - nm);
-      m[g] = nm;
-      l[g] = l[g] * a + w;
-#pragma unroll
-      for (int e = 0; e < CPL; ++e) o[g][e] = o[g][e] * a + w * v[e];
-    }
-  }
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    float* at = sh + (warp * G + g) * (D + 2);
-#pragma unroll
-    for (int e = 0; e < CPL; ++e) at[lane * CPL + e] = o[g][e];
-    if (lane == 0) { at[D] = m[g]; at[D + 1] = l[g]; }
-  }
+  if (cta >= ctas) return;
+  const int t0 = cta_start(cta), t1 = cta_start(cta + 1);
+  const int w0 = t0 + static_cast<int>(static_cast<int64_t>(warp) * (t1 - t0) / NW);
+  const int w1 = t0 + static_cast<int>(static_cast<int64_t>(warp + 1) * (t1 - t0) / NW);
   __syncthreads();
-  for (int i = threadIdx.x; i < p.group * D; i += 256) {
-    const int g = i / D, e = i % D;
-    float M = -INFINITY, L = 0.f, O = 0.f;
-    for (int w = 0; w < 8; ++w) M = fmaxf(M, sh[(w * G + g) * (D + 2) + D]);
-    for (int w = 0; w < 8; ++w) {
-      const float* at = sh + (w * G + g) * (D + 2);
-      const float f = at[D] == -INFINITY ? 0.f : exp2f(at[D] - M);
-      L += f * at[D + 1]; O += f * at[e];
+  Walk cs;
+  int row_t0 = 0;                                            // the number of the row's first tile
+  {
+    int lo = 0, hi = p.num_seqs;                             // the last b with prefix[b] * hkv <= w0
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (static_cast<int64_t>(prefix[mid]) * p.hkv <= w0) lo = mid; else hi = mid;
     }
-    p.out[b * p.out_stride + (static_cast<int64_t>(h) * p.group + g) * D + e] = __float2bfloat16_rn(L > 0.f ? O / L * p.out_scale : 0.f);
+    cs.b = lo;
+    cs.n = Walk::length(p, lo);
+    cs.count = prefix[lo + 1] - prefix[lo];
+    const int in_seq = w0 - prefix[lo] * p.hkv;
+    cs.h = cs.count > 0 ? in_seq / cs.count : 0;
+    cs.i = in_seq - cs.h * cs.count;
+    row_t0 = w0 - cs.i;
   }
+  if (lane < 2) meta_s[warp][lane][0] = -1;
+  __syncthreads();                                           // the prefix sums have been read: the ring may be filled
+
+  // ---- the fetching side ------------------------------------------------------------------------------------------------------------
+  const uint32_t ring = smem_u32(smem) + warp * C::RING;
+  Walk fs = cs;
+  int ft = w0;                                               // the next tile to fetch
+  int f_token = -1, f_block = -1;
+  auto look = [&]() {                                        // first token and block of the tile that is fetched next
+    f_token = -1;
+    if (ft >= w1) return;
+    f_token = fs.token(p);
+    if (f_token >= 0) f_block = p.block_table[fs.b * p.table_stride + p.by_block.div(f_token)];
+  };
+  int f_stage = 0;
+  auto fetch = [&]() {
+    if (ft < w1) {
+      bool ok = f_token >= 0;
+      if (ok && (f_block < 0 || f_block >= p.num_blocks)) {
+        if (lane == 0) report(p.dev_status, kDevBadBlock, fs.b);
+        ok = false;
+      }
+      if (f_token == -2 && lane == 0) report(p.dev_status, kDevBadLength, fs.b);
+      if (lane == 0) info_s[warp][f_stage] = ok ? f_token : -1;
+      if (ok) {
+        const int in_block = f_token - static_cast<int>(p.by_block.div(f_token)) * p.block_size;
+        const int64_t row = kv4_row(f_block, p.hkv, fs.h, p.block_size, in_block);
+        const uint8_t* k = p.k_codes + row * (D / 2);
+        const uint8_t* v = p.v_codes + row * (D / 2);
+        const uint32_t dst = ring + f_stage * C::STAGE;
+        constexpr int PPR = D / 32;                          // 16-byte pieces of a row
+#pragma unroll
+        for (int i = 0; i < C::TOK * PPR / 32; ++i) {
+          const int at = i * 32 + lane, t = at / PPR, piece = at % PPR;
+          cp_async16(dst + key_piece<D>(t, piece), k + at * 16);
+          cp_async16(dst + C::CODES + value_piece<D>(t, piece), v + at * 16);
+        }
+        const uint8_t* ka = p.k_affine + row * (D / 16);
+        const uint8_t* va = p.v_affine + row * (D / 16);
+        if constexpr (C::AFF / 16 >= 32) {
+          cp_async16(dst + 2 * C::CODES + lane * 16, ka + lane * 16);
+          cp_async16(dst + 2 * C::CODES + C::AFF + lane * 16, va + lane * 16);
+        } else {
+          constexpr int PA = C::AFF / 16;
+          if (lane < 2 * PA) cp_async16(dst + 2 * C::CODES + lane * 16, lane < PA ? ka + lane * 16 : va + (lane - PA) * 16);
+        }
+      }
+      ++ft;
+      fs.next(p);
+      f_stage = f_stage + 1 == NST ? 0 : f_stage + 1;
+      look();
+    }
+    cp_async_commit();
+  };
+  look();
+#pragma unroll
+  for (int i = 0; i < NST - 1; ++i) fetch();
+
+  // ---- the computing side -----------------------------------------------------------------------------------------------------------
+  const int kt = decode4_row(g);                             // this lane's token of eight, in the roles of a key's row and of a score's
+  const int vt0 = decode4_row(2 * c4), vt1 = decode4_row(2 * c4 + 1);
+  int t = w0, stage = 0;
+  while (t < w1) {
+    const int row_t1 = row_t0 + cs.count, seg_end = min(w1, row_t1);
+    const int b = cs.b, h = cs.h, n = cs.n;
+    const int start = p.window_left >= 0 ? max(0, n - 1 - p.window_left) : 0;
+
+    // q as the B operand (head g of the group in column g): word j of a lane is channels 8 (4 j + c4) ..
+    uint32_t qf[C::WK][4];
+    float qs_a[GRP], qs_b[GRP], f_a, f_b;                    // sums per group and the score's factor, of heads 2 c4 and 2 c4 + 1
+    {
+      uint4 w[C::WK];
+#pragma unroll
+      for (int j = 0; j < C::WK; ++j) {
+        w[j] = make_uint4(0, 0, 0, 0);
+        if (g < G) w[j] = *reinterpret_cast<const uint4*>(p.q + b * p.q_stride + (static_cast<int64_t>(h) * G + g) * D + 8 * (4 * j + c4));
+      }
+      float most = 0.f;
+#pragma unroll
+      for (int j = 0; j < C::WK; ++j) {
+        const uint32_t a[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = fmaxf(most, fmaxf(fabsf(bf16_lo(a[e])), fabsf(bf16_hi(a[e]))));
+      }
+      most = fmaxf(most, __shfl_xor_sync(FULL, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(FULL, most, 2));
+      const int ex = static_cast<int>(__float_as_uint(most) >> 23) - 127;
+      const int up = min(14 - ex, 126);
+      const float grow = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+      float sum[GRP];
+#pragma unroll
+      for (int j = 0; j < GRP; ++j) sum[j] = 0.f;
+#pragma unroll
+      for (int j = 0; j < C::WK; ++j) {
+        const uint32_t a[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = bf16_lo(a[e]) * grow, y = bf16_hi(a[e]) * grow;
+          sum[j / 2] += x + y;
+          const float less = (e & 1) ? 0.0625f : 1.f;        // their codes sit at bits 4-7
+          qf[j][e] = pack_f16(x * less, y * less);
+        }
+      }
+      const float f = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(min(127 + 24 - up, 254)) << 23);
+#pragma unroll
+      for (int j = 0; j < GRP; ++j) {
+        sum[j] += __shfl_xor_sync(FULL, sum[j], 1);
+        sum[j] += __shfl_xor_sync(FULL, sum[j], 2);
+        sum[j] *= 0x1p-24f;
+        qs_a[j] = __shfl_sync(FULL, sum[j], 8 * c4);
+        qs_b[j] = __shfl_sync(FULL, sum[j], 8 * c4 + 4);
+      }
+      f_a = __shfl_sync(FULL, f, 8 * c4);
+      f_b = __shfl_sync(FULL, f, 8 * c4 + 4);
+    }
+    float o[4 * C::WV][4], l_a = 0.f, l_b = 0.f, m_a = -INFINITY, m_b = -INFINITY, pm_a[GRP], pm_b[GRP];
+#pragma unroll
+    for (int i = 0; i < 4 * C::WV; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+#pragma unroll
+    for (int j = 0; j < GRP; ++j) pm_a[j] = pm_b[j] = 0.f;
+
+    for (; t < seg_end; ++t) {
+      cp_async_wait<NST - 2>();
+      __syncwarp();                                          // the tile is there for every lane, and the one before has been read by all
+      fetch();
+      const int token0 = info_s[warp][stage];
+      const uint32_t at = ring + stage * C::STAGE;
+      stage = stage + 1 == NST ? 0 : stage + 1;
+      if (token0 < 0) continue;
+
+      // ---- scores: rows are tokens, columns heads -------------------------------------------------------------------------------
+      float x[2][4];
+      uint32_t va[2][2][GRP];                                // (scale, minimum) of this lane's tokens: [16 tokens][upper eight][group]
+      const bool whole = token0 >= start && token0 + C::TOK <= n;
+      float ta = -INFINITY, tb = -INFINITY;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        float acc[GRP][4];
+#pragma unroll
+        for (int j = 0; j < GRP; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+        uint32_t k0[C::WK], k1[C::WK];
+        const int r0 = 16 * s + kt, r1 = r0 + 8;
+        if constexpr (D == 64) {
+          lds_words<2>(at + r0 * 32 + c4 * 8, k0);
+          lds_words<2>(at + r1 * 32 + c4 * 8, k1);
+        } else {
+#pragma unroll
+          for (int i = 0; i < C::WK / 4; ++i) {
+            uint32_t u[4];
+            lds_words<4>(at + key_piece<D>(r0, c4 * (C::WK / 4) + i), u);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) k0[4 * i + e] = u[e];
+            lds_words<4>(at + key_piece<D>(r1, c4 * (C::WK / 4) + i), u);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) k1[4 * i + e] = u[e];
+          }
+        }
+        uint32_t ka0[GRP], ka1[GRP];
+        lds_words<GRP>(at + 2 * C::CODES + r0 * (D / 16), ka0);
+        lds_words<GRP>(at + 2 * C::CODES + r1 * (D / 16), ka1);
+        lds_words<GRP>(at + 2 * C::CODES + C::AFF + r0 * (D / 16), va[s][0]);
+        lds_words<GRP>(at + 2 * C::CODES + C::AFF + r1 * (D / 16), va[s][1]);
+#pragma unroll
+        for (int j = 0; j < C::WK; ++j) {
+          const uint32_t u = k0[j], w = k1[j], u8 = u >> 8, w8 = w >> 8;
+          mma_f16_16816(acc[j / 2], u & LO, w & LO, u & HI, w & HI, qf[j][0], qf[j][1]);
+          mma_f16_16816(acc[j / 2], u8 & LO, w8 & LO, u8 & HI, w8 & HI, qf[j][2], qf[j][3]);
+        }
+        x[s][0] = x[s][1] = x[s][2] = x[s][3] = 0.f;
+#pragma unroll
+        for (int j = 0; j < GRP; ++j) {
+          const float s0 = kv4_scale(ka0[j]), s1 = kv4_scale(ka1[j]), m0 = kv4_min(ka0[j]), m1 = kv4_min(ka1[j]);
+          x[s][0] = fmaf(s0, acc[j][0], fmaf(m0, qs_a[j], x[s][0]));
+          x[s][1] = fmaf(s0, acc[j][1], fmaf(m0, qs_b[j], x[s][1]));
+          x[s][2] = fmaf(s1, acc[j][2], fmaf(m1, qs_a[j], x[s][2]));
+          x[s][3] = fmaf(s1, acc[j][3], fmaf(m1, qs_b[j], x[s][3]));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[s][i] *= (i & 1) ? f_b : f_a;
+          if constexpr (CAP) x[s][i] = fmaf(-2.f * p.cap_log2, fast_rcp(1.f + fast_exp2(x[s][i] * p.cap_in)), p.cap_log2);
+        }
+        if (!whole) {                                        // tokens out of sight: no weight, whatever their rows hold
+          const int j0 = token0 + r0, j1 = token0 + r1;
+          if (j0 < start || j0 >= n) {
+            x[s][0] = x[s][1] = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < GRP; ++j) va[s][0][j] = 0u;
+          }
+          if (j1 < start || j1 >= n) {
+            x[s][2] = x[s][3] = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < GRP; ++j) va[s][1][j] = 0u;
+          }
+        }
+        float big0 = 0x1p-60f, big1 = 0x1p-60f;
+#pragma unroll
+        for (int j = 0; j < GRP; ++j) { big0 = fmaxf(big0, kv4_scale(va[s][0][j])); big1 = fmaxf(big1, kv4_scale(va[s][1][j])); }
+        big0 = fast_log2(big0); big1 = fast_log2(big1);
+        ta = fmaxf(ta, fmaxf(x[s][0] + big0, x[s][2] + big1));
+        tb = fmaxf(tb, fmaxf(x[s][1] + big0, x[s][3] + big1));
+      }
+      // ---- the running reference and sum ------------------------------------------------------------------------------------------
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) {
+        ta = fmaxf(ta, __shfl_xor_sync(FULL, ta, off));
+        tb = fmaxf(tb, __shfl_xor_sync(FULL, tb, off));
+      }
+      const float na = fmaxf(m_a, ta), nb = fmaxf(m_b, tb);
+      const float ra = na == -INFINITY ? 0.f : na, rb = nb == -INFINITY ? 0.f : nb;
+      if (__any_sync(FULL, na != m_a || nb != m_b)) {
+        const float alpha_a = fast_exp2(m_a - ra), alpha_b = fast_exp2(m_b - rb);
+        l_a *= alpha_a; l_b *= alpha_b;
+#pragma unroll
+        for (int j = 0; j < GRP; ++j) { pm_a[j] *= alpha_a; pm_b[j] *= alpha_b; }
+#pragma unroll
+        for (int i = 0; i < 4 * C::WV; ++i) { o[i][0] *= alpha_a; o[i][1] *= alpha_b; o[i][2] *= alpha_a; o[i][3] *= alpha_b; }
+        m_a = na; m_b = nb;
+      }
+      // ---- weights: transposed, as the B operand of the values --------------------------------------------------------------------
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const float p0 = fast_exp2(x[s][0] - ra), p1 = fast_exp2(x[s][1] - rb), p2 = fast_exp2(x[s][2] - ra), p3 = fast_exp2(x[s][3] - rb);
+        l_a += p0 + p2; l_b += p1 + p3;
+        uint32_t v00[C::WV], v01[C::WV], v10[C::WV], v11[C::WV];
+        const int u0 = 16 * s + vt0, u1 = 16 * s + vt1;
+        const uint32_t vat = at + C::CODES;
+        auto value = [&](int tok, uint32_t (&w)[C::WV]) {
+          if constexpr (D == 256) lds_words<4>(vat + value_piece<D>(tok, g), w);
+          else lds_words<C::WV>(vat + value_piece<D>(tok, D == 128 ? g >> 1 : g >> 2) + (D == 128 ? (g & 1) * 8 : (g & 3) * 4), w);
+        };
+        value(u0, v00); value(u1, v01); value(u0 + 8, v10); value(u1 + 8, v11);
+#pragma unroll
+        for (int j = 0; j < GRP; ++j) {
+          const float s0 = kv4_scale(va[s][0][j]), s1 = kv4_scale(va[s][1][j]), m0 = kv4_min(va[s][0][j]), m1 = kv4_min(va[s][1][j]);
+          pm_a[j] = fmaf(p0, m0, fmaf(p2, m1, pm_a[j]));
+          pm_b[j] = fmaf(p1, m0, fmaf(p3, m1, pm_b[j]));
+          const uint32_t b0 = movmatrix_trans(pack_f16(p0 * s0, p1 * s0)), b1 = movmatrix_trans(pack_f16(p2 * s1, p3 * s1));
+          const uint32_t xl = __byte_perm(v00[j], v01[j], 0x5410), yl = __byte_perm(v00[j], v01[j], 0x7632);
+          const uint32_t xh = __byte_perm(v10[j], v11[j], 0x5410), yh = __byte_perm(v10[j], v11[j], 0x7632);
+          mma_f16_16816(o[4 * j], xl & LO, yl & LO, xh & LO, yh & LO, b0, b1);
+          mma_f16_16816(o[4 * j + 1], xl & HI, yl & HI, xh & HI, yh & HI, b0, b1);
+          const uint32_t xl8 = xl >> 8, yl8 = yl >> 8, xh8 = xh >> 8, yh8 = yh >> 8;
+          mma_f16_16816(o[4 * j + 2], xl8 & LO, yl8 & LO, xh8 & LO, yh8 & LO, b0, b1);
+          mma_f16_16816(o[4 * j + 3], xl8 & HI, yl8 & HI, xh8 & HI, yh8 & HI, b0, b1);
+        }
+      }
+    }
+
+    // ---- the end of the row, or of this warp's part of it ---------------------------------------------------------------------------
+#pragma unroll
+    for (int off = 4; off < 32; off <<= 1) {
+      l_a += __shfl_xor_sync(FULL, l_a, off);
+      l_b += __shfl_xor_sync(FULL, l_b, off);
+#pragma unroll
+      for (int j = 0; j < GRP; ++j) {
+        pm_a[j] += __shfl_xor_sync(FULL, pm_a[j], off);
+        pm_b[j] += __shfl_xor_sync(FULL, pm_b[j], off);
+      }
+    }
+    const bool complete = row_t0 >= w0 && row_t1 <= w1;
+    float* part = nullptr;
+    if (!complete) {
+      // the warp's last part can take the place of its ring, an earlier one (its first row's end) goes to the workspace
+      if (seg_end == w1) {
+        cp_async_wait<0>();
+        __syncwarp();
+        part = reinterpret_cast<float*>(smem + warp * C::RING);
+      } else {
+        part = p.parts + (static_cast<int64_t>(cta) * (NW + 2) + warp) * decode4_part(G, D);
+      }
+      if (lane == 0) {
+        const int slot = seg_end == w1 ? 1 : 0;
+        meta_s[warp][slot][0] = b * p.hkv + h;
+        meta_s[warp][slot][1] = row_t0;
+        meta_s[warp][slot][2] = row_t1;
+      }
+    }
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      const int head = 2 * c4 + side;
+      if (head >= G) continue;
+      const float l = side ? l_b : l_a, m = side ? m_b : m_a;
+      const float inv = l > 0.f ? (complete ? p.out_scale : 1.f) / l : 0.f;
+#pragma unroll
+      for (int j = 0; j < C::WV; ++j) {
+        float y[8];                                          // channels 64 j + 8 g ..: rows g (even) and g + 8 (odd) of four tiles
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float unit = (i & 1) ? 0x1p20f : 0x1p24f, add = side ? pm_b[j] : pm_a[j];
+          y[2 * i] = fmaf(o[4 * j + i][side], unit, add) * inv;
+          y[2 * i + 1] = fmaf(o[4 * j + i][2 + side], unit, add) * inv;
+        }
+        if (complete) store_vec<__nv_bfloat16, 8>(p.out + b * p.out_stride + (static_cast<int64_t>(h) * G + head) * D + 64 * j + 8 * g, y);
+        else store_f32<8>(part + head * D + 64 * j + 8 * g, y);
+      }
+      if (!complete && g == 0) part[G * D + head] = l > 0.f ? m + fast_log2(l) : -INFINITY;
+    }
+    // on to the next row
+    if (t < w1) {
+      cs.i = cs.count - 1;
+      cs.next(p);
+      row_t0 = row_t1;
+    }
+  }
+  cp_async_wait<0>();
+  __syncthreads();
+
+  // ---- parts of rows, put together by the CTA: neighbouring parts of one row are one run ------------------------------------------------
+  auto part_of = [&](int slot) -> const float* {             // slot = 2 * warp + (0: first row, 1: last row)
+    const int w = slot >> 1;
+    return (slot & 1) ? reinterpret_cast<const float*>(smem + w * C::RING) : p.parts + (static_cast<int64_t>(cta) * (NW + 2) + w) * decode4_part(G, D);
+  };
+  const int* meta = &meta_s[0][0][0];
+  for (int slot = 0; slot < 2 * NW;) {
+    const int row = meta[slot * 3];
+    if (row < 0) { ++slot; continue; }
+    int end = slot + 1;
+    while (end < 2 * NW && (meta[end * 3] < 0 || meta[end * 3] == row)) ++end;
+    const int r0 = meta[slot * 3 + 1], r1 = meta[slot * 3 + 2];
+    const bool complete = r0 >= t0 && r1 <= t1;
+    const int b = row / p.hkv, h = row - b * p.hkv;
+    float* mine = p.parts + (static_cast<int64_t>(cta) * (NW + 2) + NW + (r0 <= t0 ? 0 : 1)) * decode4_part(G, D);
+    for (int e = threadIdx.x; e < G * D / 4; e += NT) {
+      const int head = e * 4 / D;
+      float M = -INFINITY;
+      for (int s = slot; s < end; ++s)
+        if (meta[s * 3] >= 0) M = fmaxf(M, part_of(s)[G * D + head]);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float sum = 0.f;
+      for (int s = slot; s < end; ++s) {
+        if (meta[s * 3] < 0) continue;
+        const float* from = part_of(s);
+        const float w = M == -INFINITY ? 0.f : fast_exp2(from[G * D + head] - M);
+        const float4 v = *reinterpret_cast<const float4*>(from + e * 4);
+        acc.x = fmaf(w, v.x, acc.x); acc.y = fmaf(w, v.y, acc.y); acc.z = fmaf(w, v.z, acc.z); acc.w = fmaf(w, v.w, acc.w);
+        sum += w;
+      }
+      const float inv = sum > 0.f ? (complete ? p.out_scale : 1.f) / sum : 0.f;
+      acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
+      if (complete) {
+        *reinterpret_cast<uint2*>(p.out + b * p.out_stride + static_cast<int64_t>(h) * G * D + e * 4) =
+            make_uint2(pack_bf16(acc.x, acc.y), pack_bf16(acc.z, acc.w));
+      } else {
+        *reinterpret_cast<float4*>(mine + e * 4) = acc;
+        if ((e * 4) % D == 0) mine[G * D + head] = sum > 0.f ? M + fast_log2(sum) : -INFINITY;
+      }
+    }
+    if (!complete) {
+      // the row's other CTAs: whoever arrives last finds every part in memory
+      const int c1 = static_cast<int>(((static_cast<int64_t>(r0) + 1) * ctas - 1) / total);
+      const int c2 = static_cast<int>((static_cast<int64_t>(r1) * ctas - 1) / total);
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        int prev;
+        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(prev) : "l"(p.arrivals + row) : "memory");
+        last_s = prev == c2 - c1;
+        if (last_s) p.arrivals[row] = 0;                     // as the next launch expects it
+      }
+      __syncthreads();
+      if (last_s) {
+        const float* first = p.parts + (static_cast<int64_t>(c1) * (NW + 2) + NW + (r0 <= cta_start(c1) ? 0 : 1)) * decode4_part(G, D);
+        auto other = [&](int c) -> const float* {
+          return c == c1 ? first : p.parts + (static_cast<int64_t>(c) * (NW + 2) + NW) * decode4_part(G, D);
+        };
+        for (int e = threadIdx.x; e < G * D / 4; e += NT) {
+          const int head = e * 4 / D;
+          float M = -INFINITY;
+          for (int c = c1; c <= c2; ++c) M = fmaxf(M, __ldcg(other(c) + G * D + head));
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          float sum = 0.f;
+#pragma unroll 4
+          for (int c = c1; c <= c2; ++c) {
+            const float* from = other(c);
+            const float w = M == -INFINITY ? 0.f : fast_exp2(__ldcg(from + G * D + head) - M);
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(from + e * 4));
+            acc.x = fmaf(w, v.x, acc.x); acc.y = fmaf(w, v.y, acc.y); acc.z = fmaf(w, v.z, acc.z); acc.w = fmaf(w, v.w, acc.w);
+            sum += w;
+          }
+          const float inv = sum > 0.f ? p.out_scale / sum : 0.f;
+          *reinterpret_cast<uint2*>(p.out + b * p.out_stride + static_cast<int64_t>(h) * G * D + e * 4) =
+              make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+        }
+      }
+      __syncthreads();
+    }
+    slot = end;
+  }
+}
+
+struct Decode4Layout {
+  size_t parts, arrivals, total;
+};
+static Decode4Layout decode4_layout(int64_t seqs, int hkv, int group, int d) {
+  const int nw = d == 256 ? Decode4Cfg<256>::NW : Decode4Cfg<128>::NW;
+  Decode4Layout l;
+  l.parts = 0;
+  l.arrivals = (sizeof(float) * kDecode4MaxCtas * (nw + 2) * decode4_part(group, d) + 255) / 256 * 256;
+  l.total = l.arrivals + (sizeof(int32_t) * static_cast<size_t>(seqs) * hkv + 255) / 256 * 256;
+  return l;
 }
 
 }  // namespace mvb
 
 extern "C" size_t mvb_decode_attn4_workspace_bytes(int max_seqs, int num_q_heads, int num_kv_heads, int head_dim) {
-  if (max_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0) return 0;
-  return 256;
+  if (max_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || num_q_heads % num_kv_heads != 0) return 0;
+  return mvb::decode4_layout(max_seqs, num_kv_heads, num_q_heads / num_kv_heads, head_dim).total;
 }
 
 extern "C" int mvb_decode_attn4(const void* q, int64_t q_row_stride, const mvb_kv4_cache* cache, const int32_t* cache_seqlens,
@@ -126,31 +647,40 @@ extern "C" int mvb_decode_attn4(const void* q, int64_t q_row_stride, const mvb_k
   if (rc != kOk) return rc;
   if (num_seqs < 0 || num_q_heads <= 0 || table_width <= 0 || table_stride < table_width || !(softcap >= 0.f)) return kInvalidArgument;
   if (spans != nullptr && (budget <= 0 || window_left >= 0)) return kInvalidArgument;
-  if (num_q_heads % cache->num_kv_heads != 0 || num_q_heads / cache->num_kv_heads > kDecode4MaxGroup) return kUnsupportedShape;
+  const int hkv = cache->num_kv_heads;
+  if (num_q_heads % hkv != 0 || num_q_heads / hkv > kDecode4MaxGroup) return kUnsupportedShape;
   if (num_seqs == 0) return kOk;
   if (!q || !out || !cache_seqlens || !block_table || !workspace) return kInvalidArgument;
   if (q_row_stride % 8 || out_row_stride % 8 || !is_aligned(q, 16) || !is_aligned(out, 16) || !is_aligned(workspace, 256)) return kMisaligned;
-  if (num_seqs > 65535) return kUnsupportedShape;
-  (void)workspace_bytes;
+  // lengths and tile numbers are 32-bit; the prefix sums of the lengths have the ring's room
+  if (static_cast<int64_t>(table_width) * cache->block_size > 0x7fffffffLL || num_seqs > 16384) return kUnsupportedShape;
+  if (static_cast<double>(num_seqs) * hkv * table_width * (cache->block_size / 32) > 2147483000.0) return kUnsupportedShape;
+  const Decode4Layout l = decode4_layout(num_seqs, hkv, num_q_heads / hkv, cache->head_dim);
+  if (workspace_bytes < l.total) return kScratchTooSmall;
   const float kLog2e = 1.4426950408889634f;
   Decode4Params p;
   p.q = static_cast<const __nv_bfloat16*>(q); p.q_stride = q_row_stride; p.out = static_cast<__nv_bfloat16*>(out); p.out_stride = out_row_stride;
-  p.k_codes = static_cast<const uint32_t*>(cache->k_codes); p.v_codes = static_cast<const uint32_t*>(cache->v_codes);
-  p.k_affine = static_cast<const uint32_t*>(cache->k_affine); p.v_affine = static_cast<const uint32_t*>(cache->v_affine);
+  p.k_codes = static_cast<const uint8_t*>(cache->k_codes); p.v_codes = static_cast<const uint8_t*>(cache->v_codes);
+  p.k_affine = static_cast<const uint8_t*>(cache->k_affine); p.v_affine = static_cast<const uint8_t*>(cache->v_affine);
   p.seqlens = cache_seqlens; p.block_table = block_table; p.table_stride = table_stride; p.table_width = table_width; p.spans = spans;
   p.num_blocks = cache->num_blocks; p.by_block = FastDiv(static_cast<uint32_t>(cache->block_size));
-  p.num_seqs = num_seqs; p.hkv = cache->num_kv_heads; p.group = num_q_heads / cache->num_kv_heads; p.block_size = cache->block_size;
+  p.num_seqs = num_seqs; p.hkv = hkv; p.group = num_q_heads / hkv; p.block_size = cache->block_size;
   p.budget = budget; p.window_left = window_left;
-  p.scale_log2 = scale * kLog2e; p.cap_in = softcap > 0.f ? scale / softcap : 0.f; p.cap_log2 = softcap * kLog2e; p.out_scale = out_scale;
+  // with a cap the scores leave the sums as they are and the cap's own factors are in log2 units
+  p.scale_log2 = softcap > 0.f ? scale : scale * kLog2e;
+  p.cap_in = softcap > 0.f ? 2.f * kLog2e / softcap : 0.f; p.cap_log2 = softcap * kLog2e; p.out_scale = out_scale;
+  p.parts = static_cast<float*>(workspace);
+  p.arrivals = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + l.arrivals);
   p.dev_status = dev_status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int grid = sm_count() < kDecode4MaxCtas ? sm_count() : kDecode4MaxCtas;
   auto launch = [&](auto tag, auto cap) -> int {
     constexpr int D = decltype(tag)::value;
+    using C = Decode4Cfg<D>;
     struct Tag {};
-    const size_t smem = sizeof(float) * 8 * kDecode4MaxGroup * (D + 2);
-    const int r = opt_in_dynamic_smem<Tag>(reinterpret_cast<const void*>(&kv4_decode_kernel<D, decltype(cap)::value>), smem);
+    const int r = opt_in_dynamic_smem<Tag>(reinterpret_cast<const void*>(&kv4_decode_kernel<D, decltype(cap)::value>), C::SMEM);
     if (r != kOk) return r;
-    kv4_decode_kernel<D, decltype(cap)::value><<<dim3(p.hkv, num_seqs), 256, smem, st>>>(p);
+    kv4_decode_kernel<D, decltype(cap)::value><<<grid, C::NW * 32, C::SMEM, st>>>(p);
     return cudaGetLastError() == cudaSuccess ? kOk : kLaunchFailed;
   };
   auto by_cap = [&](auto tag) -> int { return softcap > 0.f ? launch(tag, std::true_type{}) : launch(tag, std::false_type{}); };
