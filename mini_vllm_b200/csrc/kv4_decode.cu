@@ -18,7 +18,7 @@
 // one (sequence, head), numbered sequence by sequence and head by head, and cut evenly: each CTA takes a contiguous range, each of its
 // warps a contiguous part of that.  A warp streams its tiles through a private ring in shared memory (cp.async, 16 bytes a lane, placed so
 // that the fragment loads meet no bank twice) and needs no other warp until its range is done.  Rows that lie within one warp's range go
-// straight to the output; parts of a row are put together by the CTA, and where a row crosses CTAs by the one that arrives last.  Every
+// straight to the output; parts of a row are put together by the CTA, and where a row crosses CTAs by the warps that arrive last.  Every
 // CTA works the split out for itself from the lengths (a scan in shared memory), so there is no plan to make, the grid does not depend on
 // data, and nothing ever waits for another CTA.
 #include "dtype.cuh"
@@ -45,7 +45,11 @@ struct Decode4Cfg {
   static constexpr size_t SMEM = static_cast<size_t>(NW) * RING;
 };
 
-__host__ __device__ __forceinline__ constexpr int decode4_part(int group, int d) { return group * d + kDecode4MaxGroup; }   // floats of a part
+// floats of a part: outputs of the group's heads, then their log2-sum-exps (where a CTA leaves a part for others, one copy for each warp
+// that merges a share of the channels)
+__host__ __device__ __forceinline__ constexpr int decode4_part(int group, int d) {
+  return group * d + kDecode4MaxGroup * (d == 256 ? Decode4Cfg<256>::NW : Decode4Cfg<128>::NW);
+}
 
 struct Decode4Params {
   const __nv_bfloat16* q;
@@ -60,7 +64,7 @@ struct Decode4Params {
   int table_width, num_seqs, hkv, group, block_size, budget, window_left;
   float scale_log2, cap_in, cap_log2, out_scale;
   float* parts;                        // [CTAs][NW + 2] parts: a warp's first row, then the CTA's first and last
-  int32_t* arrivals;                   // [num_seqs * hkv], zero between launches
+  int32_t* arrivals;                   // [num_seqs * hkv][NW], zero between launches
   int* dev_status;
 };
 
@@ -139,16 +143,19 @@ struct Decode4Walk {
       count = tiles(p, n);
     } while (count == 0);
   }
-  // the first token of the tile, -1: none
-  __device__ __forceinline__ int token(const Decode4Params& p) const {
-    if (p.spans == nullptr) return (first_tile(p, n) + i) * TOK;
-    constexpr int per = kKv4Span / TOK;
-    const int span = p.spans[(static_cast<int64_t>(b) * p.hkv + h) * p.budget + i / per];
-    if (span < 0) return -1;
-    if (span > (n - 1) / kKv4Span) return -2;
-    const int t = span * kKv4Span + (i % per) * TOK;
-    return t < n ? t : -1;
+};
+
+// How `total` tiles are dealt to the CTAs: no more of these than give every warp a tile (rows of a small call stay on few of them), the
+// first `rest` of them one tile more than the others.
+struct Decode4Cut {
+  int ctas, per, rest;
+  __device__ __forceinline__ Decode4Cut(int total, int warps) {
+    ctas = min(static_cast<int>(gridDim.x), (total + warps - 1) / warps);
+    per = ctas > 0 ? total / ctas : 0;
+    rest = total - per * ctas;
   }
+  __device__ __forceinline__ int start(int c) const { return c * per + min(c, rest); }
+  __device__ __forceinline__ int of(int tile) const { return tile < rest * (per + 1) ? tile / (per + 1) : (tile - rest) / per; }
 };
 
 template <int D, bool CAP>
@@ -158,10 +165,10 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
   constexpr int NW = C::NW, NT = NW * 32, NST = C::NST, GRP = C::GRP;
   constexpr uint32_t FULL = 0xffffffffu, LO = 0x000f000fu, HI = 0x00f000f0u;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int scan_s[NW];
+  __shared__ int scan_s[NW], total_s;
   __shared__ int info_s[NW][NST];                            // first token of the tile in a stage, -1: nothing to read
   __shared__ int meta_s[NW][2][3];                           // a warp's parts: row (-1: none), the row's first tile and the one behind its last
-  __shared__ int last_s;
+  __shared__ float lse_s[NW][2][kDecode4MaxGroup];           // their log2-sum-exps
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c4 = lane & 3;
   const int G = p.group;
@@ -193,33 +200,35 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
       running += s;
     }
     if (b < p.num_seqs) prefix[b] = before + x - v;
+    if (b == p.num_seqs - 1) { prefix[b + 1] = before + x; total_s = (before + x) * p.hkv; }
     __syncthreads();
   }
-  if (threadIdx.x == 0) prefix[p.num_seqs] = running;
-  const int64_t total = static_cast<int64_t>(running) * p.hkv;
-  // no more CTAs than give every warp a tile: rows of a small call stay on few of them
-  const int64_t ctas = min(static_cast<int64_t>(gridDim.x), (total + NW - 1) / NW);
   const int cta = blockIdx.x;
-  auto cta_start = [&](int64_t c) -> int { return static_cast<int>(c * total / ctas); };
-  // rows without a token: zeros
+  // sequences without a token: zeros
   for (int b = cta; b < p.num_seqs; b += gridDim.x) {
-    if (p.seqlens[b] <= 0) {
+    if (prefix[b] == prefix[b + 1]) {
       for (int e = threadIdx.x; e < p.hkv * G * D / 8; e += NT)
         *reinterpret_cast<uint4*>(p.out + b * p.out_stride + e * 8) = make_uint4(0, 0, 0, 0);
     }
   }
-  if (cta >= ctas) return;
-  const int t0 = cta_start(cta), t1 = cta_start(cta + 1);
-  const int w0 = t0 + static_cast<int>(static_cast<int64_t>(warp) * (t1 - t0) / NW);
-  const int w1 = t0 + static_cast<int>(static_cast<int64_t>(warp + 1) * (t1 - t0) / NW);
-  __syncthreads();
+  int w0, w1;
+  {
+    const Decode4Cut cut(running * p.hkv, NW);
+    if (cta >= cut.ctas) return;
+    const int t0 = cut.start(cta), tiles = cut.start(cta + 1) - t0;
+    w0 = t0 + warp * (tiles / NW) + min(warp, tiles % NW);
+    w1 = w0 + tiles / NW + (warp < tiles % NW ? 1 : 0);
+  }
   Walk cs;
   int row_t0 = 0;                                            // the number of the row's first tile
   {
-    int lo = 0, hi = p.num_seqs;                             // the last b with prefix[b] * hkv <= w0
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (static_cast<int64_t>(prefix[mid]) * p.hkv <= w0) lo = mid; else hi = mid;
+    int lo = 0, size = p.num_seqs;                           // the last b with prefix[b] * hkv <= w0 is in [lo, lo + size)
+    while (size > 1) {
+      const int step = (size + 31) / 32, at = lo + lane * step;
+      const uint32_t below = __ballot_sync(FULL, lane * step < size && prefix[at] * p.hkv <= w0);
+      const int skip = (31 - __clz(below)) * step;           // (lane 0 is always below)
+      lo += skip;
+      size = min(step, size - skip);
     }
     cs.b = lo;
     cs.n = Walk::length(p, lo);
@@ -230,32 +239,63 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
     row_t0 = w0 - cs.i;
   }
   if (lane < 2) meta_s[warp][lane][0] = -1;
+  if (lane < kDecode4MaxGroup) lse_s[warp][1][lane] = -INFINITY;
   __syncthreads();                                           // the prefix sums have been read: the ring may be filled
 
   // ---- the fetching side ------------------------------------------------------------------------------------------------------------
   const uint32_t ring = smem_u32(smem) + warp * C::RING;
   Walk fs = cs;
   int ft = w0;                                               // the next tile to fetch
+  // Where a row's tiles lie, 32 units at a time: lane i knows the block of table column known + i, or, with a list of spans, the first
+  // token and the block of its entry known + i.
+  int known = -1, u_block = -1, u_token = -1;
   int f_token = -1, f_block = -1;
   auto look = [&]() {                                        // first token and block of the tile that is fetched next
-    f_token = -1;
     if (ft >= w1) return;
-    f_token = fs.token(p);
-    if (f_token >= 0) f_block = p.block_table[fs.b * p.table_stride + p.by_block.div(f_token)];
+    const int32_t* table = p.block_table + fs.b * p.table_stride;
+    if (p.spans == nullptr) {
+      f_token = (Walk::first_tile(p, fs.n) + fs.i) * C::TOK;
+      const int col = static_cast<int>(p.by_block.div(f_token));
+      if (known < 0 || col < known || col >= known + 32) {
+        known = col;
+        u_block = col + lane < p.table_width ? __ldg(table + col + lane) : -1;
+      }
+      f_block = col - known;
+    } else {
+      constexpr int PER = kKv4Span / C::TOK;
+      const int at = fs.i / PER;
+      if (known < 0 || at >= known + 32) {
+        known = at;
+        const int32_t* list = p.spans + (static_cast<int64_t>(fs.b) * p.hkv + fs.h) * p.budget;
+        const int span = at + lane < p.budget ? __ldg(list + at + lane) : -1;
+        const bool fits = span <= (fs.n - 1) / kKv4Span;
+        if (!fits) report(p.dev_status, kDevBadLength, fs.b);
+        u_token = span >= 0 && fits ? span * kKv4Span : -1;
+        u_block = u_token >= 0 ? __ldg(table + p.by_block.div(u_token)) : -1;
+      }
+      f_token = (fs.i % PER) * C::TOK;
+      f_block = at - known;
+    }
   };
   int f_stage = 0;
   auto fetch = [&]() {
     if (ft < w1) {
-      bool ok = f_token >= 0;
-      if (ok && (f_block < 0 || f_block >= p.num_blocks)) {
+      const int block = __shfl_sync(FULL, u_block, f_block);
+      int token = f_token;
+      bool ok = true;
+      if (p.spans != nullptr) {
+        const int base = __shfl_sync(FULL, u_token, f_block);
+        token += base;
+        ok = base >= 0 && token < fs.n;
+      }
+      if (ok && (block < 0 || block >= p.num_blocks)) {
         if (lane == 0) report(p.dev_status, kDevBadBlock, fs.b);
         ok = false;
       }
-      if (f_token == -2 && lane == 0) report(p.dev_status, kDevBadLength, fs.b);
-      if (lane == 0) info_s[warp][f_stage] = ok ? f_token : -1;
+      if (lane == 0) info_s[warp][f_stage] = ok ? token : -1;
       if (ok) {
-        const int in_block = f_token - static_cast<int>(p.by_block.div(f_token)) * p.block_size;
-        const int64_t row = kv4_row(f_block, p.hkv, fs.h, p.block_size, in_block);
+        const int in_block = token - static_cast<int>(p.by_block.div(token)) * p.block_size;
+        const int64_t row = kv4_row(block, p.hkv, fs.h, p.block_size, in_block);
         const uint8_t* k = p.k_codes + row * (D / 2);
         const uint8_t* v = p.v_codes + row * (D / 2);
         const uint32_t dst = ring + f_stage * C::STAGE;
@@ -277,12 +317,24 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
         }
       }
       ++ft;
+      const int b = fs.b;
       fs.next(p);
+      if (fs.b != b || (p.spans != nullptr && fs.i == 0)) known = -1;
       f_stage = f_stage + 1 == NST ? 0 : f_stage + 1;
       look();
     }
     cp_async_commit();
   };
+  // q of a row, requested before anything that waits: word j of a lane is channels 8 (4 j + c4) .. of head g of the group
+  uint4 qw[C::WK];
+  auto ask_q = [&](int b, int h) {
+#pragma unroll
+    for (int j = 0; j < C::WK; ++j) {
+      qw[j] = make_uint4(0, 0, 0, 0);
+      if (g < G) qw[j] = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.q_stride + (static_cast<int64_t>(h) * G + g) * D + 8 * (4 * j + c4)));
+    }
+  };
+  if (w0 < w1) ask_q(cs.b, cs.h);
   look();
 #pragma unroll
   for (int i = 0; i < NST - 1; ++i) fetch();
@@ -296,20 +348,14 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
     const int b = cs.b, h = cs.h, n = cs.n;
     const int start = p.window_left >= 0 ? max(0, n - 1 - p.window_left) : 0;
 
-    // q as the B operand (head g of the group in column g): word j of a lane is channels 8 (4 j + c4) ..
+    // q as the B operand (head g of the group in column g)
     uint32_t qf[C::WK][4];
     float qs_a[GRP], qs_b[GRP], f_a, f_b;                    // sums per group and the score's factor, of heads 2 c4 and 2 c4 + 1
     {
-      uint4 w[C::WK];
-#pragma unroll
-      for (int j = 0; j < C::WK; ++j) {
-        w[j] = make_uint4(0, 0, 0, 0);
-        if (g < G) w[j] = *reinterpret_cast<const uint4*>(p.q + b * p.q_stride + (static_cast<int64_t>(h) * G + g) * D + 8 * (4 * j + c4));
-      }
       float most = 0.f;
 #pragma unroll
       for (int j = 0; j < C::WK; ++j) {
-        const uint32_t a[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+        const uint32_t a[4] = {qw[j].x, qw[j].y, qw[j].z, qw[j].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) most = fmaxf(most, fmaxf(fabsf(bf16_lo(a[e])), fabsf(bf16_hi(a[e]))));
       }
@@ -323,7 +369,7 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
       for (int j = 0; j < GRP; ++j) sum[j] = 0.f;
 #pragma unroll
       for (int j = 0; j < C::WK; ++j) {
-        const uint32_t a[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+        const uint32_t a[4] = {qw[j].x, qw[j].y, qw[j].z, qw[j].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float x = bf16_lo(a[e]) * grow, y = bf16_hi(a[e]) * grow;
@@ -478,7 +524,12 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
       }
     }
 
-    // ---- the end of the row, or of this warp's part of it ---------------------------------------------------------------------------
+    // ---- the end of the row, or of this warp's part of it; the next row's q is on its way meanwhile ------------------------------------
+    if (t < w1) {
+      cs.i = cs.count - 1;
+      cs.next(p);
+      ask_q(cs.b, cs.h);
+    }
 #pragma unroll
     for (int off = 4; off < 32; off <<= 1) {
       l_a += __shfl_xor_sync(FULL, l_a, off);
@@ -525,97 +576,153 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
         if (complete) store_vec<__nv_bfloat16, 8>(p.out + b * p.out_stride + (static_cast<int64_t>(h) * G + head) * D + 64 * j + 8 * g, y);
         else store_f32<8>(part + head * D + 64 * j + 8 * g, y);
       }
-      if (!complete && g == 0) part[G * D + head] = l > 0.f ? m + fast_log2(l) : -INFINITY;
+      if (!complete && g == 0) lse_s[warp][seg_end == w1 ? 1 : 0][head] = l > 0.f ? m + fast_log2(l) : -INFINITY;
     }
-    // on to the next row
-    if (t < w1) {
-      cs.i = cs.count - 1;
-      cs.next(p);
-      row_t0 = row_t1;
-    }
+    row_t0 = row_t1;
   }
   cp_async_wait<0>();
   __syncthreads();
 
-  // ---- parts of rows, put together by the CTA: neighbouring parts of one row are one run ------------------------------------------------
-  auto part_of = [&](int slot) -> const float* {             // slot = 2 * warp + (0: first row, 1: last row)
-    const int w = slot >> 1;
-    return (slot & 1) ? reinterpret_cast<const float*>(smem + w * C::RING) : p.parts + (static_cast<int64_t>(cta) * (NW + 2) + w) * decode4_part(G, D);
-  };
+  // ---- parts of rows, put together --------------------------------------------------------------------------------------------------
+  // The parts of a row are those of neighbouring warps, one of each: last parts in the rings, and perhaps a first part, in the workspace,
+  // of the last of these warps.  This code runs once, from a cold instruction cache: it is kept small, not unrolled.
+  const Decode4Cut cut(total_s, NW);                         // (worked out again: it need not sit in registers meanwhile)
+  const int t0 = cut.start(cta), t1 = cut.start(cta + 1);
   const int* meta = &meta_s[0][0][0];
-  for (int slot = 0; slot < 2 * NW;) {
-    const int row = meta[slot * 3];
-    if (row < 0) { ++slot; continue; }
-    int end = slot + 1;
-    while (end < 2 * NW && (meta[end * 3] < 0 || meta[end * 3] == row)) ++end;
-    const int r0 = meta[slot * 3 + 1], r1 = meta[slot * 3 + 2];
-    const bool complete = r0 >= t0 && r1 <= t1;
-    const int b = row / p.hkv, h = row - b * p.hkv;
-    float* mine = p.parts + (static_cast<int64_t>(cta) * (NW + 2) + NW + (r0 <= t0 ? 0 : 1)) * decode4_part(G, D);
-    for (int e = threadIdx.x; e < G * D / 4; e += NT) {
-      const int head = e * 4 / D;
-      float M = -INFINITY;
-      for (int s = slot; s < end; ++s)
-        if (meta[s * 3] >= 0) M = fmaxf(M, part_of(s)[G * D + head]);
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      float sum = 0.f;
-      for (int s = slot; s < end; ++s) {
-        if (meta[s * 3] < 0) continue;
-        const float* from = part_of(s);
-        const float w = M == -INFINITY ? 0.f : fast_exp2(from[G * D + head] - M);
-        const float4 v = *reinterpret_cast<const float4*>(from + e * 4);
-        acc.x = fmaf(w, v.x, acc.x); acc.y = fmaf(w, v.y, acc.y); acc.z = fmaf(w, v.z, acc.z); acc.w = fmaf(w, v.w, acc.w);
-        sum += w;
-      }
-      const float inv = sum > 0.f ? (complete ? p.out_scale : 1.f) / sum : 0.f;
-      acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
-      if (complete) {
-        *reinterpret_cast<uint2*>(p.out + b * p.out_stride + static_cast<int64_t>(h) * G * D + e * 4) =
-            make_uint2(pack_bf16(acc.x, acc.y), pack_bf16(acc.z, acc.w));
-      } else {
-        *reinterpret_cast<float4*>(mine + e * 4) = acc;
-        if ((e * 4) % D == 0) mine[G * D + head] = sum > 0.f ? M + fast_log2(sum) : -INFINITY;
+  const int of_lane = lane < NW ? lane : 0;
+  const int row_f = lane < NW ? meta_s[of_lane][0][0] : -1, row_l = lane < NW ? meta_s[of_lane][1][0] : -1;
+  const float* first_parts = p.parts + static_cast<int64_t>(cta) * (NW + 2) * decode4_part(G, D);
+  // four outputs of a row and the log2-sum-exp of their head, from the warps of the masks
+  auto sum_parts = [&](uint32_t f, uint32_t l, int e, float& lse) -> float4 {
+    const int head = e * 4 / D, wf = __ffs(f) - 1;           // (-1: no first part)
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f), acc = v;
+    if (wf >= 0) v = *reinterpret_cast<const float4*>(first_parts + wf * decode4_part(G, D) + e * 4);
+    const int lo = l != 0 ? __ffs(l) - 1 : 0, hi = 31 - __clz(l);            // (no last part: hi is -1)
+    const float xf = wf >= 0 ? lse_s[wf][0][head] : -INFINITY;
+    float M = xf, sum = 0.f;
+#pragma unroll 4
+    for (int w = lo; w <= hi; ++w) M = fmaxf(M, lse_s[w][1][head]);          // -inf where a warp has no tiles
+    const float r = M == -INFINITY ? 0.f : M;
+#pragma unroll 4
+    for (int w = lo; w <= hi; ++w) {
+      const float a = fast_exp2(lse_s[w][1][head] - r);
+      if (a > 0.f) {
+        const float4 x = *reinterpret_cast<const float4*>(smem + w * C::RING + e * 16);
+        acc.x = fmaf(a, x.x, acc.x); acc.y = fmaf(a, x.y, acc.y); acc.z = fmaf(a, x.z, acc.z); acc.w = fmaf(a, x.w, acc.w);
+        sum += a;
       }
     }
-    if (!complete) {
-      // the row's other CTAs: whoever arrives last finds every part in memory
-      const int c1 = static_cast<int>(((static_cast<int64_t>(r0) + 1) * ctas - 1) / total);
-      const int c2 = static_cast<int>((static_cast<int64_t>(r1) * ctas - 1) / total);
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        int prev;
-        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(prev) : "l"(p.arrivals + row) : "memory");
-        last_s = prev == c2 - c1;
-        if (last_s) p.arrivals[row] = 0;                     // as the next launch expects it
+    const float a = fast_exp2(xf - r);
+    acc.x = fmaf(a, v.x, acc.x); acc.y = fmaf(a, v.y, acc.y); acc.z = fmaf(a, v.z, acc.z); acc.w = fmaf(a, v.w, acc.w);
+    sum += a;
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
+    lse = sum > 0.f ? M + fast_log2(sum) : -INFINITY;
+    return acc;
+  };
+  auto put = [&](int row, int e, const float4& y, float f) {
+    const int b = row / p.hkv, h = row - b * p.hkv;
+    *reinterpret_cast<uint2*>(p.out + b * p.out_stride + static_cast<int64_t>(h) * G * D + e * 4) =
+        make_uint2(pack_bf16(y.x * f, y.y * f), pack_bf16(y.z * f, y.w * f));
+  };
+  // Job 0, 1: the rows of this warp's own parts, where they end in the CTA; the warps with a part of a row share its outputs.  Job 2, 3: the
+  // CTA's first and last row, where they go on in other CTAs: every warp takes D / NW channels of all heads, in every CTA alike.
+  constexpr int PIECES = D / NW / 4;                         // 16-byte pieces of a head that a warp takes of such a row
+  const int share = G * PIECES, E4 = G * D / 4;
+  const uint32_t cross_f = __ballot_sync(FULL, row_f >= 0 && (meta_s[of_lane][0][1] < t0 || meta_s[of_lane][0][2] > t1));
+  const uint32_t cross_l = __ballot_sync(FULL, row_l >= 0 && (meta_s[of_lane][1][1] < t0 || meta_s[of_lane][1][2] > t1));
+  auto piece = [&](int i) -> int { return i / PIECES * (D / 4) + warp * PIECES + i % PIECES; };   // of the share, as a piece of the row
+  int mine_row = -1, mine_first = 0, mine_last = 0;          // lanes 0 and 1: the crossing rows
+#pragma unroll 1
+  for (int job = 0; job < 4; ++job) {
+    int slot;
+    if (job < 2) {
+      slot = 2 * warp + job;
+    } else {
+      const uint32_t any = cross_f | cross_l;
+      if (any == 0) return;                                  // (the whole CTA)
+      const int w = job == 2 ? __ffs(any) - 1 : 31 - __clz(any);
+      slot = 2 * w + (job == 2 ? (cross_f >> w & 1 ? 0 : 1) : static_cast<int>(cross_l >> w & 1));
+    }
+    const int row = meta[slot * 3], r0 = meta[slot * 3 + 1], r1 = meta[slot * 3 + 2];
+    if (row < 0 || (job < 2 && (r0 < t0 || r1 > t1))) continue;
+    if (job == 3 && row == __shfl_sync(FULL, mine_row, 0)) continue;
+    const uint32_t f = __ballot_sync(FULL, row_f == row), l = __ballot_sync(FULL, row_l == row);
+    int at = lane, end = share;
+    if (job < 2) {
+      const int parts = __popc(f | l), mine = __popc((f | l) & ((1u << warp) - 1));
+      at = mine * E4 / parts + lane; end = (mine + 1) * E4 / parts;
+    } else if (lane == job - 2) {
+      mine_row = row; mine_first = r0; mine_last = r1;
+    }
+    float* to = p.parts + (static_cast<int64_t>(cta) * (NW + 2) + NW + (r0 <= t0 ? 0 : 1)) * decode4_part(G, D);
+    for (; at < end; at += 32) {
+      const int e = job < 2 ? at : piece(at);
+      float lse;
+      const float4 y = sum_parts(f, l, e, lse);
+      if (job < 2) {
+        put(row, e, y, p.out_scale);
+      } else {
+        *reinterpret_cast<float4*>(to + e * 4) = y;
+        if (at % PIECES == 0) to[G * D + kDecode4MaxGroup * warp + at / PIECES] = lse;
       }
-      __syncthreads();
-      if (last_s) {
-        const float* first = p.parts + (static_cast<int64_t>(c1) * (NW + 2) + NW + (r0 <= cta_start(c1) ? 0 : 1)) * decode4_part(G, D);
-        auto other = [&](int c) -> const float* {
-          return c == c1 ? first : p.parts + (static_cast<int64_t>(c) * (NW + 2) + NW) * decode4_part(G, D);
-        };
-        for (int e = threadIdx.x; e < G * D / 4; e += NT) {
-          const int head = e * 4 / D;
-          float M = -INFINITY;
-          for (int c = c1; c <= c2; ++c) M = fmaxf(M, __ldcg(other(c) + G * D + head));
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-          float sum = 0.f;
+    }
+  }
+  // Of the warps with the same channels of a crossing row, the one that arrives last finds all parts of them in memory.
+  __syncwarp();                                              // the lanes' parts come before the release
+  int c1 = 0, parts = 0;
+  if (mine_row >= 0) {
+    c1 = cut.of(mine_first);
+    parts = cut.of(mine_last - 1) - c1 + 1;
+    int32_t* count = p.arrivals + static_cast<int64_t>(mine_row) * NW + warp;
+    int prev;
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(prev) : "l"(count) : "memory");
+    if (prev == parts - 1) *count = 0;                       // as the next launch expects it
+    else parts = 0;
+  }
+  __syncwarp();
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) {
+    const int n = __shfl_sync(FULL, parts, i);
+    if (n == 0) continue;
+    const int from_cta = __shfl_sync(FULL, c1, i), row = __shfl_sync(FULL, mine_row, i), r0 = __shfl_sync(FULL, mine_first, i);
+    // a lane takes a piece, or the piece of every n-th part where a warp's share leaves lanes over
+    const int lanes = min(share, 32), split = 32 / lanes, mine = lane / lanes, first = lane - mine * lanes;
+    const float* head_part = p.parts + (static_cast<int64_t>(from_cta) * (NW + 2) + NW) * decode4_part(G, D);
+    const int64_t stride = static_cast<int64_t>(NW + 2) * decode4_part(G, D);
+    const int late = r0 <= cut.start(from_cta) ? 0 : decode4_part(G, D);     // the first CTA's part, where the row began inside it
+    for (int base = 0; base < share; base += 32) {
+      const int e = piece(base + first);
+      const bool works = mine < split && base + first < share;
+      float M = -INFINITY, sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (works) {
+        const int at_lse = G * D + kDecode4MaxGroup * warp + (base + first) / PIECES;
 #pragma unroll 4
-          for (int c = c1; c <= c2; ++c) {
-            const float* from = other(c);
-            const float w = M == -INFINITY ? 0.f : fast_exp2(__ldcg(from + G * D + head) - M);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(from + e * 4));
-            acc.x = fmaf(w, v.x, acc.x); acc.y = fmaf(w, v.y, acc.y); acc.z = fmaf(w, v.z, acc.z); acc.w = fmaf(w, v.w, acc.w);
-            sum += w;
-          }
-          const float inv = sum > 0.f ? p.out_scale / sum : 0.f;
-          *reinterpret_cast<uint2*>(p.out + b * p.out_stride + static_cast<int64_t>(h) * G * D + e * 4) =
-              make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+        for (int c = mine; c < n; c += split) {
+          const float* from = head_part + c * stride + (c == 0 ? late : 0);
+          const float lse = __ldcg(from + at_lse);
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(from + e * 4));
+          const float nm = fmaxf(M, lse), r = nm == -INFINITY ? 0.f : nm;
+          const float a = fast_exp2(M - r), f = fast_exp2(lse - r);
+          acc.x = fmaf(acc.x, a, f * v.x); acc.y = fmaf(acc.y, a, f * v.y); acc.z = fmaf(acc.z, a, f * v.z); acc.w = fmaf(acc.w, a, f * v.w);
+          sum = fmaf(sum, a, f);
+          M = nm;
         }
       }
-      __syncthreads();
+      float top = M;
+      for (int k = 0; k < split; ++k) top = fmaxf(top, __shfl_sync(FULL, M, first + k * lanes));
+      const float a = M == -INFINITY ? 0.f : fast_exp2(M - top);
+      const float4 own = make_float4(acc.x * a, acc.y * a, acc.z * a, acc.w * a);
+      const float own_sum = sum * a;
+      acc = own; sum = own_sum;
+      for (int k = 1; k < split; ++k) {                      // (lanes of the first part add the others)
+        const int from = first + k * lanes;
+        acc.x += __shfl_sync(FULL, own.x, from); acc.y += __shfl_sync(FULL, own.y, from); acc.z += __shfl_sync(FULL, own.z, from);
+        acc.w += __shfl_sync(FULL, own.w, from); sum += __shfl_sync(FULL, own_sum, from);
+      }
+      if (works && mine == 0) put(row, e, acc, sum > 0.f ? p.out_scale / sum : 0.f);
     }
-    slot = end;
   }
 }
 
@@ -627,7 +734,7 @@ static Decode4Layout decode4_layout(int64_t seqs, int hkv, int group, int d) {
   Decode4Layout l;
   l.parts = 0;
   l.arrivals = (sizeof(float) * kDecode4MaxCtas * (nw + 2) * decode4_part(group, d) + 255) / 256 * 256;
-  l.total = l.arrivals + (sizeof(int32_t) * static_cast<size_t>(seqs) * hkv + 255) / 256 * 256;
+  l.total = l.arrivals + (sizeof(int32_t) * static_cast<size_t>(seqs) * hkv * nw + 255) / 256 * 256;
   return l;
 }
 
