@@ -7,12 +7,13 @@
 // Nothing is unpacked to values.  With the codes themselves as matrix operands (masked halves of a word are fp16 subnormals, kv4.cuh)
 //     q . k_t  = sum over groups of  s_t (q . c_t) + m_t sum(q)
 //     sum_t p_t v_t = sum over t of  (p_t s_t) c_t  +  sum_t p_t m_t        per group
-// so a 32-bit word of eight codes costs five integer instructions for keys (one shift, four ANDs) and six for values (two tokens of a
-// channel have to meet in a register: a byte permutation more), and scales and minima cost a few per token.  q is brought to [2^14, 2^15)
+// so a 32-bit word of eight codes costs five integer instructions, for keys (one shift, four ANDs) and for values (where two tokens of a
+// channel have to meet in a register: a byte permutation, and the high codes of a byte are never masked out, their sums are those of
+// whole bytes less those of the low codes), and scales and minima cost a few per token.  q is brought to [2^14, 2^15)
 // by a power of two per head so that fp16 holds every bf16 exactly down to 2^-29 of the greatest; the channels whose codes sit at bits 4-7
 // (16 times as large) have it divided by 16.  Scores, softmax statistics and outputs are fp32; the weights p s are rounded once, to fp16,
 // an eighth of what bf16 weights would lose.  They never overflow: the softmax's reference is the greatest score + log2(scale), which
-// bounds every p s by 1 (scales below 2^-60 count as that).
+// bounds every p s by 2^6 (scales below 2^-60 count as that).
 //
 // Bound by memory, on paper 4608 bytes against some 450 warp instructions per 32 tokens of a 128-wide head.  Work is tiles of 32 tokens of
 // one (sequence, head), numbered sequence by sequence and head by head, and cut evenly: each CTA takes a contiguous range, each of its
@@ -158,16 +159,23 @@ struct Decode4Cut {
   __device__ __forceinline__ int of(int tile) const { return tile < rest * (per + 1) ? tile / (per + 1) : (tile - rest) / per; }
 };
 
+// a run of tiles of head h of sequence b (n tokens): its first token (behind the span's, with a list of spans) and which lane has its block
+struct Decode4Run {
+  int known, known_row, sel, token, tiles, b, h, n;
+};
+
 template <int D, bool CAP>
 __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(const Decode4Params p) {
   using C = Decode4Cfg<D>;
   using Walk = Decode4Walk<C::TOK>;
   constexpr int NW = C::NW, NT = NW * 32, NST = C::NST, GRP = C::GRP;
-  constexpr uint32_t FULL = 0xffffffffu, LO = 0x000f000fu, HI = 0x00f000f0u;
+  constexpr uint32_t FULL = 0xffffffffu, LO = 0x000f000fu, HI = 0x00f000f0u, BYTE = 0x00ff00ffu;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int scan_s[NW], total_s;
   __shared__ int info_s[NW][NST];                            // first token of the tile in a stage, -1: nothing to read
   __shared__ int meta_s[NW][2][3];                           // a warp's parts: row (-1: none), the row's first tile and the one behind its last
+  __shared__ Walk fs_s[NW], cs_s[NW];                        // a warp's fetching and computing side
+  __shared__ Decode4Run run_s[NW];
   __shared__ float lse_s[NW][2][kDecode4MaxGroup];           // their log2-sum-exps
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c4 = lane & 3;
@@ -244,84 +252,98 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
 
   // ---- the fetching side ------------------------------------------------------------------------------------------------------------
   const uint32_t ring = smem_u32(smem) + warp * C::RING;
-  Walk fs = cs;
   int ft = w0;                                               // the next tile to fetch
-  // Where a row's tiles lie, 32 units at a time: lane i knows the block of table column known + i, or, with a list of spans, the first
-  // token and the block of its entry known + i.
-  int known = -1, u_block = -1, u_token = -1;
-  int f_token = -1, f_block = -1;
-  auto look = [&]() {                                        // first token and block of the tile that is fetched next
+  // A run: tiles that lie one behind the other in memory (of one block, or of one span).  Where the runs lie is known 32 at a time: lane i
+  // has the block of table column known + i or, with a list of spans, the first token and the block of its entry known + i.
+  // What only changes from run to run is kept in shared memory.
+  int u_block = -1, u_token = -1;
+  if (lane == 0) { fs_s[warp] = cs; run_s[warp].known = 0; run_s[warp].known_row = -1; }
+  __syncwarp();
+  auto look = [&]() {                                        // the next run; its block may still be on its way
     if (ft >= w1) return;
+    Walk fs = fs_s[warp];                                    // the first tile that no run covers yet
+    int known = run_s[warp].known, known_row = run_s[warp].known_row, run_token;
     const int32_t* table = p.block_table + fs.b * p.table_stride;
+    int at, room;
     if (p.spans == nullptr) {
-      f_token = (Walk::first_tile(p, fs.n) + fs.i) * C::TOK;
-      const int col = static_cast<int>(p.by_block.div(f_token));
-      if (known < 0 || col < known || col >= known + 32) {
-        known = col;
-        u_block = col + lane < p.table_width ? __ldg(table + col + lane) : -1;
+      run_token = (Walk::first_tile(p, fs.n) + fs.i) * C::TOK;
+      at = static_cast<int>(p.by_block.div(run_token));
+      room = ((at + 1) * p.block_size - run_token) / C::TOK;
+      if (known_row != fs.b || at < known || at >= known + 32) {
+        known = at; known_row = fs.b;
+        u_block = at + lane < p.table_width ? __ldg(table + at + lane) : -1;
       }
-      f_block = col - known;
     } else {
       constexpr int PER = kKv4Span / C::TOK;
-      const int at = fs.i / PER;
-      if (known < 0 || at >= known + 32) {
-        known = at;
-        const int32_t* list = p.spans + (static_cast<int64_t>(fs.b) * p.hkv + fs.h) * p.budget;
-        const int span = at + lane < p.budget ? __ldg(list + at + lane) : -1;
+      const int row = fs.b * p.hkv + fs.h;
+      at = fs.i / PER;
+      room = PER - fs.i % PER;
+      run_token = (fs.i % PER) * C::TOK;
+      if (known_row != row || at >= known + 32) {
+        known = at; known_row = row;
+        const int span = at + lane < p.budget ? __ldg(p.spans + static_cast<int64_t>(row) * p.budget + at + lane) : -1;
         const bool fits = span <= (fs.n - 1) / kKv4Span;
         if (!fits) report(p.dev_status, kDevBadLength, fs.b);
         u_token = span >= 0 && fits ? span * kKv4Span : -1;
         u_block = u_token >= 0 ? __ldg(table + p.by_block.div(u_token)) : -1;
       }
-      f_token = (fs.i % PER) * C::TOK;
-      f_block = at - known;
     }
+    const int tiles = min(room, fs.count - fs.i), b = fs.b, h = fs.h, n = fs.n;
+    fs.i += tiles - 1;
+    fs.next(p);
+    __syncwarp();
+    if (lane == 0) { fs_s[warp] = fs; run_s[warp] = Decode4Run{known, known_row, at - known, run_token, tiles, b, h, n}; }
+    __syncwarp();
   };
-  int f_stage = 0;
+  int f_stage = 0, f_left = 0, f_token = 0, f_n = 0;
+  int64_t f_off = -1;                                        // of the codes, in bytes; < 0: nothing to read
   auto fetch = [&]() {
     if (ft < w1) {
-      const int block = __shfl_sync(FULL, u_block, f_block);
-      int token = f_token;
-      bool ok = true;
-      if (p.spans != nullptr) {
-        const int base = __shfl_sync(FULL, u_token, f_block);
-        token += base;
-        ok = base >= 0 && token < fs.n;
+      if (f_left == 0) {                                     // on to the run that look() found
+        const Decode4Run run = run_s[warp];
+        const int block = __shfl_sync(FULL, u_block, run.sel);
+        f_token = run.token; f_left = run.tiles; f_n = run.n;
+        bool ok = true;
+        if (p.spans != nullptr) {
+          const int base = __shfl_sync(FULL, u_token, run.sel);
+          f_token += base;
+          ok = base >= 0;
+        }
+        if (ok && (block < 0 || block >= p.num_blocks)) {
+          if (lane == 0) report(p.dev_status, kDevBadBlock, run.b);
+          ok = false;
+        }
+        const int in_block = f_token - static_cast<int>(p.by_block.div(max(f_token, 0))) * p.block_size;
+        f_off = ok ? kv4_row(block, p.hkv, run.h, p.block_size, in_block) * (D / 2) : -1;
       }
-      if (ok && (block < 0 || block >= p.num_blocks)) {
-        if (lane == 0) report(p.dev_status, kDevBadBlock, fs.b);
-        ok = false;
-      }
-      if (lane == 0) info_s[warp][f_stage] = ok ? token : -1;
+      const bool ok = f_off >= 0 && f_token < f_n;
+      if (lane == 0) info_s[warp][f_stage] = ok ? f_token : -1;
       if (ok) {
-        const int in_block = token - static_cast<int>(p.by_block.div(token)) * p.block_size;
-        const int64_t row = kv4_row(block, p.hkv, fs.h, p.block_size, in_block);
-        const uint8_t* k = p.k_codes + row * (D / 2);
-        const uint8_t* v = p.v_codes + row * (D / 2);
+        const uint8_t* k = p.k_codes + f_off + lane * 16;
+        const uint8_t* v = p.v_codes + f_off + lane * 16;
         const uint32_t dst = ring + f_stage * C::STAGE;
         constexpr int PPR = D / 32;                          // 16-byte pieces of a row
 #pragma unroll
         for (int i = 0; i < C::TOK * PPR / 32; ++i) {
           const int at = i * 32 + lane, t = at / PPR, piece = at % PPR;
-          cp_async16(dst + key_piece<D>(t, piece), k + at * 16);
-          cp_async16(dst + C::CODES + value_piece<D>(t, piece), v + at * 16);
+          cp_async16(dst + key_piece<D>(t, piece), k + i * 512);
+          cp_async16(dst + C::CODES + value_piece<D>(t, piece), v + i * 512);
         }
-        const uint8_t* ka = p.k_affine + row * (D / 16);
-        const uint8_t* va = p.v_affine + row * (D / 16);
+        const uint8_t* ka = p.k_affine + f_off / 8 + lane * 16;
+        const uint8_t* va = p.v_affine + f_off / 8 + lane * 16;
         if constexpr (C::AFF / 16 >= 32) {
-          cp_async16(dst + 2 * C::CODES + lane * 16, ka + lane * 16);
-          cp_async16(dst + 2 * C::CODES + C::AFF + lane * 16, va + lane * 16);
+          cp_async16(dst + 2 * C::CODES + lane * 16, ka);
+          cp_async16(dst + 2 * C::CODES + C::AFF + lane * 16, va);
         } else {
           constexpr int PA = C::AFF / 16;
-          if (lane < 2 * PA) cp_async16(dst + 2 * C::CODES + lane * 16, lane < PA ? ka + lane * 16 : va + (lane - PA) * 16);
+          if (lane < 2 * PA) cp_async16(dst + 2 * C::CODES + lane * 16, lane < PA ? ka : va - PA * 16);
         }
+        f_off += C::TOK * D / 2;
       }
       ++ft;
-      const int b = fs.b;
-      fs.next(p);
-      if (fs.b != b || (p.spans != nullptr && fs.i == 0)) known = -1;
+      f_token += C::TOK;
       f_stage = f_stage + 1 == NST ? 0 : f_stage + 1;
-      look();
+      if (--f_left == 0) look();
     }
     cp_async_commit();
   };
@@ -335,6 +357,7 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
     }
   };
   if (w0 < w1) ask_q(cs.b, cs.h);
+  if (lane == 0) cs_s[warp] = cs;
   look();
 #pragma unroll
   for (int i = 0; i < NST - 1; ++i) fetch();
@@ -344,8 +367,7 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
   const int vt0 = decode4_row(2 * c4), vt1 = decode4_row(2 * c4 + 1);
   int t = w0, stage = 0;
   while (t < w1) {
-    const int row_t1 = row_t0 + cs.count, seg_end = min(w1, row_t1);
-    const int b = cs.b, h = cs.h, n = cs.n;
+    const int n = cs_s[warp].n, row_t1 = row_t0 + cs_s[warp].count, seg_end = min(w1, row_t1);
     const int start = p.window_left >= 0 ? max(0, n - 1 - p.window_left) : 0;
 
     // q as the B operand (head g of the group in column g)
@@ -474,26 +496,26 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
 #pragma unroll
         for (int j = 0; j < GRP; ++j) { big0 = fmaxf(big0, kv4_scale(va[s][0][j])); big1 = fmaxf(big1, kv4_scale(va[s][1][j])); }
         big0 = fast_log2(big0); big1 = fast_log2(big1);
-        ta = fmaxf(ta, fmaxf(x[s][0] + big0, x[s][2] + big1));
-        tb = fmaxf(tb, fmaxf(x[s][1] + big0, x[s][3] + big1));
+        ta = fmax3(ta, x[s][0] + big0, x[s][2] + big1);
+        tb = fmax3(tb, x[s][1] + big0, x[s][3] + big1);
       }
-      // ---- the running reference and sum ------------------------------------------------------------------------------------------
+      // ---- the running reference: moved only when a weight would pass 2^6, which fp16 holds with room to spare ----------------------------
+      if (__any_sync(FULL, ta > m_a + 6.f || tb > m_b + 6.f)) {
 #pragma unroll
-      for (int off = 4; off < 32; off <<= 1) {
-        ta = fmaxf(ta, __shfl_xor_sync(FULL, ta, off));
-        tb = fmaxf(tb, __shfl_xor_sync(FULL, tb, off));
-      }
-      const float na = fmaxf(m_a, ta), nb = fmaxf(m_b, tb);
-      const float ra = na == -INFINITY ? 0.f : na, rb = nb == -INFINITY ? 0.f : nb;
-      if (__any_sync(FULL, na != m_a || nb != m_b)) {
-        const float alpha_a = fast_exp2(m_a - ra), alpha_b = fast_exp2(m_b - rb);
+        for (int off = 4; off < 32; off <<= 1) {
+          ta = fmaxf(ta, __shfl_xor_sync(FULL, ta, off));
+          tb = fmaxf(tb, __shfl_xor_sync(FULL, tb, off));
+        }
+        ta = fmaxf(m_a, ta); tb = fmaxf(m_b, tb);
+        const float alpha_a = ta == -INFINITY ? 1.f : fast_exp2(m_a - ta), alpha_b = tb == -INFINITY ? 1.f : fast_exp2(m_b - tb);
+        m_a = ta; m_b = tb;
         l_a *= alpha_a; l_b *= alpha_b;
 #pragma unroll
         for (int j = 0; j < GRP; ++j) { pm_a[j] *= alpha_a; pm_b[j] *= alpha_b; }
 #pragma unroll
         for (int i = 0; i < 4 * C::WV; ++i) { o[i][0] *= alpha_a; o[i][1] *= alpha_b; o[i][2] *= alpha_a; o[i][3] *= alpha_b; }
-        m_a = na; m_b = nb;
       }
+      const float ra = m_a == -INFINITY ? 0.f : m_a, rb = m_b == -INFINITY ? 0.f : m_b;
       // ---- weights: transposed, as the B operand of the values --------------------------------------------------------------------
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
@@ -515,20 +537,28 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
           const uint32_t b0 = movmatrix_trans(pack_f16(p0 * s0, p1 * s0)), b1 = movmatrix_trans(pack_f16(p2 * s1, p3 * s1));
           const uint32_t xl = __byte_perm(v00[j], v01[j], 0x5410), yl = __byte_perm(v00[j], v01[j], 0x7632);
           const uint32_t xh = __byte_perm(v10[j], v11[j], 0x5410), yh = __byte_perm(v10[j], v11[j], 0x7632);
+          // channels 0, 1 of the lane's word by their own codes, 2, 3 by whole bytes c + 16 c' (less those of 0, 1 at the end); 4 .. 7 alike
+          const uint32_t xl8 = __byte_perm(xl, 0u, 0x4341), yl8 = __byte_perm(yl, 0u, 0x4341);
+          const uint32_t xh8 = __byte_perm(xh, 0u, 0x4341), yh8 = __byte_perm(yh, 0u, 0x4341);
           mma_f16_16816(o[4 * j], xl & LO, yl & LO, xh & LO, yh & LO, b0, b1);
-          mma_f16_16816(o[4 * j + 1], xl & HI, yl & HI, xh & HI, yh & HI, b0, b1);
-          const uint32_t xl8 = xl >> 8, yl8 = yl >> 8, xh8 = xh >> 8, yh8 = yh >> 8;
+          mma_f16_16816(o[4 * j + 1], xl & BYTE, yl & BYTE, xh & BYTE, yh & BYTE, b0, b1);
           mma_f16_16816(o[4 * j + 2], xl8 & LO, yl8 & LO, xh8 & LO, yh8 & LO, b0, b1);
-          mma_f16_16816(o[4 * j + 3], xl8 & HI, yl8 & HI, xh8 & HI, yh8 & HI, b0, b1);
+          mma_f16_16816(o[4 * j + 3], xl8, yl8, xh8, yh8, b0, b1);
         }
       }
     }
 
     // ---- the end of the row, or of this warp's part of it; the next row's q is on its way meanwhile ------------------------------------
+    const int b = cs_s[warp].b, h = cs_s[warp].h;
+    __syncwarp();
     if (t < w1) {
-      cs.i = cs.count - 1;
-      cs.next(p);
-      ask_q(cs.b, cs.h);
+      Walk to = cs_s[warp];
+      to.i = to.count - 1;
+      to.next(p);
+      ask_q(to.b, to.h);
+      __syncwarp();
+      if (lane == 0) cs_s[warp] = to;
+      __syncwarp();
     }
 #pragma unroll
     for (int off = 4; off < 32; off <<= 1) {
@@ -569,9 +599,11 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
         float y[8];                                          // channels 64 j + 8 g ..: rows g (even) and g + 8 (odd) of four tiles
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float unit = (i & 1) ? 0x1p20f : 0x1p24f, add = side ? pm_b[j] : pm_a[j];
-          y[2 * i] = fmaf(o[4 * j + i][side], unit, add) * inv;
-          y[2 * i + 1] = fmaf(o[4 * j + i][2 + side], unit, add) * inv;
+          const float add = side ? pm_b[j] : pm_a[j];
+          const float* even = o[4 * j + (i & 2)];
+          const float* at = o[4 * j + i];
+          y[2 * i] = (i & 1) ? fmaf(at[side] - even[side], 0x1p20f, add) * inv : fmaf(at[side], 0x1p24f, add) * inv;
+          y[2 * i + 1] = (i & 1) ? fmaf(at[2 + side] - even[2 + side], 0x1p20f, add) * inv : fmaf(at[2 + side], 0x1p24f, add) * inv;
         }
         if (complete) store_vec<__nv_bfloat16, 8>(p.out + b * p.out_stride + (static_cast<int64_t>(h) * G + head) * D + 64 * j + 8 * g, y);
         else store_f32<8>(part + head * D + 64 * j + 8 * g, y);

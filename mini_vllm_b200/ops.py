@@ -31,8 +31,14 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+# torch's own accessors of the current device and of its current stream's handle, without the objects of the public API around them
+# (0.1 us against 3)
+_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    return _raw_stream(_device()) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
 
 def _need(t: torch.Tensor, dtype, name: str) -> None:
@@ -1197,31 +1203,51 @@ def moe_gemm(x: torch.Tensor, weight: torch.Tensor, rows: ExpertRows, k: int,
 
 
 # ---- rotation in all its forms, and a paged cache of keys and values in 4 bits ------------------------------------------------------
+def _refuse(t: torch.Tensor, dtype, name: str, device: int) -> None:
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (the kernels have no CPU path)")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    raise ValueError(f"{name} is on {t.device}; the current device is cuda:{device}")
+
+
 def _here(*named: tuple) -> None:
-    """Every (tensor, dtype or None, name) is a tensor of the current device (None: not given)."""
-    device = None
+    """Every (tensor or None, dtype, name) is a tensor of that type on the current device.  (None: not given.)"""
+    device = -1
     for t, dtype, name in named:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError(f"{name} must be a CUDA tensor (the kernels have no CPU path)")
-        if dtype is not None and t.dtype != dtype:
-            raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-        if device is None:
-            device = torch.cuda.current_device()
-        if t.device.index != device:
-            raise ValueError(f"{name} is on {t.device}; the current device is cuda:{device}")
-
-
-def _need_rows(t: torch.Tensor | None, name: str) -> None:
-    """[tokens, heads, size] with heads next to each other; only the token stride is free."""
-    if t is not None and t.numel():
-        _heads_contiguous(t, name)
+        if t is not None:
+            if device < 0 and t.is_cuda:
+                device = _device()
+            if t.dtype is not dtype or t.get_device() != device or device < 0:
+                _refuse(t, dtype, name, device)
 
 
 def _need_shape(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
+
+
+def _row_stride(t: torch.Tensor | None, shape: tuple, name: str) -> int:
+    """The token stride of a tensor [tokens, heads, size] of this shape with heads next to each other."""
+    if t is None:
+        return 0
+    if t.shape != shape:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim] = {tuple(shape)}, got {tuple(t.shape)}")
+    s = t.stride()
+    if (s[2] != 1 or (s[1] != shape[2] and shape[1] != 1)) and t.numel():
+        raise ValueError(f"{name} must have contiguous heads")
+    return s[0]
+
+
+def _need_numbers(t: torch.Tensor, n: int, name: str) -> None:
+    if t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be one contiguous number per token, {n} of them")
+
+
+def _need_angles(cos_sin: torch.Tensor) -> tuple[int, int]:
+    if cos_sin.dim() != 2 or not cos_sin.is_contiguous():
+        raise ValueError("cos_sin must be [positions, rotated channels], contiguous")
+    return cos_sin.shape
 
 
 def rotary(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tensor, cos_sin: torch.Tensor, interleaved: bool = False,
@@ -1230,27 +1256,30 @@ def rotary(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tens
     None) by the angles of ``cos_sin`` fp32 ``[positions, rotated channels]`` (cosines, then sines; ``models.layers.rotary`` builds them):
     pairs ``(2i, 2i + 1)`` if ``interleaved``, else halves.  In place, or into ``q_out`` and ``k_out`` (apart from ``q`` and ``k``)."""
     one = q if q is not None else k
-    _need_shape(one is not None, "rotary needs q or k")
-    if one.dtype not in _DTYPE:
-        raise TypeError(f"q and k must be bfloat16 or float32, got {one.dtype}")
-    q_out, k_out = q if q_out is None else q_out, k if k_out is None else k_out
-    _here((q, one.dtype, "q"), (k, one.dtype, "k"), (q_out, one.dtype, "q_out"), (k_out, one.dtype, "k_out"),
-          (positions, torch.int64, "positions"), (cos_sin, torch.float32, "cos_sin"), (status, torch.int32, "status"))
-    for t, like, name in ((q, q, "q"), (k, k, "k"), (q_out, q, "q_out"), (k_out, k, "k_out")):
-        _need_rows(t, name)
-        _need_shape(t is None or (t.dim() == 3 and like is not None and t.shape == like.shape), f"{name} must be [tokens, heads, head_dim], as its input")
+    if one is None or (q is None and q_out is not None) or (k is None and k_out is not None):
+        raise ValueError("rotary needs q or k, and each output its input")
+    dtype = one.dtype
+    if dtype not in _DTYPE:
+        raise TypeError(f"q and k must be bfloat16 or float32, got {dtype}")
+    if q_out is None:
+        q_out = q
+    if k_out is None:
+        k_out = k
+    _here((q, dtype, "q"), (k, dtype, "k"), (q_out, dtype, "q_out"), (k_out, dtype, "k_out"), (positions, torch.int64, "positions"),
+          (cos_sin, torch.float32, "cos_sin"), (status, torch.int32, "status"))
+    if one.dim() != 3:
+        raise ValueError("q and k must be [tokens, heads, head_dim]")
     T, _, d = one.shape
-    for t in (q, k):
-        _need_shape(t is None or (t.shape[0] == T and t.shape[2] == d), "q and k must have the same tokens and head size")
-    _need_shape(positions.numel() == T and positions.is_contiguous(), "positions must be one contiguous number per token")
-    _need_shape(cos_sin.dim() == 2 and cos_sin.is_contiguous(), "cos_sin must be [positions, rotated channels], contiguous")
-    heads = [0 if t is None else t.shape[1] for t in (q, k)]
-    stride = lambda t: 0 if t is None else t.stride(0)
-    rc = _cabi.load().mvb_rotary(_ptr(q), stride(q), _ptr(k), stride(k), _ptr(q_out), stride(q_out), _ptr(k_out), stride(k_out),
-                                 _ptr(positions), _ptr(cos_sin), cos_sin.shape[0], T, heads[0], heads[1], d, cos_sin.shape[1],
-                                 1 if interleaved else 0, _DTYPE[one.dtype], _ptr(status), _stream())
-    _cabi.check(rc, "mvb_rotary")
-    LaunchCounter.add(1 if T else 0)
+    hq, hkv = 0 if q is None else q.shape[1], 0 if k is None else k.shape[1]
+    strides = [_row_stride(t, (T, h, d), name) for t, h, name in ((q, hq, "q"), (k, hkv, "k"), (q_out, hq, "q_out"), (k_out, hkv, "k_out"))]
+    _need_numbers(positions, T, "positions")
+    max_pos, rot = _need_angles(cos_sin)
+    rc = _cabi.load().mvb_rotary(_ptr(q), strides[0], _ptr(k), strides[1], _ptr(q_out), strides[2], _ptr(k_out), strides[3],
+                                 positions.data_ptr(), cos_sin.data_ptr(), max_pos, T, hq, hkv, d, rot, 1 if interleaved else 0,
+                                 _DTYPE[dtype], _ptr(status), _stream())
+    if rc:
+        _cabi.check(rc, "mvb_rotary")
+    LaunchCounter.total += 1 if T else 0
     return q_out, k_out
 
 
@@ -1273,6 +1302,12 @@ class KV4Cache:
             if t.dtype != dtype:
                 raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
             _need_shape(tuple(t.shape) == tuple(want) and t.is_contiguous(), f"{name} must be contiguous {tuple(want)}, got {tuple(t.shape)}")
+            _need_shape(t.device == self.k_codes.device, f"{name} is on {t.device}, k_codes on {self.k_codes.device}")
+        sizes = (shape[0], shape[2], shape[1], shape[3] * 2)       # blocks, tokens of a block, heads, channels
+        object.__setattr__(self, "sizes", sizes)
+        args = _cabi.KV4Cache(*(t.data_ptr() for t in (self.k_codes, self.k_affine, self.v_codes, self.v_affine)), *sizes)
+        object.__setattr__(self, "_args", args)
+        object.__setattr__(self, "_ref", ctypes.byref(args))
 
     @classmethod
     def empty(cls, num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int, device) -> "KV4Cache":
@@ -1287,28 +1322,26 @@ class KV4Cache:
 
     @property
     def num_blocks(self) -> int:
-        return self.k_codes.shape[0]
-
-    @property
-    def num_kv_heads(self) -> int:
-        return self.k_codes.shape[1]
+        return self.sizes[0]
 
     @property
     def block_size(self) -> int:
-        return self.k_codes.shape[2]
+        return self.sizes[1]
+
+    @property
+    def num_kv_heads(self) -> int:
+        return self.sizes[2]
 
     @property
     def head_dim(self) -> int:
-        return self.k_codes.shape[3] * 2
-
-    def named(self) -> tuple:
-        return ((self.k_codes, torch.uint8, "k_codes"), (self.k_affine, torch.bfloat16, "k_affine"), (self.v_codes, torch.uint8, "v_codes"),
-                (self.v_affine, torch.bfloat16, "v_affine"))
+        return self.sizes[3]
 
     def struct(self):
         """The C argument."""
-        return ctypes.byref(_cabi.KV4Cache(_ptr(self.k_codes), _ptr(self.k_affine), _ptr(self.v_codes), _ptr(self.v_affine), self.num_blocks,
-                                           self.block_size, self.num_kv_heads, self.head_dim))
+        args = self._args
+        args.k_codes, args.k_affine = self.k_codes.data_ptr(), self.k_affine.data_ptr()
+        args.v_codes, args.v_affine = self.v_codes.data_ptr(), self.v_affine.data_ptr()
+        return self._ref
 
 
 def rotary_kv4_write(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor | None, cos_sin: torch.Tensor | None,
@@ -1317,36 +1350,42 @@ def rotary_kv4_write(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, p
     """Turns ``q`` (in place or into ``q_out``) and ``k`` as ``rotary`` does, and writes ``k`` and ``v`` in 4 bits to their cache slots
     (-1: none); ``k_in_place``: the turned k also goes back to ``k``.  ``cos_sin`` None: nothing is turned.  bf16; the rotated channels a
     multiple of 16.  Returns the turned q."""
-    q_out = q if q_out is None else q_out
-    _need_shape(q is not None or q_out is None, "q_out needs q")
-    _here((k, torch.bfloat16, "k"), (v, torch.bfloat16, "v"), (q, torch.bfloat16, "q"), (q_out, torch.bfloat16, "q_out"),
-          (positions if cos_sin is not None else None, torch.int64, "positions"), (cos_sin, torch.float32, "cos_sin"),
-          (slot_mapping, torch.int32, "slot_mapping"), (status, torch.int32, "status"), *cache.named())
-    T, d = k.shape[0], cache.head_dim
-    for t, heads, name in ((k, cache.num_kv_heads, "k"), (v, cache.num_kv_heads, "v"), (q, None, "q"), (q_out, None, "q_out")):
-        if t is not None:
-            _need_rows(t, name)
-            _need_shape(t.dim() == 3 and t.shape[0] == T and t.shape[2] == d and heads in (None, t.shape[1]),
-                        f"{name} must be [tokens, heads, head_dim] as the cache has them, got {tuple(t.shape)}")
-    _need_shape(q is None or q.shape == q_out.shape, "q_out must have the shape of q")
-    _need_shape(slot_mapping.numel() == T and slot_mapping.is_contiguous(), "slot_mapping must be one contiguous number per token")
+    if q_out is None:
+        q_out = q
+    elif q is None:
+        raise ValueError("q_out needs q")
+    if cos_sin is None:
+        positions = None
+    elif positions is None:
+        raise ValueError("cos_sin needs positions")
+    bf16 = torch.bfloat16
+    _here((k, bf16, "k"), (v, bf16, "v"), (q, bf16, "q"), (q_out, bf16, "q_out"), (positions, torch.int64, "positions"),
+          (cos_sin, torch.float32, "cos_sin"), (slot_mapping, torch.int32, "slot_mapping"), (cache.k_codes, torch.uint8, "the cache"),
+          (status, torch.int32, "status"))
+    T, hq = k.shape[0], 0 if q is None else q.shape[1]
+    _, _, hkv, d = cache.sizes
+    k_stride, v_stride = _row_stride(k, (T, hkv, d), "k"), _row_stride(v, (T, hkv, d), "v")
+    q_stride, qo_stride = _row_stride(q, (T, hq, d), "q"), _row_stride(q_out, (T, hq, d), "q_out")
+    _need_numbers(slot_mapping, T, "slot_mapping")
     max_pos = rot = 0
     if cos_sin is not None:
-        _need_shape(positions is not None and positions.numel() == T and positions.is_contiguous(), "positions must be one contiguous number per token")
-        _need_shape(cos_sin.dim() == 2 and cos_sin.is_contiguous(), "cos_sin must be [positions, rotated channels], contiguous")
-        max_pos, rot = cos_sin.shape
+        _need_numbers(positions, T, "positions")
+        max_pos, rot = _need_angles(cos_sin)
     rc = _cabi.load().mvb_rotary_kv4_write(
-        _ptr(q), 0 if q is None else q.stride(0), _ptr(q_out), 0 if q is None else q_out.stride(0), _ptr(k), k.stride(0), _ptr(v), v.stride(0),
-        _ptr(positions) if cos_sin is not None else None, _ptr(cos_sin), max_pos, rot, 1 if interleaved else 0, _ptr(slot_mapping),
-        cache.struct(), T, 0 if q is None else q.shape[1], 1 if k_in_place else 0, _ptr(status), _stream())
-    _cabi.check(rc, "mvb_rotary_kv4_write")
-    LaunchCounter.add(1 if T else 0)
+        _ptr(q), q_stride, _ptr(q_out), qo_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride, _ptr(positions), _ptr(cos_sin), max_pos,
+        rot, 1 if interleaved else 0, slot_mapping.data_ptr(), cache.struct(), T, hq, 1 if k_in_place else 0, _ptr(status), _stream())
+    if rc:
+        _cabi.check(rc, "mvb_rotary_kv4_write")
+    LaunchCounter.total += 1 if T else 0
     return q_out
 
 
-def _need_table(block_table: torch.Tensor, rows: int) -> None:
-    _need_shape(block_table.dim() == 2 and block_table.stride(1) == 1 and block_table.shape[0] >= rows and block_table.shape[1] > 0,
-                "block_table must be [sequences, blocks] with neighbouring blocks of a sequence next to each other")
+def _need_table(block_table: torch.Tensor, rows: int) -> tuple[int, int]:
+    """(row stride, width) of a block table with at least this many rows."""
+    shape, stride = block_table.shape, block_table.stride()
+    if len(shape) != 2 or stride[1] != 1 or shape[0] < rows or shape[1] == 0:
+        raise ValueError("block_table must be [sequences, blocks] with neighbouring blocks of a sequence next to each other")
+    return max(stride[0], shape[1]) if shape[0] == 1 else stride[0], shape[1]
 
 
 def kv4_gather(cache: KV4Cache, cu_seqlens_k: torch.Tensor, block_table: torch.Tensor, num_rows: int, k_out: torch.Tensor | None = None,
@@ -1354,18 +1393,22 @@ def kv4_gather(cache: KV4Cache, cu_seqlens_k: torch.Tensor, block_table: torch.T
     """The cached contexts of a ragged step as dense bf16 rows ``[num_rows, Hkv, D]``, as ``prefill_attn`` reads them: sequence ``b`` from row
     ``cu_seqlens_k[b]`` on.  ``num_rows`` is the host's count of them; rows behind the last sequence stay as they are."""
     _here((cu_seqlens_k, torch.int32, "cu_seqlens_k"), (block_table, torch.int32, "block_table"), (k_out, torch.bfloat16, "k_out"),
-          (v_out, torch.bfloat16, "v_out"), (status, torch.int32, "status"), *cache.named())
+          (v_out, torch.bfloat16, "v_out"), (cache.k_codes, torch.uint8, "the cache"), (status, torch.int32, "status"))
     n = cu_seqlens_k.numel() - 1
     _need_shape(n >= 0 and cu_seqlens_k.is_contiguous(), "cu_seqlens_k must be [sequences + 1], contiguous")
-    _need_table(block_table, n)
-    shape = (num_rows, cache.num_kv_heads, cache.head_dim)
-    k_out, v_out = (torch.empty(shape, dtype=torch.bfloat16, device=cu_seqlens_k.device) if t is None else t for t in (k_out, v_out))
-    for t, name in ((k_out, "k_out"), (v_out, "v_out")):
-        _need_shape(tuple(t.shape) == shape and t.is_contiguous(), f"{name} must be contiguous {shape}")
-    rc = _cabi.load().mvb_kv4_gather(cache.struct(), _ptr(cu_seqlens_k), _ptr(block_table), block_table.stride(0), block_table.shape[1], n,
-                                     num_rows, _ptr(k_out), _ptr(v_out), _ptr(status), _stream())
-    _cabi.check(rc, "mvb_kv4_gather")
-    LaunchCounter.add(1 if n and num_rows else 0)
+    stride, width = _need_table(block_table, n)
+    shape = (num_rows, cache.sizes[2], cache.sizes[3])
+    if k_out is None:
+        k_out = torch.empty(shape, dtype=torch.bfloat16, device=cu_seqlens_k.device)
+    if v_out is None:
+        v_out = torch.empty(shape, dtype=torch.bfloat16, device=cu_seqlens_k.device)
+    _need_shape(k_out.shape == shape and k_out.is_contiguous() and v_out.shape == shape and v_out.is_contiguous(),
+                f"k_out and v_out must be contiguous {shape}")
+    rc = _cabi.load().mvb_kv4_gather(cache.struct(), cu_seqlens_k.data_ptr(), block_table.data_ptr(), stride, width, n, num_rows,
+                                     k_out.data_ptr(), v_out.data_ptr(), _ptr(status), _stream())
+    if rc:
+        _cabi.check(rc, "mvb_kv4_gather")
+    LaunchCounter.total += 1 if n and num_rows else 0
     return k_out, v_out
 
 
@@ -1382,51 +1425,50 @@ def decode_attn4(q: torch.Tensor, cache: KV4Cache, cache_seqlens: torch.Tensor, 
                  status: torch.Tensor | None = None, softcap: float = 0.0, out_scale: float = 1.0) -> torch.Tensor:
     """``decode_attn`` over a cache in 4 bits: ``q [B, Hq, D]`` bf16, one new token per sequence.  ``spans`` int32 ``[B, Hkv, budget]``
     (``kv4_select``): only these spans of 64 tokens are read, each listed once, entries below 0 skipped.  No plan is needed."""
-    _here((q, torch.bfloat16, "q"), (cache_seqlens, torch.int32, "cache_seqlens"), (block_table, torch.int32, "block_table"),
-          (workspace, torch.uint8, "workspace"), (spans, torch.int32, "spans"), (out, torch.bfloat16, "out"), (status, torch.int32, "status"),
-          *cache.named())
-    _need_rows(q, "q")
-    B, hq, d = q.shape
-    _need_shape(d == cache.head_dim, f"q has heads of {d}, the cache of {cache.head_dim}")
-    _need_shape(cache_seqlens.numel() >= B and cache_seqlens.is_contiguous(), "cache_seqlens must be one contiguous number per sequence")
-    _need_table(block_table, B)
-    if spans is not None:
-        _need_shape(spans.dim() == 3 and spans.shape[:2] == (B, cache.num_kv_heads) and spans.is_contiguous(),
-                    "spans must be contiguous [sequences, kv heads, budget]")
+    bf16, i32 = torch.bfloat16, torch.int32
     if out is None:
-        out = torch.empty(B, hq, d, dtype=torch.bfloat16, device=q.device)
-    _need_rows(out, "out")
-    _need_shape(out.shape == q.shape, "out must have the shape of q")
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    _here((q, bf16, "q"), (cache_seqlens, i32, "cache_seqlens"), (block_table, i32, "block_table"), (workspace, torch.uint8, "workspace"),
+          (spans, i32, "spans"), (out, bf16, "out"), (cache.k_codes, torch.uint8, "the cache"), (status, i32, "status"))
+    _, _, hkv, d = cache.sizes
+    _need_shape(q.dim() == 3, "q must be [sequences, heads, head_dim]")
+    B, hq, _ = q.shape
+    q_stride, out_stride = _row_stride(q, (B, hq, d), "q"), _row_stride(out, (B, hq, d), "out")
+    _need_shape(cache_seqlens.numel() >= B and cache_seqlens.is_contiguous(), "cache_seqlens must be one contiguous number per sequence")
+    stride, width = _need_table(block_table, B)
+    budget = 0
+    if spans is not None:
+        _need_shape(spans.dim() == 3 and spans.shape[:2] == (B, hkv) and spans.is_contiguous(), "spans must be contiguous [sequences, kv heads, budget]")
+        budget = spans.shape[2]
     rc = _cabi.load().mvb_decode_attn4(
-        _ptr(q), q.stride(0), cache.struct(), _ptr(cache_seqlens), _ptr(block_table), block_table.stride(0), block_table.shape[1], _ptr(spans),
-        0 if spans is None else spans.shape[2], B, hq, float(scale), window_left, float(softcap), float(out_scale), _ptr(out), out.stride(0),
-        _ptr(workspace), workspace.numel(), _ptr(status), _stream())
-    _cabi.check(rc, "mvb_decode_attn4")
-    LaunchCounter.add(1 if B else 0)
+        q.data_ptr(), q_stride, cache.struct(), cache_seqlens.data_ptr(), block_table.data_ptr(), stride, width, _ptr(spans), budget, B, hq,
+        scale, window_left, softcap, out_scale, out.data_ptr(), out_stride, workspace.data_ptr(), workspace.numel(), _ptr(status), _stream())
+    if rc:
+        _cabi.check(rc, "mvb_decode_attn4")
+    LaunchCounter.total += 1 if B else 0
     return out
 
 
 def kv4_summaries(cache: KV4Cache) -> torch.Tensor:
     """Room for the bounds of every span of the cache's keys (written by ``kv4_summarise``, read by ``kv4_select``)."""
-    return torch.zeros(cache.num_blocks, cache.num_kv_heads, cache.block_size // 64, 2, cache.head_dim, dtype=torch.bfloat16,
-                       device=cache.k_codes.device)
-
-
-def _need_summaries(summaries: torch.Tensor, d: int) -> None:
-    _need_shape(summaries.dim() == 5 and summaries.shape[3:] == (2, d) and summaries.is_contiguous(),
-                "summaries must be contiguous [blocks, kv heads, block_size / 64, 2, head_dim]")
+    blocks, size, hkv, d = cache.sizes
+    return torch.zeros(blocks, hkv, size // 64, 2, d, dtype=torch.bfloat16, device=cache.k_codes.device)
 
 
 def kv4_summarise(cache: KV4Cache, slot_mapping: torch.Tensor, summaries: torch.Tensor, status: torch.Tensor | None = None) -> torch.Tensor:
     """Renews the bounds of the spans that a step has just written to: per channel the least and the greatest key over the span's rows up to
     the step's last one.  ``slot_mapping`` as for the write, a sequence's tokens next to each other and in order."""
-    _here((slot_mapping, torch.int32, "slot_mapping"), (summaries, torch.bfloat16, "summaries"), (status, torch.int32, "status"), *cache.named())
-    _need_summaries(summaries, cache.head_dim)
-    _need_shape(summaries.shape[:3] == (cache.num_blocks, cache.num_kv_heads, cache.block_size // 64), "summaries must be those of the cache")
-    _need_shape(slot_mapping.is_contiguous(), "slot_mapping must be contiguous")
-    rc = _cabi.load().mvb_kv4_summarise(cache.struct(), _ptr(slot_mapping), slot_mapping.numel(), _ptr(summaries), _ptr(status), _stream())
-    _cabi.check(rc, "mvb_kv4_summarise")
-    LaunchCounter.add(1 if slot_mapping.numel() else 0)
+    _here((slot_mapping, torch.int32, "slot_mapping"), (summaries, torch.bfloat16, "summaries"), (cache.k_codes, torch.uint8, "the cache"),
+          (status, torch.int32, "status"))
+    blocks, size, hkv, d = cache.sizes
+    _need_shape(summaries.shape == (blocks, hkv, size // 64, 2, d) and summaries.is_contiguous(),
+                "summaries must be contiguous [blocks, kv heads, block_size / 64, 2, head_dim], as the cache has them")
+    T = slot_mapping.numel()
+    _need_numbers(slot_mapping, T, "slot_mapping")
+    rc = _cabi.load().mvb_kv4_summarise(cache.struct(), slot_mapping.data_ptr(), T, summaries.data_ptr(), _ptr(status), _stream())
+    if rc:
+        _cabi.check(rc, "mvb_kv4_summarise")
+    LaunchCounter.total += 1 if T else 0
     return summaries
 
 
@@ -1437,18 +1479,21 @@ def kv4_select(q: torch.Tensor, summaries: torch.Tensor, cache_seqlens: torch.Te
     span are always among them, and of equal bounds the lower index is taken."""
     _here((q, torch.bfloat16, "q"), (summaries, torch.bfloat16, "summaries"), (cache_seqlens, torch.int32, "cache_seqlens"),
           (block_table, torch.int32, "block_table"), (out, torch.int32, "out"), (status, torch.int32, "status"))
-    _need_rows(q, "q")
+    _need_shape(q.dim() == 3 and summaries.dim() == 5 and summaries.is_contiguous(), "q must be [sequences, heads, head_dim], summaries contiguous "
+                "[blocks, kv heads, block_size / 64, 2, head_dim]")
     B, hq, d = q.shape
-    _need_summaries(summaries, d)
+    q_stride = _row_stride(q, (B, hq, d), "q")
     blocks, hkv, per_block = summaries.shape[:3]
-    _need_shape(per_block * 64 == block_size, f"summaries have {per_block} spans a block, blocks have {block_size} tokens")
+    _need_shape(per_block * 64 == block_size and summaries.shape[3:] == (2, d), f"summaries {tuple(summaries.shape)} are not those of blocks of "
+                f"{block_size} tokens and heads of {d}")
     _need_shape(cache_seqlens.numel() >= B and cache_seqlens.is_contiguous(), "cache_seqlens must be one contiguous number per sequence")
-    _need_table(block_table, B)
+    stride, width = _need_table(block_table, B)
     if out is None:
-        out = torch.empty(B, hkv, max(budget, 0), dtype=torch.int32, device=q.device)
-    _need_shape(tuple(out.shape) == (B, hkv, budget) and out.is_contiguous(), "out must be contiguous [sequences, kv heads, budget]")
-    rc = _cabi.load().mvb_kv4_select(_ptr(q), q.stride(0), _ptr(summaries), blocks, block_size, _ptr(cache_seqlens), _ptr(block_table),
-                                     block_table.stride(0), block_table.shape[1], B, hq, hkv, d, budget, _ptr(out), _ptr(status), _stream())
-    _cabi.check(rc, "mvb_kv4_select")
-    LaunchCounter.add(1 if B else 0)
+        out = torch.empty((B, hkv, max(budget, 0)), dtype=torch.int32, device=q.device)
+    _need_shape(out.shape == (B, hkv, budget) and out.is_contiguous(), "out must be contiguous [sequences, kv heads, budget]")
+    rc = _cabi.load().mvb_kv4_select(q.data_ptr(), q_stride, summaries.data_ptr(), blocks, block_size, cache_seqlens.data_ptr(),
+                                     block_table.data_ptr(), stride, width, B, hq, hkv, d, budget, out.data_ptr(), _ptr(status), _stream())
+    if rc:
+        _cabi.check(rc, "mvb_kv4_select")
+    LaunchCounter.total += 1 if B else 0
     return out
