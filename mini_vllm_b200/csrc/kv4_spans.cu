@@ -23,14 +23,16 @@ struct SummariseParams {
   int* dev_status;
 };
 
-// A warp per (token, head): the last of a step's tokens inside a span renews the span's bounds from the rows up to its own.  A token is the
-// last one when the next row of the step does not follow it in the same span.
-template <int D>
+// The last of a step's tokens inside a span renews the span's bounds from the rows up to its own; a token is the last one when the next row
+// of the step does not follow it in the same span.  WARPS warps share a (token, head): eight where a step has few tokens (decoding: nearly
+// every token is such a last one, and a span is then one round of loads), one where it has many (prompts: one token in 64 has work).
+template <int D, int WARPS>
 __global__ void __launch_bounds__(256) kv4_summarise_kernel(const SummariseParams p) {
-  constexpr int LPH = D / 8, RPW = 32 / LPH;
+  constexpr int LPH = D / 8, RPW = 32 / LPH, ROUNDS = kKv4Span / (RPW * WARPS);
   constexpr uint32_t FULL = 0xffffffffu;
-  const int lane = threadIdx.x & 31, c = lane % LPH, sub = lane / LPH;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  __shared__ float part_s[WARPS > 1 ? WARPS : 1][2][D];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane % LPH, sub = lane / LPH;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * (8 / WARPS) + (WARPS > 1 ? 0 : warp);
   if (t >= p.tokens) return;
   const int64_t slot = p.slots[t];
   if (slot < 0 || slot >= p.num_slots) {
@@ -43,15 +45,31 @@ __global__ void __launch_bounds__(256) kv4_summarise_kernel(const SummariseParam
   const int64_t block = slot / p.block_size;
   const int in_block = static_cast<int>(slot - block * p.block_size), span = in_block / kKv4Span;
   const int64_t row0 = kv4_row(block, p.hkv, h, p.block_size, span * kKv4Span);
+  const int first = (WARPS > 1 ? warp : 0) * RPW + sub;
   float lo[8], hi[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) { lo[e] = INFINITY; hi[e] = -INFINITY; }
-#pragma unroll 4
-  for (int r = sub; r <= end; r += RPW) {
-    float y[8];
-    kv4_values(__ldg(p.k_codes + (row0 + r) * (D / 8) + kv4_word<D>(c, true)), __ldg(p.k_affine + (row0 + r) * (D / 64) + (c >> 3)), y);
+  constexpr int AT_ONCE = ROUNDS < 8 ? ROUNDS : 8;
+#pragma unroll 1
+  for (int base = 0; base < ROUNDS; base += AT_ONCE) {
+    uint32_t word[AT_ONCE], affine[AT_ONCE];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) { lo[e] = fminf(lo[e], y[e]); hi[e] = fmaxf(hi[e], y[e]); }
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const int r = first + (base + i) * RPW * WARPS;
+      if (r <= end) {
+        word[i] = __ldg(p.k_codes + (row0 + r) * (D / 8) + kv4_word<D>(c, true));
+        affine[i] = __ldg(p.k_affine + (row0 + r) * (D / 64) + (c >> 3));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      if (first + (base + i) * RPW * WARPS <= end) {
+        float y[8];
+        kv4_values(word[i], affine[i], y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { lo[e] = fminf(lo[e], y[e]); hi[e] = fmaxf(hi[e], y[e]); }
+      }
+    }
   }
 #pragma unroll
   for (int off = LPH; off < 32; off <<= 1) {
@@ -62,9 +80,24 @@ __global__ void __launch_bounds__(256) kv4_summarise_kernel(const SummariseParam
     }
   }
   __nv_bfloat16* out = p.summaries + ((block * p.hkv + h) * (p.block_size / kKv4Span) + span) * (2 * D);
-  if (sub == 0) {
-    store_vec<__nv_bfloat16, 8>(out + c * 8, lo);
-    store_vec<__nv_bfloat16, 8>(out + D + c * 8, hi);
+  if constexpr (WARPS == 1) {
+    if (sub == 0) {
+      store_vec<__nv_bfloat16, 8>(out + c * 8, lo);
+      store_vec<__nv_bfloat16, 8>(out + D + c * 8, hi);
+    }
+  } else {
+    if (sub == 0) {
+      store_f32<8>(&part_s[warp][0][c * 8], lo);
+      store_f32<8>(&part_s[warp][1][c * 8], hi);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * D; i += 256) {
+      const int side = i / D, e = i % D;
+      float y = part_s[0][side][e];
+#pragma unroll
+      for (int w = 1; w < WARPS; ++w) y = side ? fmaxf(y, part_s[w][side][e]) : fminf(y, part_s[w][side][e]);
+      out[i] = __float2bfloat16_rn(y);
+    }
   }
 }
 
@@ -113,70 +146,104 @@ __device__ __forceinline__ int block_prefix(int v, int* scratch, int& total) {
   return before + x - v;
 }
 
-// A block per (KV head, sequence): the sums, then the budget-th greatest by radix selection on their bits, eight at a time, then the
-// chosen indices in order (of equal sums the lower ones).
+// A cluster of CL blocks per (KV head, sequence).  Its blocks share the spans and send their sums' bits, as keys that ascend with the sum, to the
+// first one, which finds the budget-th greatest by radix selection, eight bits at a time from the first one in which keys differ, and
+// writes the chosen indices in order (of equal sums the lower ones).  Eight lanes take a span, so that a warp has four spans in flight.
+// 4 sequences of 9000-40000 tokens, 8 KV heads: 67 us with one block and one span a warp, XX with eight blocks.
 template <int D>
 __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(const SelectParams p) {
   constexpr uint32_t FULL = 0xffffffffu;
-  constexpr int CPL = D / 32;                                // channels of a lane
+  constexpr int PIECES = D / 64;                             // of eight channels, of a lane
   extern __shared__ uint64_t keys[];
+  __shared__ __align__(16) float q_s[kSelectMaxGroup * D];
   __shared__ int hist[256], scratch[kSelectThreads / 32], pick_s[2];
-  const int h = blockIdx.x, b = blockIdx.y;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ unsigned long long differ_s;
+  uint32_t cl, rank;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(cl));
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const int h = blockIdx.x / cl, b = blockIdx.y;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane & 7;
   const int n = p.seqlens[b];
   int32_t* out = p.out + (static_cast<int64_t>(b) * p.hkv + h) * p.budget;
   int count = n > 0 ? (n + kKv4Span - 1) / kKv4Span : 0;
-  const int most = p.table_width * (p.block_size / kKv4Span);
+  const int per_block = p.block_size / kKv4Span, most = p.table_width * per_block;
   if (count > most) {                                        // a length that its block list does not hold
     if (threadIdx.x == 0) report(p.dev_status, kDevBadLength, b);
     count = most;
   }
-  if (count <= p.budget) {
-    for (int i = threadIdx.x; i < p.budget; i += kSelectThreads) out[i] = i < count ? i : -1;
+  if (count <= p.budget) {                                   // (the whole cluster)
+    if (rank == 0)
+      for (int i = threadIdx.x; i < p.budget; i += kSelectThreads) out[i] = i < count ? i : -1;
     return;
   }
-  float q[kSelectMaxGroup][CPL];
+  if (cl > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");      // (every block has begun before one writes to another)
+  const int32_t* table = p.block_table + b * p.table_stride;
+  for (int i = threadIdx.x; i < p.group * D; i += kSelectThreads)
+    q_s[i] = __bfloat162float(p.q[b * p.q_stride + static_cast<int64_t>(h) * p.group * D + i]);
+  if (threadIdx.x == 0) differ_s = 0;
+  __syncthreads();
+  if (cl > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  uint32_t keys_0;                                           // the first block's keys, in the cluster's shared memory
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(keys_0) : "r"(smem_u32(keys)));
+  const int stride = cl * (kSelectThreads / 8);
+  for (int base = (rank * (kSelectThreads / 32) + warp) * 4; base < count; base += stride) {     // warp-uniform
+    const int s = base + (lane >> 3);
+    const bool inner = s > 0 && s < count - 1;               // the first and the last one are taken anyway
+    int64_t block = -1;
+    if (inner) block = __ldg(table + s / per_block);
+    const bool ok = block >= 0 && block < p.num_blocks;
+    if (inner && !ok && sub == 0) report(p.dev_status, kDevBadBlock, b);
+    const __nv_bfloat16* at = p.summaries + ((ok ? block * p.hkv + h : 0) * per_block + (ok ? s % per_block : 0)) * (2 * D);
+    double sum = 0.0, sum2 = 0.0;
+    float lo[PIECES][8], hi[PIECES][8];
 #pragma unroll
-  for (int g = 0; g < kSelectMaxGroup; ++g) {
+    for (int i = 0; i < PIECES; ++i) {
+      load_vec<__nv_bfloat16, 8>(at + (i * 8 + sub) * 8, lo[i]);
+      load_vec<__nv_bfloat16, 8>(at + D + (i * 8 + sub) * 8, hi[i]);
+    }
+    for (int g = 0; g < p.group; ++g) {
 #pragma unroll
-    for (int e = 0; e < CPL; ++e)
-      q[g][e] = g < p.group ? __bfloat162float(p.q[b * p.q_stride + (static_cast<int64_t>(h) * p.group + g) * D + lane * CPL + e]) : 0.f;
-  }
-  const int per_block = p.block_size / kKv4Span;
-  for (int s = warp; s < count; s += kSelectThreads / 32) {
-    const int64_t block = p.block_table[b * p.table_stride + s / per_block];
-    double sum = 0.0;
-    if (block >= 0 && block < p.num_blocks) {
-      const __nv_bfloat16* at = p.summaries + ((block * p.hkv + h) * per_block + s % per_block) * (2 * D) + lane * CPL;
-      float lo[CPL], hi[CPL];
+      for (int i = 0; i < PIECES; ++i) {
+        float q[8];
+        load_f32<8>(q_s + g * D + (i * 8 + sub) * 8, q);
 #pragma unroll
-      for (int e = 0; e < CPL; e += 2) {
-        const uint32_t a = __ldg(reinterpret_cast<const uint32_t*>(at + e)), z = __ldg(reinterpret_cast<const uint32_t*>(at + D + e));
-        lo[e] = bf16_lo(a); lo[e + 1] = bf16_hi(a); hi[e] = bf16_lo(z); hi[e + 1] = bf16_hi(z);
-      }
-#pragma unroll
-      for (int g = 0; g < kSelectMaxGroup; ++g) {
-        if (g < p.group) {
-#pragma unroll
-          for (int e = 0; e < CPL; ++e) sum += static_cast<double>(fmaxf(q[g][e] * lo[e], q[g][e] * hi[e]));
+        for (int e = 0; e < 8; e += 2) {
+          sum += static_cast<double>(fmaxf(q[e] * lo[i][e], q[e] * hi[i][e]));
+          sum2 += static_cast<double>(fmaxf(q[e + 1] * lo[i][e + 1], q[e + 1] * hi[i][e + 1]));
         }
       }
-    } else if (lane == 0) {
-      report(p.dev_status, kDevBadBlock, b);
     }
+    sum += sum2;
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(FULL, sum, off);
-    if (lane == 0) keys[s] = s == 0 || s == count - 1 ? ~0ull : order_key(sum);
+    for (int off = 4; off > 0; off >>= 1) sum += __shfl_xor_sync(FULL, sum, off);
+    if (sub == 0 && s < count)
+      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(keys_0 + 8u * s), "l"(ok ? order_key(sum) : order_key(0.0)) : "memory");
   }
+  if (cl > 1) {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (rank != 0) return;
+  } else {
+    __syncthreads();
+  }
+  // ---- the first block: which of the inner spans -------------------------------------------------------------------------------------
+  const uint64_t sample = keys[1];
+  uint64_t differ = 0;
+  for (int s = 1 + threadIdx.x; s < count - 1; s += kSelectThreads) differ |= keys[s] ^ sample;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) differ |= __shfl_xor_sync(FULL, differ, off);
+  if (lane == 0 && differ != 0) atomicOr(&differ_s, static_cast<unsigned long long>(differ));
   __syncthreads();
-  uint64_t prefix = 0, mask = 0;
-  int need = p.budget;                                       // still to be found among the keys that share the prefix
-  for (int shift = 56; shift >= 0; shift -= 8) {
+  differ = differ_s;
+  int top = 64 - __clzll(static_cast<long long>(differ));    // bits from here on are the same in all keys
+  uint64_t mask = top == 64 ? 0 : ~0ull << top, prefix = sample & mask;
+  int need = p.budget - 2;                                   // still to be found among the keys that share the prefix
+  while (top > 0 && need > 0) {
+    const int shift = max(top - 8, 0), width = top - shift;
     hist[threadIdx.x] = 0;
     __syncthreads();
-    for (int s = threadIdx.x; s < count; s += kSelectThreads) {
+    for (int s = 1 + threadIdx.x; s < count - 1; s += kSelectThreads) {
       const uint64_t k = keys[s];
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
+      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << width) - 1)], 1);
     }
     __syncthreads();
     const int bin = 255 - static_cast<int>(threadIdx.x), mine = hist[bin];
@@ -185,11 +252,12 @@ __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(const Select
     if (above < need && above + mine >= need) { pick_s[0] = bin; pick_s[1] = need - above; }
     __syncthreads();
     prefix |= static_cast<uint64_t>(pick_s[0]) << shift;
-    mask |= 255ull << shift;
+    mask |= ((1ull << width) - 1) << shift;
     need = pick_s[1];
-    const bool all = hist[pick_s[0]] == need;                // every key of this bin is taken
+    top = shift;
+    const bool all = hist[pick_s[0]] == need;                // every key that shares the prefix is taken
     __syncthreads();
-    if (all) { need = 0x7fffffff; break; }
+    if (all) break;
   }
   // a thread walks a run of neighbouring spans; keys equal to the prefix (under the mask) are taken up to `need`, the lower indices first
   const int run = (count + kSelectThreads - 1) / kSelectThreads;
@@ -197,17 +265,19 @@ __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(const Select
   int equal = 0, over = 0, total;
   for (int s = first; s < last; ++s) {
     const uint64_t k = keys[s] & mask;
-    equal += k == prefix;
-    over += k > prefix;
+    const bool ends = s == 0 || s == count - 1;
+    over += ends || k > prefix;
+    equal += !ends && k == prefix;
   }
   const int equal_before = block_prefix(equal, scratch, total);
-  const int equal_taken = max(0, min(equal, need - equal_before));
-  int at = block_prefix(over + equal_taken, scratch, total);
-  int left = equal_taken;
+  int left = max(0, min(equal, need - equal_before));
+  int at = block_prefix(over + left, scratch, total);
   for (int s = first; s < last; ++s) {
     const uint64_t k = keys[s] & mask;
-    if (k > prefix || (k == prefix && left > 0)) {
-      left -= k == prefix;
+    const bool ends = s == 0 || s == count - 1;
+    bool take = ends || k > prefix;
+    if (!take && k == prefix && left > 0) { take = true; --left; }
+    if (take) {
       if (at < p.budget) out[at] = s;
       ++at;
     }
@@ -231,12 +301,19 @@ extern "C" int mvb_kv4_summarise(const mvb_kv4_cache* cache, const int32_t* slot
   p.slots = slot_mapping; p.summaries = static_cast<__nv_bfloat16*>(summaries);
   p.num_slots = cache->num_blocks * cache->block_size;
   p.tokens = num_tokens; p.hkv = cache->num_kv_heads; p.block_size = cache->block_size; p.dev_status = dev_status;
-  const dim3 grid((static_cast<unsigned>(num_tokens) + 7) / 8, cache->num_kv_heads);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (cache->head_dim == 64) kv4_summarise_kernel<64><<<grid, 256, 0, st>>>(p);
-  else if (cache->head_dim == 128) kv4_summarise_kernel<128><<<grid, 256, 0, st>>>(p);
-  else kv4_summarise_kernel<256><<<grid, 256, 0, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? kOk : kLaunchFailed;
+  // a block for each (token, head) up to a few per SM's place for them; more are mostly prompts
+  const bool few = static_cast<int64_t>(num_tokens) * cache->num_kv_heads <= 4096;
+  const dim3 grid(few ? num_tokens : (static_cast<unsigned>(num_tokens) + 7) / 8, cache->num_kv_heads);
+  auto launch = [&](auto tag) -> int {
+    constexpr int D = decltype(tag)::value;
+    if (few) kv4_summarise_kernel<D, 8><<<grid, 256, 0, st>>>(p);
+    else kv4_summarise_kernel<D, 1><<<grid, 256, 0, st>>>(p);
+    return cudaGetLastError() == cudaSuccess ? kOk : kLaunchFailed;
+  };
+  if (cache->head_dim == 64) return launch(std::integral_constant<int, 64>{});
+  if (cache->head_dim == 128) return launch(std::integral_constant<int, 128>{});
+  return launch(std::integral_constant<int, 256>{});
 }
 
 extern "C" int mvb_kv4_select(const void* q, int64_t q_row_stride, const void* summaries, int64_t num_blocks, int block_size,
@@ -257,17 +334,28 @@ extern "C" int mvb_kv4_select(const void* q, int64_t q_row_stride, const void* s
   p.table_width = table_width; p.hkv = num_kv_heads; p.group = num_q_heads / num_kv_heads; p.block_size = block_size; p.budget = budget;
   p.dev_status = dev_status;
   const size_t smem = sizeof(uint64_t) * static_cast<size_t>(table_width) * (block_size / kKv4Span);
-  const dim3 grid(num_kv_heads, num_seqs);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // blocks enough for every SM to have two, a cluster of at most eight for one (sequence, head)
+  int cl = 1;
+  while (cl < 8 && static_cast<int64_t>(num_kv_heads) * num_seqs * cl < 2 * sm_count()) cl *= 2;
   auto launch = [&](auto tag) -> int {
     constexpr int D = decltype(tag)::value;
     struct Tag {};
-    if (smem > 40 * 1024) {
+    if (smem > 32 * 1024) {
       const int rc = opt_in_dynamic_smem<Tag>(reinterpret_cast<const void*>(&kv4_select_kernel<D>), smem);
       if (rc != kOk) return rc;
     }
-    kv4_select_kernel<D><<<grid, kSelectThreads, smem, st>>>(p);
-    return cudaGetLastError() == cudaSuccess ? kOk : kLaunchFailed;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cl; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(num_kv_heads) * cl, num_seqs);
+    cfg.blockDim = dim3(kSelectThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kv4_select_kernel<D>, p) == cudaSuccess ? kOk : kLaunchFailed;
   };
   if (head_dim == 64) return launch(std::integral_constant<int, 64>{});
   if (head_dim == 128) return launch(std::integral_constant<int, 128>{});

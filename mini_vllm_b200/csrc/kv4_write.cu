@@ -32,13 +32,43 @@ struct Kv4WriteParams {
   int* dev_status;
 };
 
-// round(t / s) for 0 <= t <= about 15 s, as the correctly rounded quotient rounds: the product with the approximate reciprocal decides
-// unless it lies within 2^-10 of a half, which a division then settles
-__device__ __forceinline__ uint32_t kv4_code(float t, float s, float r) {
-  float f = t * r;
-  const float n = rintf(f);
-  if (fabsf(fabsf(f - n) - 0.5f) < 0x1p-10f) f = __fdiv_rn(t, s);
-  return static_cast<uint32_t>(fminf(rintf(f), 15.f));
+// The codes round(t / s), 0 <= t <= 15 s (1 + 2^-8), of eight channels as a word, r within 2^-22 of 1 / s.  Adding 1.5 * 2^23 rounds t r to a
+// whole number that then stands in the float's last bits.  Where t r comes near a half the code is decided exactly: n s and the middle
+// (n + 1/2) s between two codes take 13 bits, so t - n s against s / 2 is exact, and a quotient is rounded as its correctly rounded fp32
+// value would be (that is a half only where t is the middle itself: t's last place is never finer than the quotient's).
+__device__ __forceinline__ uint32_t kv4_codes(const float (&t)[8], float s, float r) {
+  constexpr float kRound = 12582912.f;
+  constexpr uint32_t kPlaces = 0x11111111u;                  // one in each of the eight 4-bit places
+  float n[8], worst = 0.f;
+  uint32_t word = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float f = t[e] * r, z = f + kRound;
+    n[e] = z - kRound;
+    worst = fmaxf(worst, fabsf(f - n[e]));
+    word += __float_as_uint(z) << kv4_shift(e);
+  }
+  word -= __float_as_uint(kRound) * kPlaces;                 // modulo 2^32: the codes alone remain
+  if (worst > 0.5f - 0x1p-16f) {
+    word = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float off = fmaf(-n[e], s, t[e]), over = fabsf(off) - 0.5f * s;
+      const bool odd = (__float_as_uint(n[e] + kRound) & 1u) != 0;
+      if (over > 0.f || (over == 0.f && odd)) n[e] += off > 0.f ? 1.f : -1.f;
+      word |= (__float_as_uint(n[e] + kRound) & 15u) << kv4_shift(e);
+    }
+  }
+  return word;
+}
+
+__device__ __forceinline__ uint32_t min_bf16x2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 x = __hmin2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&x);
+}
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 x = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&x);
 }
 
 template <int D, bool INTER, int ITEMS>
@@ -130,27 +160,25 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4WriteParams p) 
     if (row < rows && is_q) *reinterpret_cast<uint4*>(p.q_out + static_cast<int64_t>(t) * p.qo_stride + static_cast<int64_t>(row) * D + c * 8) = x[i];
     if (row < rows && !is_q && !is_v && p.k_in_place && turns && ok)
       *reinterpret_cast<uint4*>(p.k + static_cast<int64_t>(t) * p.k_stride + static_cast<int64_t>(row - p.hq) * D + c * 8) = x[i];
-    if (slot < 0) continue;                                  // warp-uniform
-    // the group's bounds; every lane of the warp takes part (rows of q and rows past the last one for nothing)
-    float lo = fminf(fminf(fminf(y[0], y[1]), fminf(y[2], y[3])), fminf(fminf(y[4], y[5]), fminf(y[6], y[7])));
-    float hi = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
+    if (slot < 0 || __all_sync(FULL, is_q || row >= rows)) continue;      // warp-uniform
+    // the group's least and greatest value, as the pair (least, -greatest): one minimum for both; every lane of the warp takes part
+    const uint32_t least2 = min_bf16x2(min_bf16x2(x[i].x, x[i].y), min_bf16x2(x[i].z, x[i].w));
+    const uint32_t most2 = max_bf16x2(max_bf16x2(x[i].x, x[i].y), max_bf16x2(x[i].z, x[i].w));
+    uint32_t pair = min_bf16x2(__byte_perm(least2, most2, 0x5410) ^ 0x80000000u, __byte_perm(least2, most2, 0x7632) ^ 0x80000000u);
 #pragma unroll
-    for (int off = 1; off < 8; off <<= 1) {
-      lo = fminf(lo, __shfl_xor_sync(FULL, lo, off));
-      hi = fmaxf(hi, __shfl_xor_sync(FULL, hi, off));
-    }
+    for (int off = 1; off < 8; off <<= 1) pair = min_bf16x2(pair, __shfl_xor_sync(FULL, pair, off));
+    const float lo = bf16_lo(pair), hi = -bf16_hi(pair);
     if (row >= rows || is_q) continue;
     const float scale = __bfloat162float(__float2bfloat16_rn(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f)));
-    uint32_t word = 0;
-    if (scale > 0.f) {
-      const bool usual = scale > 0x1p-100f && scale < 0x1p100f;            // (its reciprocal is a normal number)
-      const float r = fast_rcp(scale);
+    float d[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float d = __fsub_rn(y[e], lo);
-        const uint32_t code = usual ? kv4_code(d, scale, r) : static_cast<uint32_t>(fminf(rintf(__fdiv_rn(d, scale)), 15.f));
-        word |= (code & 15u) << kv4_shift(e);
-      }
+    for (int e = 0; e < 8; ++e) d[e] = __fsub_rn(y[e], lo);
+    uint32_t word = 0;
+    if (scale > 0x1p-100f && scale < 0x1p100f) {             // the usual case: the reciprocal is a normal number, no code passes 15
+      word = kv4_codes(d, scale, fast_rcp(scale));
+    } else if (scale > 0.f) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) word |= (static_cast<uint32_t>(fminf(rintf(__fdiv_rn(d[e], scale)), 15.f)) & 15u) << kv4_shift(e);
     }
     const int h = row - p.hq - (is_v ? p.hkv : 0);
     const int64_t at = kv4_row(block, p.hkv, h, p.block_size, in_block);

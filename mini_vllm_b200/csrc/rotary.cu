@@ -47,54 +47,65 @@ __device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
   b = __fadd_rn(__fmul_rn(b, c), __fmul_rn(x, s));
 }
 
-// V elements to a vector (1: a unit is one pair of elements)
-template <class T, int V, bool INTER>
+// V elements to a vector (1: a unit is one pair of elements).  A thread takes ITEMS units, a block's width apart, and requests all of them
+// before it turns the first: 16384 tokens of 40 heads, a 128-wide head half turned: 86 us with one unit, XX with four; few tokens are
+// spread over more threads instead.
+template <class T, int V, bool INTER, int ITEMS>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= p.total) return;
-  const uint32_t t = p.by_token.div(static_cast<uint32_t>(i));
-  const uint32_t in_token = static_cast<uint32_t>(i) - t * p.by_token.n;
-  const uint32_t head = p.by_head.div(in_token);
-  const int unit = static_cast<int>(in_token - head * p.by_head.n);
-  const bool is_q = static_cast<int>(head) < p.hq;
-  const int h = is_q ? head : head - p.hq;
-  const T* src = static_cast<const T*>(is_q ? p.q : p.k) + static_cast<int64_t>(t) * (is_q ? p.q_stride : p.k_stride) + static_cast<int64_t>(h) * p.d;
-  T* dst = static_cast<T*>(is_q ? p.q_out : p.k_out) + static_cast<int64_t>(t) * (is_q ? p.qo_stride : p.ko_stride) + static_cast<int64_t>(h) * p.d;
+  constexpr bool PAIR = !(INTER && V > 1);                   // a unit's partners are two vectors
   const int half = p.rot / 2;
-  if (unit >= p.rot_units) {                                 // carried along
-    float x[V];
-    const int at = p.rot + (unit - p.rot_units) * V;
-    load_vec<T, V>(src + at, x);
-    store_vec<T, V>(dst + at, x);
-    return;
+  float a[ITEMS][V], b[ITEMS][PAIR ? V : 1];
+  T* dst[ITEMS];
+  int where[ITEMS];                                          // the unit's number inside its head's turned ones, -1: carried along, -2: none
+  uint32_t token[ITEMS];
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) {
+    const int64_t i = (static_cast<int64_t>(blockIdx.x) * ITEMS + j) * 256 + threadIdx.x;
+    where[j] = -2;
+    if (i >= p.total) continue;
+    const uint32_t t = p.by_token.div(static_cast<uint32_t>(i));
+    const uint32_t in_token = static_cast<uint32_t>(i) - t * p.by_token.n;
+    const uint32_t head = p.by_head.div(in_token);
+    const int unit = static_cast<int>(in_token - head * p.by_head.n);
+    const bool is_q = static_cast<int>(head) < p.hq;
+    const int64_t h = static_cast<int64_t>(is_q ? head : head - p.hq) * p.d;
+    const T* src = static_cast<const T*>(is_q ? p.q : p.k) + static_cast<int64_t>(t) * (is_q ? p.q_stride : p.k_stride) + h;
+    dst[j] = static_cast<T*>(is_q ? p.q_out : p.k_out) + static_cast<int64_t>(t) * (is_q ? p.qo_stride : p.ko_stride) + h;
+    token[j] = t;
+    int one;
+    if (unit >= p.rot_units) {
+      where[j] = -1;
+      one = p.rot + (unit - p.rot_units) * V;
+    } else {
+      where[j] = unit;
+      one = PAIR && INTER ? 2 * unit : unit * V;
+      if constexpr (PAIR) load_vec<T, V>(src + (INTER ? one + 1 : one + half), b[j]);
+    }
+    load_vec<T, V>(src + one, a[j]);
+    dst[j] += one;
   }
-  const int64_t pos = p.positions[t];
-  const bool ok = pos >= 0 && pos < p.max_pos;
-  if (!ok) report(p.dev_status, kDevBadPosition, t);
-  const float* row = p.cos_sin + (ok ? pos : 0) * p.rot;
-  if constexpr (INTER && V > 1) {
-    float x[V], c[V / 2], s[V / 2];
-    load_vec<T, V>(src + unit * V, x);
-    load_table<V / 2>(row + unit * (V / 2), c);
-    load_table<V / 2>(row + half + unit * (V / 2), s);
-    if (ok) {
 #pragma unroll
-      for (int e = 0; e < V / 2; ++e) turn(x[2 * e], x[2 * e + 1], c[e], s[e]);
-    }
-    store_vec<T, V>(dst + unit * V, x);
-  } else {
-    const int one = INTER ? 2 * unit : unit * V, two = INTER ? one + 1 : one + half;
-    float a[V], b[V], c[V], s[V];
-    load_vec<T, V>(src + one, a);
-    load_vec<T, V>(src + two, b);
-    load_table<V>(row + unit * V, c);
-    load_table<V>(row + half + unit * V, s);
-    if (ok) {
+  for (int j = 0; j < ITEMS; ++j) {
+    if (where[j] < -1) continue;
+    if (where[j] >= 0) {
+      const int64_t pos = p.positions[token[j]];
+      const bool ok = pos >= 0 && pos < p.max_pos;
+      if (!ok) report(p.dev_status, kDevBadPosition, static_cast<int>(token[j]));
+      constexpr int N = PAIR ? V : V / 2;                    // angles of a unit
+      float c[N], s[N];
+      const float* row = p.cos_sin + (ok ? pos : 0) * p.rot + where[j] * N;
+      load_table<N>(row, c);
+      load_table<N>(row + half, s);
+      if (ok) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) turn(a[e], b[e], c[e], s[e]);
+        for (int e = 0; e < N; ++e) {
+          if constexpr (PAIR) turn(a[j][e], b[j][e], c[e], s[e]);
+          else turn(a[j][2 * e], a[j][2 * e + 1], c[e], s[e]);
+        }
+      }
+      if constexpr (PAIR) store_vec<T, V>(dst[j] + (INTER ? 1 : half), b[j]);
     }
-    store_vec<T, V>(dst + one, a);
-    store_vec<T, V>(dst + two, b);
+    store_vec<T, V>(dst[j], a[j]);
   }
 }
 
@@ -113,11 +124,14 @@ static int launch_rotary(RotaryParams& p, bool inter, cudaStream_t stream) {
   p.total = per_token * p.tokens;
   p.by_token = FastDiv(static_cast<uint32_t>(per_token));
   p.by_head = FastDiv(static_cast<uint32_t>(p.units));
-  const unsigned grid = static_cast<unsigned>((p.total + 255) / 256);
-  if (vec && inter) rotary_kernel<T, V, true><<<grid, 256, 0, stream>>>(p);
-  else if (vec) rotary_kernel<T, V, false><<<grid, 256, 0, stream>>>(p);
-  else if (inter) rotary_kernel<T, 1, true><<<grid, 256, 0, stream>>>(p);
-  else rotary_kernel<T, 1, false><<<grid, 256, 0, stream>>>(p);
+  const bool many = vec && p.total >= static_cast<int64_t>(sm_count()) * 2048 * 4;     // four units still leave every SM its 2048 threads
+  const unsigned grid = static_cast<unsigned>((p.total + 255) / 256), fewer = (grid + 3) / 4;
+  if (many && inter) rotary_kernel<T, V, true, 4><<<fewer, 256, 0, stream>>>(p);
+  else if (many) rotary_kernel<T, V, false, 4><<<fewer, 256, 0, stream>>>(p);
+  else if (vec && inter) rotary_kernel<T, V, true, 1><<<grid, 256, 0, stream>>>(p);
+  else if (vec) rotary_kernel<T, V, false, 1><<<grid, 256, 0, stream>>>(p);
+  else if (inter) rotary_kernel<T, 1, true, 1><<<grid, 256, 0, stream>>>(p);
+  else rotary_kernel<T, 1, false, 1><<<grid, 256, 0, stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? kOk : kLaunchFailed;
 }
 
