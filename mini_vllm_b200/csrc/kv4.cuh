@@ -40,11 +40,18 @@ __host__ __device__ __forceinline__ int64_t kv4_row(int64_t block, int hkv, int 
 __device__ __forceinline__ float kv4_scale(uint32_t affine) { return __uint_as_float(affine << 16); }
 __device__ __forceinline__ float kv4_min(uint32_t affine) { return __uint_as_float(affine & 0xffff0000u); }
 
-// what the eight codes of a word stand for; the product is exact in fp32 and the sum is rounded once
+// What the eight codes of a word stand for; the product is exact in fp32 and the sum is rounded once.  A code becomes a float as the last
+// bits of 2^23 + 16^i c, less 2^23 and over 16^i in one exact step: one integer instruction a code, the rest on the multipliers.
 __device__ __forceinline__ void kv4_values(uint32_t word, uint32_t affine, float (&v)[8]) {
   const float s = kv4_scale(affine), m = kv4_min(affine);
+  const uint32_t upper = word >> 16;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = fmaf(s, static_cast<float>((word >> kv4_shift(e)) & 15u), m);
+  for (int e = 0; e < 8; ++e) {
+    const int place = 4 * (e >> 1);
+    const uint32_t x = (((e & 1) ? upper : word) & (15u << place)) | 0x4b000000u;
+    const float unit = 1.f / static_cast<float>(1u << place);
+    v[e] = fmaf(s, fmaf(__uint_as_float(x), unit, -8388608.f * unit), m);
+  }
 }
 
 inline bool kv4_aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }

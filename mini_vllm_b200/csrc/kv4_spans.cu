@@ -185,39 +185,45 @@ __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(const Select
   if (cl > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   uint32_t keys_0;                                           // the first block's keys, in the cluster's shared memory
   asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(keys_0) : "r"(smem_u32(keys)));
-  const int stride = cl * (kSelectThreads / 8);
-  for (int base = (rank * (kSelectThreads / 32) + warp) * 4; base < count; base += stride) {     // warp-uniform
-    const int s = base + (lane >> 3);
-    const bool inner = s > 0 && s < count - 1;               // the first and the last one are taken anyway
-    int64_t block = -1;
-    if (inner) block = __ldg(table + s / per_block);
-    const bool ok = block >= 0 && block < p.num_blocks;
-    if (inner && !ok && sub == 0) report(p.dev_status, kDevBadBlock, b);
-    const __nv_bfloat16* at = p.summaries + ((ok ? block * p.hkv + h : 0) * per_block + (ok ? s % per_block : 0)) * (2 * D);
-    double sum = 0.0, sum2 = 0.0;
-    float lo[PIECES][8], hi[PIECES][8];
+  constexpr int NS = D == 256 ? 1 : 2;                       // spans that eight lanes have in flight
+  const int stride = cl * (kSelectThreads / 8) * NS;
+  for (int base = (rank * (kSelectThreads / 32) + warp) * 4 * NS; base < count; base += stride) {     // warp-uniform
+    uint4 lo[NS][PIECES], hi[NS][PIECES];
+    bool ok[NS];
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      load_vec<__nv_bfloat16, 8>(at + (i * 8 + sub) * 8, lo[i]);
-      load_vec<__nv_bfloat16, 8>(at + D + (i * 8 + sub) * 8, hi[i]);
+    for (int k = 0; k < NS; ++k) {
+      const int s = base + 4 * k + (lane >> 3);
+      const bool inner = s > 0 && s < count - 1;             // the first and the last one are taken anyway
+      int64_t block = -1;
+      if (inner) block = __ldg(table + s / per_block);
+      ok[k] = block >= 0 && block < p.num_blocks;
+      if (inner && !ok[k] && sub == 0) report(p.dev_status, kDevBadBlock, b);
+      const uint4* at = reinterpret_cast<const uint4*>(p.summaries + ((ok[k] ? block * p.hkv + h : 0) * per_block + (ok[k] ? s % per_block : 0)) * (2 * D));
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) { lo[k][i] = __ldg(at + i * 8 + sub); hi[k][i] = __ldg(at + D / 8 + i * 8 + sub); }
     }
-    for (int g = 0; g < p.group; ++g) {
+#pragma unroll
+    for (int k = 0; k < NS; ++k) {
+      const int s = base + 4 * k + (lane >> 3);
+      double sum = 0.0, sum2 = 0.0;
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
-        float q[8];
-        load_f32<8>(q_s + g * D + (i * 8 + sub) * 8, q);
+        const uint32_t l[4] = {lo[k][i].x, lo[k][i].y, lo[k][i].z, lo[k][i].w}, u[4] = {hi[k][i].x, hi[k][i].y, hi[k][i].z, hi[k][i].w};
+        for (int g = 0; g < p.group; ++g) {
+          float q[8];
+          load_f32<8>(q_s + g * D + (i * 8 + sub) * 8, q);
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          sum += static_cast<double>(fmaxf(q[e] * lo[i][e], q[e] * hi[i][e]));
-          sum2 += static_cast<double>(fmaxf(q[e + 1] * lo[i][e + 1], q[e + 1] * hi[i][e + 1]));
+          for (int e = 0; e < 4; ++e) {
+            sum += static_cast<double>(fmaxf(q[2 * e] * bf16_lo(l[e]), q[2 * e] * bf16_lo(u[e])));
+            sum2 += static_cast<double>(fmaxf(q[2 * e + 1] * bf16_hi(l[e]), q[2 * e + 1] * bf16_hi(u[e])));
+          }
         }
       }
-    }
-    sum += sum2;
+      sum += sum2;
 #pragma unroll
-    for (int off = 4; off > 0; off >>= 1) sum += __shfl_xor_sync(FULL, sum, off);
-    if (sub == 0 && s < count)
-      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(keys_0 + 8u * s), "l"(ok ? order_key(sum) : order_key(0.0)) : "memory");
+      for (int off = 4; off > 0; off >>= 1) sum += __shfl_xor_sync(FULL, sum, off);
+      if (sub == 0 && s < count) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(keys_0 + 8u * s), "l"(order_key(ok[k] ? sum : 0.0)));
+    }
   }
   if (cl > 1) {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -226,6 +232,24 @@ __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(const Select
     __syncthreads();
   }
   // ---- the first block: which of the inner spans -------------------------------------------------------------------------------------
+  if (count <= kSelectThreads) {                             // a thread has a span and counts the better ones: no passes, one prefix sum
+    const int s = threadIdx.x;
+    const bool ends = s == 0 || s == count - 1;
+    int better = s < count ? 0 : count;
+    if (s < count && !ends) {
+      const uint64_t mine = keys[s];
+#pragma unroll 4
+      for (int o = 1; o < count - 1; ++o) {
+        const uint64_t k = keys[o];
+        better += k > mine || (k == mine && o < s);
+      }
+    }
+    const bool take = ends || better < p.budget - 2;
+    int total;
+    const int at = block_prefix(take ? 1 : 0, scratch, total);
+    if (take && at < p.budget) out[at] = s;
+    return;
+  }
   const uint64_t sample = keys[1];
   uint64_t differ = 0;
   for (int s = 1 + threadIdx.x; s < count - 1; s += kSelectThreads) differ |= keys[s] ^ sample;

@@ -32,34 +32,20 @@ struct Kv4WriteParams {
   int* dev_status;
 };
 
-// The codes round(t / s), 0 <= t <= 15 s (1 + 2^-8), of eight channels as a word, r within 2^-22 of 1 / s.  Adding 1.5 * 2^23 rounds t r to a
-// whole number that then stands in the float's last bits.  Where t r comes near a half the code is decided exactly: n s and the middle
-// (n + 1/2) s between two codes take 13 bits, so t - n s against s / 2 is exact, and a quotient is rounded as its correctly rounded fp32
-// value would be (that is a half only where t is the middle itself: t's last place is never finer than the quotient's).
+// The codes round(t / s), 0 <= t <= 15 s (1 + 2^-8), of eight channels as a word, r within 2^-22 of 1 / s.  f is the correctly rounded
+// quotient: with f0 = t r the remainder t - f0 s takes 8 bits (s has 8) and is exact, f0 + r (t - f0 s) is within 2^-44 of t / s, and no
+// such quotient is that near the middle between two fp32 numbers.  So halves are halves and go to the even code.  Adding 1.5 * 2^23 rounds
+// to a whole number, which then stands in the float's last bits.
 __device__ __forceinline__ uint32_t kv4_codes(const float (&t)[8], float s, float r) {
   constexpr float kRound = 12582912.f;
   constexpr uint32_t kPlaces = 0x11111111u;                  // one in each of the eight 4-bit places
-  float n[8], worst = 0.f;
   uint32_t word = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float f = t[e] * r, z = f + kRound;
-    n[e] = z - kRound;
-    worst = fmaxf(worst, fabsf(f - n[e]));
-    word += __float_as_uint(z) << kv4_shift(e);
+    const float f0 = __fmul_rn(t[e], r), f = fmaf(fmaf(-f0, s, t[e]), r, f0);
+    word += __float_as_uint(__fadd_rn(f, kRound)) << kv4_shift(e);
   }
-  word -= __float_as_uint(kRound) * kPlaces;                 // modulo 2^32: the codes alone remain
-  if (worst > 0.5f - 0x1p-16f) {
-    word = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float off = fmaf(-n[e], s, t[e]), over = fabsf(off) - 0.5f * s;
-      const bool odd = (__float_as_uint(n[e] + kRound) & 1u) != 0;
-      if (over > 0.f || (over == 0.f && odd)) n[e] += off > 0.f ? 1.f : -1.f;
-      word |= (__float_as_uint(n[e] + kRound) & 15u) << kv4_shift(e);
-    }
-  }
-  return word;
+  return word - __float_as_uint(kRound) * kPlaces;           // modulo 2^32: the codes alone remain
 }
 
 __device__ __forceinline__ uint32_t min_bf16x2(uint32_t a, uint32_t b) {
@@ -72,7 +58,7 @@ __device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
 }
 
 template <int D, bool INTER, int ITEMS>
-__global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4WriteParams p) {
+__global__ void __launch_bounds__(256, ITEMS == 4 ? 4 : 1) kv4_write_kernel(const Kv4WriteParams p) {
   constexpr int LPH = D / 8, RPW = 32 / LPH;                 // lanes of a row, rows a warp holds at once
   constexpr uint32_t FULL = 0xffffffffu;
   const int lane = threadIdx.x & 31, c = lane % LPH, sub = lane / LPH;

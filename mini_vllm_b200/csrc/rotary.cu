@@ -9,6 +9,8 @@
 #include "host_util.cuh"
 #include "kv4.cuh"
 
+#include <type_traits>
+
 namespace mvb {
 
 struct RotaryParams {
@@ -47,65 +49,67 @@ __device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
   b = __fadd_rn(__fmul_rn(b, c), __fmul_rn(x, s));
 }
 
-// V elements to a vector (1: a unit is one pair of elements).  A thread takes ITEMS units, a block's width apart, and requests all of them
-// before it turns the first: 16384 tokens of 40 heads, a 128-wide head half turned: 86 us with one unit, XX with four; few tokens are
-// spread over more threads instead.
-template <class T, int V, bool INTER, int ITEMS>
+// V elements to a vector (1: a unit is one pair of elements).  A thread takes the same unit of HEADS neighbouring heads of a token, so that
+// it loads the unit's angles once, and requests all of them before it turns the first.
+template <class T, int V, bool INTER, int HEADS>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
   constexpr bool PAIR = !(INTER && V > 1);                   // a unit's partners are two vectors
-  const int half = p.rot / 2;
-  float a[ITEMS][V], b[ITEMS][PAIR ? V : 1];
-  T* dst[ITEMS];
-  int where[ITEMS];                                          // the unit's number inside its head's turned ones, -1: carried along, -2: none
-  uint32_t token[ITEMS];
+  constexpr int N = PAIR ? V : V / 2;                        // angles of a unit
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= p.total) return;
+  const int half = p.rot / 2, heads = p.hq + p.hkv;
+  const uint32_t t = p.by_token.div(static_cast<uint32_t>(i));
+  const uint32_t in_token = static_cast<uint32_t>(i) - t * p.by_token.n;
+  const uint32_t group = p.by_head.div(in_token);
+  const int unit = static_cast<int>(in_token - group * p.by_head.n), head0 = static_cast<int>(group) * HEADS;
+  const bool turned = unit < p.rot_units;
+  const int one = !turned ? p.rot + (unit - p.rot_units) * V : PAIR && INTER ? 2 * unit : unit * V;
+  const int two = INTER ? one + 1 : one + half;
+  const int64_t pos = turned ? __ldg(p.positions + t) : 0;
+  auto at = [&](int head, bool out) -> T* {
+    const bool is_q = head < p.hq;
+    const T* base = static_cast<const T*>(out ? (is_q ? p.q_out : p.k_out) : (is_q ? p.q : p.k));
+    const int64_t stride = out ? (is_q ? p.qo_stride : p.ko_stride) : (is_q ? p.q_stride : p.k_stride);
+    return const_cast<T*>(base) + static_cast<int64_t>(t) * stride + static_cast<int64_t>(is_q ? head : head - p.hq) * p.d;
+  };
+  using Raw = std::conditional_t<V == 1, T, uint4>;          // as it lies in memory, until its turn
+  Raw a[HEADS], b[HEADS];
 #pragma unroll
-  for (int j = 0; j < ITEMS; ++j) {
-    const int64_t i = (static_cast<int64_t>(blockIdx.x) * ITEMS + j) * 256 + threadIdx.x;
-    where[j] = -2;
-    if (i >= p.total) continue;
-    const uint32_t t = p.by_token.div(static_cast<uint32_t>(i));
-    const uint32_t in_token = static_cast<uint32_t>(i) - t * p.by_token.n;
-    const uint32_t head = p.by_head.div(in_token);
-    const int unit = static_cast<int>(in_token - head * p.by_head.n);
-    const bool is_q = static_cast<int>(head) < p.hq;
-    const int64_t h = static_cast<int64_t>(is_q ? head : head - p.hq) * p.d;
-    const T* src = static_cast<const T*>(is_q ? p.q : p.k) + static_cast<int64_t>(t) * (is_q ? p.q_stride : p.k_stride) + h;
-    dst[j] = static_cast<T*>(is_q ? p.q_out : p.k_out) + static_cast<int64_t>(t) * (is_q ? p.qo_stride : p.ko_stride) + h;
-    token[j] = t;
-    int one;
-    if (unit >= p.rot_units) {
-      where[j] = -1;
-      one = p.rot + (unit - p.rot_units) * V;
-    } else {
-      where[j] = unit;
-      one = PAIR && INTER ? 2 * unit : unit * V;
-      if constexpr (PAIR) load_vec<T, V>(src + (INTER ? one + 1 : one + half), b[j]);
+  for (int j = 0; j < HEADS; ++j) {
+    if (head0 + j < heads) {
+      const T* src = at(head0 + j, false);
+      a[j] = *reinterpret_cast<const Raw*>(src + one);
+      if (PAIR && turned) b[j] = *reinterpret_cast<const Raw*>(src + two);
     }
-    load_vec<T, V>(src + one, a[j]);
-    dst[j] += one;
+  }
+  const bool ok = pos >= 0 && pos < p.max_pos;
+  float c[N], s[N];
+  if (turned) {
+    if (!ok) report(p.dev_status, kDevBadPosition, static_cast<int>(t));
+    const float* row = p.cos_sin + (ok ? pos : 0) * p.rot + unit * N;
+    load_table<N>(row, c);
+    load_table<N>(row + half, s);
   }
 #pragma unroll
-  for (int j = 0; j < ITEMS; ++j) {
-    if (where[j] < -1) continue;
-    if (where[j] >= 0) {
-      const int64_t pos = p.positions[token[j]];
-      const bool ok = pos >= 0 && pos < p.max_pos;
-      if (!ok) report(p.dev_status, kDevBadPosition, static_cast<int>(token[j]));
-      constexpr int N = PAIR ? V : V / 2;                    // angles of a unit
-      float c[N], s[N];
-      const float* row = p.cos_sin + (ok ? pos : 0) * p.rot + where[j] * N;
-      load_table<N>(row, c);
-      load_table<N>(row + half, s);
+  for (int j = 0; j < HEADS; ++j) {
+    if (head0 + j >= heads) break;
+    T* dst = at(head0 + j, true);
+    if (turned) {
+      float x[V], y[V];
+      load_vec<T, V>(reinterpret_cast<const T*>(&a[j]), x);
+      if constexpr (PAIR) load_vec<T, V>(reinterpret_cast<const T*>(&b[j]), y);
       if (ok) {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-          if constexpr (PAIR) turn(a[j][e], b[j][e], c[e], s[e]);
-          else turn(a[j][2 * e], a[j][2 * e + 1], c[e], s[e]);
+          if constexpr (PAIR) turn(x[e], y[e], c[e], s[e]);
+          else turn(x[2 * e], x[2 * e + 1], c[e], s[e]);
         }
       }
-      if constexpr (PAIR) store_vec<T, V>(dst[j] + (INTER ? 1 : half), b[j]);
+      store_vec<T, V>(dst + one, x);
+      if constexpr (PAIR) store_vec<T, V>(dst + two, y);
+    } else {
+      *reinterpret_cast<Raw*>(dst + one) = a[j];
     }
-    store_vec<T, V>(dst[j], a[j]);
   }
 }
 
@@ -119,15 +123,17 @@ static int launch_rotary(RotaryParams& p, bool inter, cudaStream_t stream) {
   const int v = vec ? V : 1;
   p.rot_units = vec && inter ? p.rot / V : p.rot / 2 / v;
   p.units = p.rot_units + (in_place ? 0 : (p.d - p.rot) / v);
-  const int64_t per_token = static_cast<int64_t>(p.hq + p.hkv) * p.units;
+  const int heads = p.hq + p.hkv;
+  // four heads a thread where that still leaves every SM its 2048 threads, one where there are few tokens
+  const bool many = vec && static_cast<int64_t>((heads + 3) / 4) * p.units * p.tokens >= static_cast<int64_t>(sm_count()) * 2048;
+  const int64_t per_token = static_cast<int64_t>(many ? (heads + 3) / 4 : heads) * p.units;
   if (per_token > 0x7fffffffLL / (p.tokens > 0 ? p.tokens : 1)) return kUnsupportedShape;
   p.total = per_token * p.tokens;
   p.by_token = FastDiv(static_cast<uint32_t>(per_token));
   p.by_head = FastDiv(static_cast<uint32_t>(p.units));
-  const bool many = vec && p.total >= static_cast<int64_t>(sm_count()) * 2048 * 4;     // four units still leave every SM its 2048 threads
-  const unsigned grid = static_cast<unsigned>((p.total + 255) / 256), fewer = (grid + 3) / 4;
-  if (many && inter) rotary_kernel<T, V, true, 4><<<fewer, 256, 0, stream>>>(p);
-  else if (many) rotary_kernel<T, V, false, 4><<<fewer, 256, 0, stream>>>(p);
+  const unsigned grid = static_cast<unsigned>((p.total + 255) / 256);
+  if (many && inter) rotary_kernel<T, V, true, 4><<<grid, 256, 0, stream>>>(p);
+  else if (many) rotary_kernel<T, V, false, 4><<<grid, 256, 0, stream>>>(p);
   else if (vec && inter) rotary_kernel<T, V, true, 1><<<grid, 256, 0, stream>>>(p);
   else if (vec) rotary_kernel<T, V, false, 1><<<grid, 256, 0, stream>>>(p);
   else if (inter) rotary_kernel<T, 1, true, 1><<<grid, 256, 0, stream>>>(p);
