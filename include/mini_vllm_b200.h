@@ -628,6 +628,7 @@ int mvb_row_norm_rope_kv_write(int dtype, void* q, int64_t q_row_stride, void* k
  *   sequence stand next to each other, in order.
  * mvb_kv4_select: per sequence and KV head the `budget` (>= 2) spans with the greatest sum over the group's heads and the channels of
  *   max(q least, q greatest), the first and the last span always among them, of equal sums the lower index; ascending, -1 behind them.
+ *   max_tokens: the longest context that may come (at most 1048576, and what the table holds); a longer one is reported and cut there.
  */
 typedef struct mvb_kv4_cache {
   void* k_codes;
@@ -656,7 +657,8 @@ int mvb_kv4_summarise(const mvb_kv4_cache* cache, const int32_t* slot_mapping, i
                       void* stream);
 int mvb_kv4_select(const void* q, int64_t q_row_stride, const void* summaries, int64_t num_blocks, int block_size,
                    const int32_t* cache_seqlens, const int32_t* block_table, int64_t table_stride, int table_width, int num_seqs,
-                   int num_q_heads, int num_kv_heads, int head_dim, int budget, int32_t* spans, int32_t* dev_status, void* stream);
+                   int num_q_heads, int num_kv_heads, int head_dim, int max_tokens, int budget, int32_t* spans, int32_t* dev_status,
+                   void* stream);
 
 #ifdef __cplusplus
 }

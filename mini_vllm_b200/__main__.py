@@ -23,6 +23,8 @@ def main(argv: list[str] | None = None) -> int:
     ap.add_argument("--ignore-eos", action="store_true")
     ap.add_argument("--max-model-len", type=int, default=4096)
     ap.add_argument("--chunked-prefill", action="store_true", help="prompts enter in portions of the token budget")
+    ap.add_argument("--kv-cache-bits", type=int, default=16, choices=[4, 16], help="4: keys and values are cached in 4 bits")
+    ap.add_argument("--decode-spans", type=int, default=None, help="with 4 bits: spans of 64 tokens that a decode step reads per sequence and head")
     ap.add_argument("--max-batched-tokens", type=int, default=16384)
     ap.add_argument("--seed", type=int, default=0)
     args = ap.parse_args(argv)
@@ -31,7 +33,8 @@ def main(argv: list[str] | None = None) -> int:
     from .engine.engine import Engine
     engine = Engine(Config(model=args.model, dtype=getattr(torch, args.dtype) if args.dtype else None,
                            max_model_len=args.max_model_len, max_num_batched_tokens=args.max_batched_tokens,
-                           max_num_batched_seqs=max(8, len(args.prompt)), enable_chunked_prefill=args.chunked_prefill, seed=args.seed))
+                           max_num_batched_seqs=max(8, len(args.prompt)), enable_chunked_prefill=args.chunked_prefill, seed=args.seed,
+                           kv_cache_bits=args.kv_cache_bits, decode_spans=args.decode_spans))
     encode = (lambda p: [int(t) for t in p.split()]) if engine.tokenizer is None else engine.tokenizer.encode
     params = SamplingParams(temperature=args.temperature, max_tokens=args.max_tokens, top_k=args.top_k, top_p=args.top_p,
                             ignore_eos=args.ignore_eos)

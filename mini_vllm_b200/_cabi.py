@@ -116,7 +116,7 @@ SIGNATURES = {
     "mvb_decode_attn4_workspace_bytes": (sz, [i32, i32, i32, i32]),
     "mvb_decode_attn4": (i32, [vp, i64, vp, vp, vp, i64, i32, vp, i32, i32, i32, f32, i32, f32, f32, vp, i64, vp, sz, vp, vp]),
     "mvb_kv4_summarise": (i32, [vp, vp, i32, vp, vp, vp]),
-    "mvb_kv4_select": (i32, [vp, i64, vp, i64, i32, vp, vp, i64, i32, i32, i32, i32, i32, i32, vp, vp, vp]),
+    "mvb_kv4_select": (i32, [vp, i64, vp, i64, i32, vp, vp, i64, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp]),
 }
 
 _lib = None

@@ -42,6 +42,10 @@ class Config:
     enable_prefix_cache: bool = False        # the reference ships with prefix caching switched off
     enable_mixed_steps: bool = False         # extension: new prompts join a step of running decodes (scheduler.py)
     enable_chunked_prefill: bool = False     # extension: prompts enter in portions of at most the token budget
+    kv_cache_bits: int = 16                  # extension: 4 = keys and values are cached and read in 4 bits, with a scale and a minimum per 64 channels
+    # extension (with kv_cache_bits=4): a decode step reads this many spans of 64 tokens per sequence and KV head, those whose bounds promise the
+    # greatest scores, in layers without a window (None: all tokens)
+    decode_spans: Optional[int] = None
     num_state_slots: Optional[int] = None    # recurrent models: sequences that can hold state (None: max_num_batched_seqs)
 
     # executor
@@ -78,6 +82,10 @@ class Config:
                 self.eos_token_ids = {eos}
             else:
                 self.eos_token_ids = set(eos)
+        if self.kv_cache_bits not in (4, 16):
+            raise ValueError("kv_cache_bits must be 16 (the activations' own type) or 4")
+        if self.decode_spans is not None and (self.kv_cache_bits != 4 or self.decode_spans < 2):
+            raise ValueError("decode_spans needs kv_cache_bits=4, and at least 2 spans (the first and the last one are always read)")
         if self.kv_cache_block_size % 128 != 0:
             raise ValueError("kv_cache_block_size must be a multiple of 128 (the prefill KV tile)")
 
@@ -90,6 +98,9 @@ def _flatten_hf(cfg) -> SimpleNamespace:
              "sliding_window", "rope_theta", "rope_local_base_freq"]
     out = SimpleNamespace(**{n: getattr(cfg, n) for n in names if hasattr(cfg, n)})
     rp = getattr(cfg, "rope_parameters", None)
+    scaling = getattr(cfg, "rope_scaling", None) or (rp.get("full_attention", rp) if isinstance(rp, dict) else None)
+    if isinstance(scaling, dict) and scaling.get("rope_type", scaling.get("type", "default")) != "default":
+        out.rope_scaling = dict(scaling)
     if isinstance(rp, dict):
         if "rope_theta" in rp and not hasattr(out, "rope_theta"):
             out.rope_theta = rp["rope_theta"]

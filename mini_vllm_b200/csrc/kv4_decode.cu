@@ -12,8 +12,9 @@
 // whole bytes less those of the low codes), and scales and minima cost a few per token.  q is brought to [2^14, 2^15)
 // by a power of two per head so that fp16 holds every bf16 exactly down to 2^-29 of the greatest; the channels whose codes sit at bits 4-7
 // (16 times as large) have it divided by 16.  Scores, softmax statistics and outputs are fp32; the weights p s are rounded once, to fp16,
-// an eighth of what bf16 weights would lose.  They never overflow: the softmax's reference is the greatest score + log2(scale), which
-// bounds every p s by 2^6 (scales below 2^-60 count as that).
+// an eighth of what bf16 weights would lose.  They never overflow: the softmax's reference is the greatest score + log2(size of the
+// token's values), with size = max(scale, 2^-20 |minimum|, 2^-100), which bounds every p s by 2^6 and every p m by 2^26; a minimum that
+// large leaves nothing of its codes in the bf16 output.
 //
 // Bound by memory, on paper 4608 bytes against some 450 warp instructions per 32 tokens of a 128-wide head.  Work is tiles of 32 tokens of
 // one (sequence, head), numbered sequence by sequence and head by head, and cut evenly: each CTA takes a contiguous range, each of its
@@ -62,7 +63,7 @@ struct Decode4Params {
   const int32_t* spans;                // [num_seqs, hkv, budget] or nullptr
   int64_t table_stride, num_blocks;
   FastDiv by_block;
-  int table_width, num_seqs, hkv, group, block_size, budget, window_left;
+  int table_width, max_len, num_seqs, hkv, group, block_size, budget, window_left;
   float scale_log2, cap_in, cap_log2, out_scale;
   float* parts;                        // [CTAs][NW + 2] parts: a warp's first row, then the CTA's first and last
   int32_t* arrivals;                   // [num_seqs * hkv][NW], zero between launches
@@ -122,8 +123,7 @@ template <int TOK>
 struct Decode4Walk {
   int b, h, i, count, n;               // tile i of `count` of head h of sequence b, which has n tokens
   __device__ __forceinline__ static int length(const Decode4Params& p, int b) {
-    const int n = p.seqlens[b], most = p.table_width * p.block_size;
-    return min(n, most);
+    return min(p.seqlens[b], p.max_len);
   }
   __device__ __forceinline__ static int first_tile(const Decode4Params& p, int n) {
     return p.window_left >= 0 ? max(0, n - 1 - p.window_left) / TOK : 0;
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
     int v = 0;
     if (b < p.num_seqs) {
       const int n = p.seqlens[b];
-      if (n > p.table_width * p.block_size) report(p.dev_status, kDevBadLength, b);
+      if (n > p.max_len) report(p.dev_status, kDevBadLength, b);
       v = Walk::tiles(p, Walk::length(p, b));
     }
     int x = v;
@@ -492,9 +492,12 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
             for (int j = 0; j < GRP; ++j) va[s][1][j] = 0u;
           }
         }
-        float big0 = 0x1p-60f, big1 = 0x1p-60f;
+        float big0 = 0x1p-100f, big1 = 0x1p-100f;
 #pragma unroll
-        for (int j = 0; j < GRP; ++j) { big0 = fmaxf(big0, kv4_scale(va[s][0][j])); big1 = fmaxf(big1, kv4_scale(va[s][1][j])); }
+        for (int j = 0; j < GRP; ++j) {
+          big0 = fmax3(big0, kv4_scale(va[s][0][j]), fabsf(kv4_min(va[s][0][j])) * 0x1p-20f);
+          big1 = fmax3(big1, kv4_scale(va[s][1][j]), fabsf(kv4_min(va[s][1][j])) * 0x1p-20f);
+        }
         big0 = fast_log2(big0); big1 = fast_log2(big1);
         ta = fmax3(ta, x[s][0] + big0, x[s][2] + big1);
         tb = fmax3(tb, x[s][1] + big0, x[s][3] + big1);
@@ -758,23 +761,24 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
   }
 }
 
-struct Decode4Layout {
-  size_t parts, arrivals, total;
-};
-static Decode4Layout decode4_layout(int64_t seqs, int hkv, int group, int d) {
-  const int nw = d == 256 ? Decode4Cfg<256>::NW : Decode4Cfg<128>::NW;
-  Decode4Layout l;
-  l.parts = 0;
-  l.arrivals = (sizeof(float) * kDecode4MaxCtas * (nw + 2) * decode4_part(group, d) + 255) / 256 * 256;
-  l.total = l.arrivals + (sizeof(int32_t) * static_cast<size_t>(seqs) * hkv * nw + 255) / 256 * 256;
-  return l;
+// The parts have the room that the largest head shape needs, so that the counters lie at the same place for every shape and batch: one
+// workspace may serve different calls one after the other and the counters are zero between them.
+constexpr size_t decode4_parts_bytes(int d, int nw) {
+  return sizeof(float) * kDecode4MaxCtas * (nw + 2) * decode4_part(kDecode4MaxGroup, d);
+}
+constexpr size_t kDecode4Parts = decode4_parts_bytes(256, Decode4Cfg<256>::NW) > decode4_parts_bytes(128, Decode4Cfg<128>::NW)
+                                     ? decode4_parts_bytes(256, Decode4Cfg<256>::NW) : decode4_parts_bytes(128, Decode4Cfg<128>::NW);
+static_assert(kDecode4Parts % 256 == 0, "");
+
+static size_t decode4_bytes(int64_t seqs, int hkv) {
+  return kDecode4Parts + (sizeof(int32_t) * static_cast<size_t>(seqs) * hkv * Decode4Cfg<128>::NW + 255) / 256 * 256;
 }
 
 }  // namespace mvb
 
 extern "C" size_t mvb_decode_attn4_workspace_bytes(int max_seqs, int num_q_heads, int num_kv_heads, int head_dim) {
   if (max_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || num_q_heads % num_kv_heads != 0) return 0;
-  return mvb::decode4_layout(max_seqs, num_kv_heads, num_q_heads / num_kv_heads, head_dim).total;
+  return mvb::decode4_bytes(max_seqs, num_kv_heads);
 }
 
 extern "C" int mvb_decode_attn4(const void* q, int64_t q_row_stride, const mvb_kv4_cache* cache, const int32_t* cache_seqlens,
@@ -793,9 +797,9 @@ extern "C" int mvb_decode_attn4(const void* q, int64_t q_row_stride, const mvb_k
   if (q_row_stride % 8 || out_row_stride % 8 || !is_aligned(q, 16) || !is_aligned(out, 16) || !is_aligned(workspace, 256)) return kMisaligned;
   // lengths and tile numbers are 32-bit; the prefix sums of the lengths have the ring's room
   if (static_cast<int64_t>(table_width) * cache->block_size > 0x7fffffffLL || num_seqs > 16384) return kUnsupportedShape;
-  if (static_cast<double>(num_seqs) * hkv * table_width * (cache->block_size / 32) > 2147483000.0) return kUnsupportedShape;
-  const Decode4Layout l = decode4_layout(num_seqs, hkv, num_q_heads / hkv, cache->head_dim);
-  if (workspace_bytes < l.total) return kScratchTooSmall;
+  const int64_t longest = table_width < cache->num_blocks ? table_width : cache->num_blocks;
+  if (static_cast<double>(num_seqs) * hkv * longest * (cache->block_size / 32) > 2147483000.0) return kUnsupportedShape;
+  if (workspace_bytes < decode4_bytes(num_seqs, hkv)) return kScratchTooSmall;
   const float kLog2e = 1.4426950408889634f;
   Decode4Params p;
   p.q = static_cast<const __nv_bfloat16*>(q); p.q_stride = q_row_stride; p.out = static_cast<__nv_bfloat16*>(out); p.out_stride = out_row_stride;
@@ -803,13 +807,13 @@ extern "C" int mvb_decode_attn4(const void* q, int64_t q_row_stride, const mvb_k
   p.k_affine = static_cast<const uint8_t*>(cache->k_affine); p.v_affine = static_cast<const uint8_t*>(cache->v_affine);
   p.seqlens = cache_seqlens; p.block_table = block_table; p.table_stride = table_stride; p.table_width = table_width; p.spans = spans;
   p.num_blocks = cache->num_blocks; p.by_block = FastDiv(static_cast<uint32_t>(cache->block_size));
-  p.num_seqs = num_seqs; p.hkv = hkv; p.group = num_q_heads / hkv; p.block_size = cache->block_size;
+  p.max_len = static_cast<int>(longest * cache->block_size); p.num_seqs = num_seqs; p.hkv = hkv; p.group = num_q_heads / hkv; p.block_size = cache->block_size;
   p.budget = budget; p.window_left = window_left;
   // with a cap the scores leave the sums as they are and the cap's own factors are in log2 units
   p.scale_log2 = softcap > 0.f ? scale : scale * kLog2e;
   p.cap_in = softcap > 0.f ? 2.f * kLog2e / softcap : 0.f; p.cap_log2 = softcap * kLog2e; p.out_scale = out_scale;
   p.parts = static_cast<float*>(workspace);
-  p.arrivals = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + l.arrivals);
+  p.arrivals = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + kDecode4Parts);
   p.dev_status = dev_status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int grid = sm_count() < kDecode4MaxCtas ? sm_count() : kDecode4MaxCtas;

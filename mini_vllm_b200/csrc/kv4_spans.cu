@@ -109,7 +109,7 @@ struct SelectParams {
   const int32_t* block_table;
   int64_t table_stride, num_blocks;
   int32_t* out;
-  int table_width, hkv, group, block_size, budget;
+  int max_spans, hkv, group, block_size, budget;
   int* dev_status;
 };
 
@@ -166,10 +166,10 @@ __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(const Select
   const int n = p.seqlens[b];
   int32_t* out = p.out + (static_cast<int64_t>(b) * p.hkv + h) * p.budget;
   int count = n > 0 ? (n + kKv4Span - 1) / kKv4Span : 0;
-  const int per_block = p.block_size / kKv4Span, most = p.table_width * per_block;
-  if (count > most) {                                        // a length that its block list does not hold
+  const int per_block = p.block_size / kKv4Span;
+  if (count > p.max_spans) {                                 // longer than the caller said, or than its block list holds
     if (threadIdx.x == 0) report(p.dev_status, kDevBadLength, b);
-    count = most;
+    count = p.max_spans;
   }
   if (count <= p.budget) {                                   // (the whole cluster)
     if (rank == 0)
@@ -342,22 +342,28 @@ extern "C" int mvb_kv4_summarise(const mvb_kv4_cache* cache, const int32_t* slot
 
 extern "C" int mvb_kv4_select(const void* q, int64_t q_row_stride, const void* summaries, int64_t num_blocks, int block_size,
                               const int32_t* cache_seqlens, const int32_t* block_table, int64_t table_stride, int table_width, int num_seqs,
-                              int num_q_heads, int num_kv_heads, int head_dim, int budget, int32_t* spans, int32_t* dev_status, void* stream) {
+                              int num_q_heads, int num_kv_heads, int head_dim, int max_tokens, int budget, int32_t* spans,
+                              int32_t* dev_status, void* stream) {
   using namespace mvb;
-  if (num_seqs < 0 || num_blocks <= 0 || block_size <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || table_width <= 0 || budget < 2)
+  if (num_seqs < 0 || num_blocks <= 0 || block_size <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || table_width <= 0 || max_tokens <= 0 || budget < 2)
     return kInvalidArgument;
   if (head_dim != 64 && head_dim != 128 && head_dim != 256) return kUnsupportedShape;
   if (num_q_heads % num_kv_heads != 0 || num_q_heads / num_kv_heads > kSelectMaxGroup || block_size % kKv4Span != 0) return kUnsupportedShape;
-  if (static_cast<int64_t>(table_width) * (block_size / kKv4Span) > kSelectMaxSpans || num_seqs > 65535) return kUnsupportedShape;
+  if (num_seqs > 65535) return kUnsupportedShape;
+  // keys in shared memory: for the longest context that may come
+  int64_t spans_most = static_cast<int64_t>(table_width) * (block_size / kKv4Span);
+  const int64_t said = (static_cast<int64_t>(max_tokens) + kKv4Span - 1) / kKv4Span;
+  if (said < spans_most) spans_most = said;
+  if (spans_most > kSelectMaxSpans) return kUnsupportedShape;
   if (num_seqs == 0) return kOk;
   if (!q || !summaries || !cache_seqlens || !block_table || !spans || table_stride < table_width) return kInvalidArgument;
   if (!is_aligned(q, 2) || !is_aligned(summaries, 16)) return kMisaligned;
   SelectParams p;
   p.q = static_cast<const __nv_bfloat16*>(q); p.q_stride = q_row_stride; p.summaries = static_cast<const __nv_bfloat16*>(summaries);
   p.seqlens = cache_seqlens; p.block_table = block_table; p.table_stride = table_stride; p.num_blocks = num_blocks; p.out = spans;
-  p.table_width = table_width; p.hkv = num_kv_heads; p.group = num_q_heads / num_kv_heads; p.block_size = block_size; p.budget = budget;
+  p.max_spans = static_cast<int>(spans_most); p.hkv = num_kv_heads; p.group = num_q_heads / num_kv_heads; p.block_size = block_size; p.budget = budget;
   p.dev_status = dev_status;
-  const size_t smem = sizeof(uint64_t) * static_cast<size_t>(table_width) * (block_size / kKv4Span);
+  const size_t smem = sizeof(uint64_t) * static_cast<size_t>(spans_most);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // blocks enough for every SM to have two, a cluster of at most eight for one (sequence, head)
   int cl = 1;

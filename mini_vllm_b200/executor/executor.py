@@ -86,6 +86,7 @@ class Executor:
         self.h2d_bytes = 0                   # bytes uploaded by the packing path (for the bench's e2e line)
         self.d2h_bytes = 0
         self.graph_runner = None
+        self.kv4 = False                       # keys and values are cached in 4 bits: prompts, too, read them from there (set with the pool)
         self._warmup_model()
         self._init_states()
         self._init_kv_cache()
@@ -123,11 +124,17 @@ class Executor:
         shapes = [(m.num_kv_heads, m.head_dim) for m in self.attention_layers]
         per_token = 2 * sum(h * d for h, d in shapes) + sum(m.latent_width for m in self.latent_layers)
         block_bytes = self.block_size * per_token * hf.dtype.itemsize
+        kv4 = cfg.kv_cache_bits == 4
+        if kv4:
+            block_bytes = self._kv4_block_bytes()
         room = int(total * cfg.gpu_memory_utilization - (total - free) - peak + current)
         fit = room // block_bytes if block_bytes else cfg.kv_cache_num_blocks
         if fit <= 0:
             raise RuntimeError("no memory left for the KV cache")
         cfg.kv_cache_num_blocks = min(fit, cfg.kv_cache_num_blocks)
+        if kv4:
+            log.info("allocated %d KV blocks of 4-bit codes", cfg.kv_cache_num_blocks)
+            return self._bind_kv4()
         pool = lambda *dims: torch.empty(*dims, dtype=hf.dtype, device=self.device)
         if len(set(shapes)) <= 1:
             heads, head_dim = shapes[0] if shapes else (1, 1)
@@ -141,6 +148,25 @@ class Executor:
             module.k_cache, module.v_cache = k, v
         for module in self.latent_layers:
             module.latent_cache = pool(cfg.kv_cache_num_blocks, self.block_size, module.latent_width)
+
+    def _kv4_block_bytes(self) -> int:
+        """Bytes of one block in all layers; raises for a model that a cache in 4 bits does not serve."""
+        layers, cfg = self.attention_layers, self.config
+        if not layers or self.latent_layers or self.recurrent or not all(m.takes_kv4(cfg.hf_config.dtype) for m in layers):
+            raise ValueError("kv_cache_bits=4 needs bf16 attention layers of 128 or 256 channels a head throughout, without sinks, biases by "
+                             "distance, kept tokens, gates or borrowed keys")
+        tokens = sum(ops.KV4Cache.token_bytes(m.num_kv_heads, m.head_dim) for m in layers) * self.block_size
+        bounds = sum(m.num_kv_heads * (self.block_size // 64) * 4 * m.head_dim for m in layers if m.window_left < 0)
+        return tokens + (bounds if cfg.decode_spans else 0)
+
+    def _bind_kv4(self) -> None:
+        """One cache in 4 bits per layer, all of the same number of blocks, served by the same block tables."""
+        cfg, self.kv4 = self.config, True
+        for m in self.attention_layers:
+            m.kv4 = ops.KV4Cache.empty(cfg.kv_cache_num_blocks, self.block_size, m.num_kv_heads, m.head_dim, self.device)
+            if cfg.decode_spans and m.window_left < 0:
+                m.summaries = ops.kv4_summaries(m.kv4)
+                m.decode_spans, m.max_context = cfg.decode_spans, cfg.hf_config.max_position_embeddings
 
     # ---- packing ---------------------------------------------------------------------------------
     @staticmethod
@@ -188,7 +214,7 @@ class Executor:
         self.h2d_bytes += meta.numel() * 4
         meta, state_slots = self._take_slots(meta, b)
         width = max(int(nblk.max()), 1)
-        out = ops.pack_prefill(meta, b, t, int(blk_off[-1]), width, self.block_size, bool(cached.any()), self.status)
+        out = ops.pack_prefill(meta, b, t, int(blk_off[-1]), width, self.block_size, bool(cached.any()) or self.kv4, self.status)
         ctx = Context(prefill=True, positions=out["positions"], cu_seqlens_q=out["cu_seqlens_q"],
                       cu_seqlens_k=out["cu_seqlens_k"], slot_mapping=out["slot_mapping"],
                       max_seqlen_q=int(q_len.max()), max_seqlen_k=int(seq_len.max()),
@@ -338,7 +364,7 @@ class Executor:
             meta, state_slots = self._take_slots(meta, b)
             slots_dev = meta[meta.numel() - b:]
             width = max(int(nblk.max()), 1)
-            out = ops.pack_prefill(meta, b, t, int(blk_off[-1]), width, self.block_size, bool(cached.any()), self.status)
+            out = ops.pack_prefill(meta, b, t, int(blk_off[-1]), width, self.block_size, bool(cached.any()) or self.kv4, self.status)
             ctx = Context(prefill=True, positions=out["positions"], cu_seqlens_q=out["cu_seqlens_q"],
                           cu_seqlens_k=out["cu_seqlens_k"], slot_mapping=out["slot_mapping"],
                           max_seqlen_q=int(q_len.max()), max_seqlen_k=int(seq_len.max()),

@@ -131,7 +131,8 @@ class DecoderLM(nn.Module):
             self.register_buffer("embed_scale", torch.tensor(float(cfg.hidden_size) ** 0.5), persistent=False)
         else:
             self.embed_scale = None
-        self.rotary = RotaryEmbedding(cfg.head_dim, cfg.max_position_embeddings, cfg.rope_theta)
+        self.rotary = RotaryEmbedding(cfg.head_dim, cfg.max_position_embeddings, cfg.rope_theta,
+                                      scaling=getattr(cfg, "rope_scaling", None))
         self.rotary_local = (RotaryEmbedding(cfg.head_dim, cfg.max_position_embeddings, cfg.rope_local_base_freq)
                              if gemma else None)
         # The reference hands its attention layer (sliding_window, -1) and that layer's contract reads the

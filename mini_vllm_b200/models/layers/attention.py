@@ -45,6 +45,21 @@ def decode_workspace_for(device, max_seqs: int, num_heads: int, num_kv_heads: in
     return ws
 
 
+def decode4_workspace_for(device, max_seqs: int, num_heads: int, num_kv_heads: int, head_dim: int) -> torch.Tensor:
+    """The same for attention over a cache in 4 bits, which needs no plan: shared by all layers of a head shape, whatever their window."""
+    key = (device, "kv4", num_heads, num_kv_heads, head_dim)
+    ws = _workspaces.get(key)
+    need = ops._cabi.load().mvb_decode_attn4_workspace_bytes(max_seqs, num_heads, num_kv_heads, head_dim)
+    if ws is None or ws.numel() < need:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("decode workspace must be allocated before CUDA graph capture "
+                               "(run one eager decode step of the largest batch first)")
+        if ws is not None:
+            _superseded.append(ws)
+        ws = _workspaces[key] = ops.decode4_workspace(max(max_seqs, 512), num_heads, num_kv_heads, head_dim, device)
+    return ws
+
+
 def prefill_items_for(ctx: Context, layer):
     """The step's prefill work list, if the packing step built one for the layer's query-block size."""
     if ctx.prefill_items is None:
@@ -69,6 +84,11 @@ class FlashAttention(nn.Module):
         self.sinks = self.slopes = None   # fp32 [num_heads] each, set by whoever owns them
         self.__dict__["source"] = source  # (not a submodule of this one)
         self.lends = False                # some later layer reads this one's keys and values
+        # in the caches' place, one in 4 bits; with decode_spans > 0 also the bounds of its spans of 64 tokens: a decode step then reads only so
+        # many of them per sequence and KV head (layers without a window)
+        self.kv4: ops.KV4Cache | None = None
+        self.summaries: torch.Tensor | None = None
+        self.decode_spans = self.max_context = 0
         if source is None:
             # placeholders the executor replaces with views of its KV pool (found by hasattr)
             self.k_cache = self.v_cache = torch.tensor([])
@@ -93,8 +113,22 @@ class FlashAttention(nn.Module):
             return None
         return ops.AttnExtras(self.sinks, self.slopes, head_gate, self.keep_first)
 
+    def takes_kv4(self, dtype: torch.dtype) -> bool:
+        """Whether a cache in 4 bits can stand in for this layer's keys and values."""
+        return (dtype == torch.bfloat16 and self.head_dim in (128, 256) and self.num_heads <= 8 * self.num_kv_heads and
+                self.source is None and not self.lends and self._extras(None) is None)
+
+    def _write_kv4(self, ctx: Context, q, k, v, positions, cos_sin) -> None:
+        if ctx.prefill and ctx.block_table is None:
+            raise ValueError("a cache in 4 bits needs the step's block table: prompts read their keys and values back from it")
+        ops.rotary_kv4_write(q, k, v, positions, cos_sin, ctx.slot_mapping, self.kv4, status=ctx.status)
+        if self.summaries is not None:
+            ops.kv4_summarise(self.kv4, ctx.slot_mapping, self.summaries, status=ctx.status)
+
     def forward(self, ctx: Context, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
-        if self._has_cache():
+        if self.kv4 is not None:
+            self._write_kv4(ctx, None, k, v, None, None)
+        elif self._has_cache():
             ops.rope_kv_write(None, k, v, None, None, ctx.slot_mapping, self.k_cache, self.v_cache,
                               k_in_place=False, status=ctx.status)
         return self._attend(ctx, q, k, v)
@@ -105,6 +139,11 @@ class FlashAttention(nn.Module):
         """q, k NOT yet rotated: RoPE (in place on q and k) + cache write in one kernel, then attention.  ``cos_sin_cache`` None: no
         rotation; ``norm`` (size, eps): q and k are divided by their root mean square behind it; ``row_norm``: norms in front of it, in
         the same kernel.  With a ``source`` k and v are None."""
+        if self.kv4 is not None:
+            if norm is not None or row_norm is not None or head_gate is not None:
+                raise ValueError("a cache in 4 bits goes with plain rotated attention: no norms, no gates")
+            self._write_kv4(ctx, q, k, v, positions, cos_sin_cache)
+            return self._attend(ctx, q, k, v, out)
         if self.source is not None:
             k, v = ctx.shared.get(self.source, (None, None))          # this step's own, for prompts without earlier tokens
             if cos_sin_cache is not None or norm is not None:
@@ -146,16 +185,30 @@ class FlashAttention(nn.Module):
                            positions: torch.Tensor, cos_sin_cache: torch.Tensor, q_weight: torch.Tensor,
                            k_weight: torch.Tensor, eps: float, unit_offset: bool) -> torch.Tensor:
         """q, k straight from the projection (views of the packed qkv output): per-head RMSNorm, RoPE
-        and the cache write in one kernel (q and k updated in place), then attention."""
-        has_cache = self._has_cache()
+        and the cache write in one kernel (q and k updated in place), then attention.  (A cache in 4 bits is written by a kernel of its
+        own behind it.)"""
+        has_cache = self.kv4 is None and self._has_cache()
         ops.qk_norm_rope_kv_write(q, k, v, q_weight, k_weight, eps, unit_offset, positions, cos_sin_cache,
                                   ctx.slot_mapping if has_cache else None, self.k_cache if has_cache else None,
                                   self.v_cache if has_cache else None,
-                                  k_in_place=ctx.prefill and ctx.block_table is None, status=ctx.status)
+                                  k_in_place=self.kv4 is not None or (ctx.prefill and ctx.block_table is None), status=ctx.status)
+        if self.kv4 is not None:
+            self._write_kv4(ctx, None, k, v, None, None)
         return self._attend(ctx, q, k, v)
+
+    def _decode4(self, ctx: Context, q: torch.Tensor, table: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
+        ws = decode4_workspace_for(q.device, q.shape[0], self.num_heads, self.num_kv_heads, self.head_dim)
+        spans = None
+        if self.summaries is not None:
+            spans = ops.kv4_select(q, self.summaries, ctx.cache_seqlens, table, self.kv4.block_size, self.decode_spans, status=ctx.status,
+                                   max_context=self.max_context)
+        return ops.decode_attn4(q, self.kv4, ctx.cache_seqlens, table, self.scaling, self.window_left, ws, spans=spans, out=out,
+                                status=ctx.status, softcap=self.softcap, out_scale=self.out_scale)
 
     def _decode(self, ctx: Context, q: torch.Tensor, table: torch.Tensor, out: torch.Tensor | None = None,
                 extras: ops.AttnExtras | None = None) -> torch.Tensor:
+        if self.kv4 is not None:
+            return self._decode4(ctx, q, table, out)
         (k_cache, v_cache), wl = self._caches(), self.window_left
         kind = (wl, self.keep_first) if self.keep_first else wl
         key = (kind, self.num_heads, self.num_kv_heads, self.head_dim)
@@ -169,6 +222,11 @@ class FlashAttention(nn.Module):
                                status=ctx.status, softcap=self.softcap, out_scale=self.out_scale, extras=extras)
 
     def _prefill(self, ctx: Context, q, k, v, cu_q, cu_k, table, out=None, extras=None) -> torch.Tensor:
+        if table is not None and self.kv4 is not None:
+            # whole contexts, the step's own tokens among them, as the cache gives them back: a token is read alike by every step, in
+            # whichever portions and mixtures prompts come
+            k, v = ops.kv4_gather(self.kv4, cu_k, table, ctx.prompt_keys, status=ctx.status)
+            table = None
         return ops.prefill_attn(q, k, v, cu_q, cu_k, ctx.max_seqlen_q, self.scaling, self.window_left, block_table=table,
                                 out=out, status=ctx.status, items=prefill_items_for(ctx, self), softcap=self.softcap,
                                 out_scale=self.out_scale, extras=extras)
@@ -183,7 +241,7 @@ class FlashAttention(nn.Module):
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         part = (lambda a, b: None) if extras is None else extras.rows
-        self._prefill(ctx, q[:tp], *self._caches(), ctx.cu_seqlens_q[:bp + 1], ctx.cu_seqlens_k[:bp + 1],
+        self._prefill(ctx, q[:tp], *(self._caches() if self.kv4 is None else (None, None)), ctx.cu_seqlens_q[:bp + 1], ctx.cu_seqlens_k[:bp + 1],
                       ctx.block_table[:bp], out[:tp], part(0, tp))
         self._decode(ctx, q[tp:], ctx.block_table[bp:], out[tp:], part(tp, q.shape[0]))
         return out
@@ -193,7 +251,7 @@ class FlashAttention(nn.Module):
         if ctx.prefill and ctx.num_decode:
             return self._attend_mixed(ctx, q, out, extras)
         if ctx.prefill:
-            if ctx.block_table is not None:        # prefix cache in play: keys come from the pool
+            if ctx.block_table is not None and self.kv4 is None:        # prefix cache in play: keys come from the pool
                 k, v = self._caches()
             return self._prefill(ctx, q, k, v, ctx.cu_seqlens_q, ctx.cu_seqlens_k, ctx.block_table, out, extras)
         # decode: q [B,Hq,D] -> [B,1,Hq,D] like flash_attn_with_kvcache on q.unsqueeze(1)

@@ -1473,10 +1473,11 @@ def kv4_summarise(cache: KV4Cache, slot_mapping: torch.Tensor, summaries: torch.
 
 
 def kv4_select(q: torch.Tensor, summaries: torch.Tensor, cache_seqlens: torch.Tensor, block_table: torch.Tensor, block_size: int, budget: int,
-               out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+               out: torch.Tensor | None = None, status: torch.Tensor | None = None, max_context: int | None = None) -> torch.Tensor:
     """The spans of 64 tokens that ``decode_attn4`` should read: int32 ``[B, Hkv, budget]``, ascending, -1 behind them.  Per sequence and KV
     head the ``budget`` (at least 2) spans with the greatest bound on ``q . k``, added up over the group's heads; the first and the last
-    span are always among them, and of equal bounds the lower index is taken."""
+    span are always among them, and of equal bounds the lower index is taken.  ``max_context``: the longest context that may come, where
+    the table is wider than that (None: what the table holds; at most 1 M tokens)."""
     _here((q, torch.bfloat16, "q"), (summaries, torch.bfloat16, "summaries"), (cache_seqlens, torch.int32, "cache_seqlens"),
           (block_table, torch.int32, "block_table"), (out, torch.int32, "out"), (status, torch.int32, "status"))
     _need_shape(q.dim() == 3 and summaries.dim() == 5 and summaries.is_contiguous(), "q must be [sequences, heads, head_dim], summaries contiguous "
@@ -1492,7 +1493,8 @@ def kv4_select(q: torch.Tensor, summaries: torch.Tensor, cache_seqlens: torch.Te
         out = torch.empty((B, hkv, max(budget, 0)), dtype=torch.int32, device=q.device)
     _need_shape(out.shape == (B, hkv, budget) and out.is_contiguous(), "out must be contiguous [sequences, kv heads, budget]")
     rc = _cabi.load().mvb_kv4_select(q.data_ptr(), q_stride, summaries.data_ptr(), blocks, block_size, cache_seqlens.data_ptr(),
-                                     block_table.data_ptr(), stride, width, B, hq, hkv, d, budget, out.data_ptr(), _ptr(status), _stream())
+                                     block_table.data_ptr(), stride, width, B, hq, hkv, d,
+                                     width * block_size if max_context is None else max_context, budget, out.data_ptr(), _ptr(status), _stream())
     if rc:
         _cabi.check(rc, "mvb_kv4_select")
     LaunchCounter.total += 1 if B else 0
