@@ -164,6 +164,11 @@ struct Decode4Run {
   int known, known_row, sel, token, tiles, b, h, n;
 };
 
+// a CTA's tiles and, where whole CTAs are given to rows, the first CTA of its row and their number (first < 0: the even cut)
+struct Decode4Share {
+  int t0, t1, first, parts;
+};
+
 template <int D, bool CAP>
 __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(const Decode4Params p) {
   using C = Decode4Cfg<D>;
@@ -171,84 +176,127 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
   constexpr int NW = C::NW, NT = NW * 32, NST = C::NST, GRP = C::GRP;
   constexpr uint32_t FULL = 0xffffffffu, LO = 0x000f000fu, HI = 0x00f000f0u, BYTE = 0x00ff00ffu;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int scan_s[NW], total_s;
+  __shared__ int total_s;
+  __shared__ Decode4Share cut_s;
   __shared__ int info_s[NW][NST];                            // first token of the tile in a stage, -1: nothing to read
   __shared__ int meta_s[NW][2][3];                           // a warp's parts: row (-1: none), the row's first tile and the one behind its last
   __shared__ Walk fs_s[NW], cs_s[NW];                        // a warp's fetching and computing side
   __shared__ Decode4Run run_s[NW];
-  __shared__ float lse_s[NW][2][kDecode4MaxGroup];           // their log2-sum-exps
+  __shared__ __align__(16) float lse_s[2][kDecode4MaxGroup][NW];            // log2-sum-exps of the warps' first and last parts, -inf: none
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c4 = lane & 3;
   const int G = p.group;
 
-  // ---- the split: a prefix sum of the tile counts in the memory that will be the ring ------------------------------------------------
-  int* prefix = reinterpret_cast<int*>(smem);
-  int running = 0;
-  for (int base = 0; base < p.num_seqs; base += NT) {
-    const int b = base + threadIdx.x;
-    int v = 0;
-    if (b < p.num_seqs) {
-      const int n = p.seqlens[b];
-      if (n > p.max_len) report(p.dev_status, kDevBadLength, b);
-      v = Walk::tiles(p, Walk::length(p, b));
-    }
-    int x = v;
+  // ---- the split.  Every warp works it out for itself: lane i sums up the tiles of the i-th run of neighbouring sequences ---------------
+  const int cta = blockIdx.x;
+  const int lane_seqs = (p.num_seqs + 31) / 32, b0 = min(lane * lane_seqs, p.num_seqs), b1 = min(b0 + lane_seqs, p.num_seqs);
+  auto tiles_of = [&](int b) -> int { return Walk::tiles(p, Walk::length(p, b)); };
+  auto before_me = [&](int own, int& sum) -> int {           // exclusive sum over the lanes, and all of them
+    int x = own;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
       const int y = __shfl_up_sync(FULL, x, off);
       if (lane >= off) x += y;
     }
-    if (lane == 31) scan_s[warp] = x;
-    __syncthreads();
-    int before = running;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const int s = scan_s[w];
-      before += w < warp ? s : 0;
-      running += s;
-    }
-    if (b < p.num_seqs) prefix[b] = before + x - v;
-    if (b == p.num_seqs - 1) { prefix[b + 1] = before + x; total_s = (before + x) * p.hkv; }
-    __syncthreads();
+    sum = __shfl_sync(FULL, x, 31);
+    return x - own;
+  };
+  int own = 0, some = 0, total;
+#pragma unroll 4
+  for (int b = b0; b < b1; ++b) {
+    const int n = p.seqlens[b];
+    if (n > p.max_len && warp == 0) report(p.dev_status, kDevBadLength, b);
+    const int v = Walk::tiles(p, min(n, p.max_len));
+    own += v;
+    some += v > 0;
   }
-  const int cta = blockIdx.x;
-  // sequences without a token: zeros
-  for (int b = cta; b < p.num_seqs; b += gridDim.x) {
-    if (prefix[b] == prefix[b + 1]) {
-      for (int e = threadIdx.x; e < p.hkv * G * D / 8; e += NT)
-        *reinterpret_cast<uint4*>(p.out + b * p.out_stride + e * 8) = make_uint4(0, 0, 0, 0);
+  const int pre = before_me(own, total);
+  some = __reduce_add_sync(FULL, some);
+  total *= p.hkv;
+  if (some < p.num_seqs) {                                   // sequences without a token: zeros
+    for (int b = cta; b < p.num_seqs; b += gridDim.x) {
+      if (p.seqlens[b] <= 0) {
+        for (int e = threadIdx.x; e < p.hkv * G * D / 8; e += NT)
+          *reinterpret_cast<uint4*>(p.out + b * p.out_stride + e * 8) = make_uint4(0, 0, 0, 0);
+      }
     }
   }
+  // Few rows: whole CTAs for each of them, in proportion to its tiles but one for a row of up to three tiles a warp, so that a CTA works on one
+  // row and most need no other CTA.  Where some CTA would get much more than its share, or there are more rows than CTAs: the even cut.
+  // (8 rows of 22 tiles: 15.4 us cut evenly, XX by rows; 128 rows of up to 17 tiles of 256-wide heads: 18.9 and XX; 8 rows of 1280: 30.5 and XX.)
+  const int grid = gridDim.x, share = (total + grid - 1) / grid;
+  const float part_of_grid = static_cast<float>(grid) / static_cast<float>(max(total, 1));
+  auto ctas_of = [&](int v) -> int {                         // (a tile a warp at least: no CTA is left without one)
+    return v == 0 ? 0 : v <= 3 * NW ? 1 : max(1, min(static_cast<int>(static_cast<float>(v) * part_of_grid), v / NW));
+  };
+  Decode4Share mine{0, 0, -1, 0};
+  bool by_rows = false;
+  if (static_cast<int64_t>(some) * p.hkv <= grid) {
+    int ctas = 0, all;
+    bool much = false;
+    const int bound = share + share / 8 + 3 * NW;
+#pragma unroll 4
+    for (int b = b0; b < b1; ++b) {
+      const int v = tiles_of(b), n = ctas_of(v);
+      ctas += n * p.hkv;
+      much |= v > n * bound;
+    }
+    const int pre_ctas = before_me(ctas, all);
+    by_rows = !__any_sync(FULL, much) && all <= grid;
+    if (by_rows) {
+      if (cta >= all) return;
+      int c = pre_ctas, at = pre, n = 1, v = 0;
+      const bool here = cta >= pre_ctas && cta < pre_ctas + ctas;
+      if (here) {
+#pragma unroll 1
+        for (int b = b0; b < b1; ++b, c += n * p.hkv, at += v) {
+          v = tiles_of(b);
+          n = ctas_of(v);
+          if (cta < c + n * p.hkv) break;
+        }
+      }
+      const int src = __ffs(__ballot_sync(FULL, here)) - 1;
+      c = __shfl_sync(FULL, c, src); at = __shfl_sync(FULL, at, src); n = __shfl_sync(FULL, n, src); v = __shfl_sync(FULL, v, src);
+      const int h = (cta - c) / n, i = cta - c - h * n, per = v / n, rest = v - per * n, t0 = (at * p.hkv + h * v) + i * per + min(i, rest);
+      mine = Decode4Share{t0, t0 + per + (i < rest ? 1 : 0), cta - i, n};
+    }
+  }
+  if (!by_rows) {
+    const Decode4Cut cut(total, NW);
+    if (cta >= cut.ctas) return;
+    mine.t0 = cut.start(cta);
+    mine.t1 = cut.start(cta + 1);
+  }
+  if (threadIdx.x == 0) { cut_s = mine; total_s = total; }
   int w0, w1;
   {
-    const Decode4Cut cut(running * p.hkv, NW);
-    if (cta >= cut.ctas) return;
-    const int t0 = cut.start(cta), tiles = cut.start(cta + 1) - t0;
-    w0 = t0 + warp * (tiles / NW) + min(warp, tiles % NW);
+    const int tiles = mine.t1 - mine.t0;
+    w0 = mine.t0 + warp * (tiles / NW) + min(warp, tiles % NW);
     w1 = w0 + tiles / NW + (warp < tiles % NW ? 1 : 0);
   }
   Walk cs;
   int row_t0 = 0;                                            // the number of the row's first tile
   {
-    int lo = 0, size = p.num_seqs;                           // the last b with prefix[b] * hkv <= w0 is in [lo, lo + size)
-    while (size > 1) {
-      const int step = (size + 31) / 32, at = lo + lane * step;
-      const uint32_t below = __ballot_sync(FULL, lane * step < size && prefix[at] * p.hkv <= w0);
-      const int skip = (31 - __clz(below)) * step;           // (lane 0 is always below)
-      lo += skip;
-      size = min(step, size - skip);
+    const int src = 31 - __clz(__ballot_sync(FULL, pre * p.hkv <= w0));     // whose sequences hold tile w0 (of a warp without tiles: anyone's)
+    int b = b0, at = pre, v = 0;
+    if (lane == src) {
+#pragma unroll 1
+      for (; b < b1; ++b, at += v) {
+        v = tiles_of(b);
+        if (w0 < (at + v) * p.hkv) break;
+      }
     }
-    cs.b = lo;
-    cs.n = Walk::length(p, lo);
-    cs.count = prefix[lo + 1] - prefix[lo];
-    const int in_seq = w0 - prefix[lo] * p.hkv;
+    cs.b = min(__shfl_sync(FULL, b, src), p.num_seqs - 1);
+    at = __shfl_sync(FULL, at, src);
+    cs.count = __shfl_sync(FULL, v, src);
+    cs.n = Walk::length(p, cs.b);
+    const int in_seq = w0 - at * p.hkv;
     cs.h = cs.count > 0 ? in_seq / cs.count : 0;
     cs.i = in_seq - cs.h * cs.count;
     row_t0 = w0 - cs.i;
   }
   if (lane < 2) meta_s[warp][lane][0] = -1;
-  if (lane < kDecode4MaxGroup) lse_s[warp][1][lane] = -INFINITY;
-  __syncthreads();                                           // the prefix sums have been read: the ring may be filled
+  if (lane < kDecode4MaxGroup) lse_s[1][lane][warp] = -INFINITY;
 
   // ---- the fetching side ------------------------------------------------------------------------------------------------------------
   const uint32_t ring = smem_u32(smem) + warp * C::RING;
@@ -611,7 +659,7 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
         if (complete) store_vec<__nv_bfloat16, 8>(p.out + b * p.out_stride + (static_cast<int64_t>(h) * G + head) * D + 64 * j + 8 * g, y);
         else store_f32<8>(part + head * D + 64 * j + 8 * g, y);
       }
-      if (!complete && g == 0) lse_s[warp][seg_end == w1 ? 1 : 0][head] = l > 0.f ? m + fast_log2(l) : -INFINITY;
+      if (!complete && g == 0) lse_s[seg_end == w1 ? 1 : 0][head][warp] = l > 0.f ? m + fast_log2(l) : -INFINITY;
     }
     row_t0 = row_t1;
   }
@@ -620,9 +668,10 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
 
   // ---- parts of rows, put together --------------------------------------------------------------------------------------------------
   // The parts of a row are those of neighbouring warps, one of each: last parts in the rings, and perhaps a first part, in the workspace,
-  // of the last of these warps.  This code runs once, from a cold instruction cache: it is kept small, not unrolled.
-  const Decode4Cut cut(total_s, NW);                         // (worked out again: it need not sit in registers meanwhile)
-  const int t0 = cut.start(cta), t1 = cut.start(cta + 1);
+  // of the last of these warps.  This code runs once, from a cold instruction cache and a load behind the other: one copy of it serves all
+  // jobs, and inside it everything that can be requested at once is.
+  const Decode4Share mine_s = cut_s;
+  const int t0 = mine_s.t0, t1 = mine_s.t1;
   const int* meta = &meta_s[0][0][0];
   const int of_lane = lane < NW ? lane : 0;
   const int row_f = lane < NW ? meta_s[of_lane][0][0] : -1, row_l = lane < NW ? meta_s[of_lane][1][0] : -1;
@@ -632,24 +681,27 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
     const int head = e * 4 / D, wf = __ffs(f) - 1;           // (-1: no first part)
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f), acc = v;
     if (wf >= 0) v = *reinterpret_cast<const float4*>(first_parts + wf * decode4_part(G, D) + e * 4);
-    const int lo = l != 0 ? __ffs(l) - 1 : 0, hi = 31 - __clz(l);            // (no last part: hi is -1)
-    const float xf = wf >= 0 ? lse_s[wf][0][head] : -INFINITY;
-    float M = xf, sum = 0.f;
-#pragma unroll 4
-    for (int w = lo; w <= hi; ++w) M = fmaxf(M, lse_s[w][1][head]);          // -inf where a warp has no tiles
-    const float r = M == -INFINITY ? 0.f : M;
-#pragma unroll 4
-    for (int w = lo; w <= hi; ++w) {
-      const float a = fast_exp2(lse_s[w][1][head] - r);
-      if (a > 0.f) {
-        const float4 x = *reinterpret_cast<const float4*>(smem + w * C::RING + e * 16);
-        acc.x = fmaf(a, x.x, acc.x); acc.y = fmaf(a, x.y, acc.y); acc.z = fmaf(a, x.z, acc.z); acc.w = fmaf(a, x.w, acc.w);
-        sum += a;
-      }
+    float x[NW];
+#pragma unroll
+    for (int w = 0; w < NW; w += 4) *reinterpret_cast<float4*>(x + w) = *reinterpret_cast<const float4*>(&lse_s[1][head][w]);
+    const float xf = wf >= 0 ? lse_s[0][head][wf] : -INFINITY;
+    float M = xf;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      if (((l >> w) & 1) == 0) x[w] = -INFINITY;
+      M = fmaxf(M, x[w]);
     }
-    const float a = fast_exp2(xf - r);
-    acc.x = fmaf(a, v.x, acc.x); acc.y = fmaf(a, v.y, acc.y); acc.z = fmaf(a, v.z, acc.z); acc.w = fmaf(a, v.w, acc.w);
-    sum += a;
+    const float r = M == -INFINITY ? 0.f : M;
+    float sum = fast_exp2(xf - r);
+    acc.x = sum * v.x; acc.y = sum * v.y; acc.z = sum * v.z; acc.w = sum * v.w;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float a = fast_exp2(x[w] - r);
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (a > 0.f) y = *reinterpret_cast<const float4*>(smem + w * C::RING + e * 16);      // (a warp without a part has anything there)
+      acc.x = fmaf(a, y.x, acc.x); acc.y = fmaf(a, y.y, acc.y); acc.z = fmaf(a, y.z, acc.z); acc.w = fmaf(a, y.w, acc.w);
+      sum += a;
+    }
     const float inv = sum > 0.f ? 1.f / sum : 0.f;
     acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
     lse = sum > 0.f ? M + fast_log2(sum) : -INFINITY;
@@ -663,7 +715,7 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
   // Job 0, 1: the rows of this warp's own parts, where they end in the CTA; the warps with a part of a row share its outputs.  Job 2, 3: the
   // CTA's first and last row, where they go on in other CTAs: every warp takes D / NW channels of all heads, in every CTA alike.
   constexpr int PIECES = D / NW / 4;                         // 16-byte pieces of a head that a warp takes of such a row
-  const int share = G * PIECES, E4 = G * D / 4;
+  const int owned = G * PIECES, E4 = G * D / 4;
   const uint32_t cross_f = __ballot_sync(FULL, row_f >= 0 && (meta_s[of_lane][0][1] < t0 || meta_s[of_lane][0][2] > t1));
   const uint32_t cross_l = __ballot_sync(FULL, row_l >= 0 && (meta_s[of_lane][1][1] < t0 || meta_s[of_lane][1][2] > t1));
   auto piece = [&](int i) -> int { return i / PIECES * (D / 4) + warp * PIECES + i % PIECES; };   // of the share, as a piece of the row
@@ -683,7 +735,7 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
     if (row < 0 || (job < 2 && (r0 < t0 || r1 > t1))) continue;
     if (job == 3 && row == __shfl_sync(FULL, mine_row, 0)) continue;
     const uint32_t f = __ballot_sync(FULL, row_f == row), l = __ballot_sync(FULL, row_l == row);
-    int at = lane, end = share;
+    int at = lane, end = owned;
     if (job < 2) {
       const int parts = __popc(f | l), mine = __popc((f | l) & ((1u << warp) - 1));
       at = mine * E4 / parts + lane; end = (mine + 1) * E4 / parts;
@@ -705,10 +757,15 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
   }
   // Of the warps with the same channels of a crossing row, the one that arrives last finds all parts of them in memory.
   __syncwarp();                                              // the lanes' parts come before the release
-  int c1 = 0, parts = 0;
-  if (mine_row >= 0) {
-    c1 = cut.of(mine_first);
-    parts = cut.of(mine_last - 1) - c1 + 1;
+  const Decode4Cut cut(total_s, NW);
+  int c1 = mine_s.first, parts = mine_s.parts;
+  if (mine_row < 0) {
+    parts = 0;
+  } else {
+    if (c1 < 0) {
+      c1 = cut.of(mine_first);
+      parts = cut.of(mine_last - 1) - c1 + 1;
+    }
     int32_t* count = p.arrivals + static_cast<int64_t>(mine_row) * NW + warp;
     int prev;
     asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(prev) : "l"(count) : "memory");
@@ -722,27 +779,39 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
     if (n == 0) continue;
     const int from_cta = __shfl_sync(FULL, c1, i), row = __shfl_sync(FULL, mine_row, i), r0 = __shfl_sync(FULL, mine_first, i);
     // a lane takes a piece, or the piece of every n-th part where a warp's share leaves lanes over
-    const int lanes = min(share, 32), split = 32 / lanes, mine = lane / lanes, first = lane - mine * lanes;
+    const int lanes = min(owned, 32), split = 32 / lanes, mine = lane / lanes, first = lane - mine * lanes;
     const float* head_part = p.parts + (static_cast<int64_t>(from_cta) * (NW + 2) + NW) * decode4_part(G, D);
     const int64_t stride = static_cast<int64_t>(NW + 2) * decode4_part(G, D);
-    const int late = r0 <= cut.start(from_cta) ? 0 : decode4_part(G, D);     // the first CTA's part, where the row began inside it
-    for (int base = 0; base < share; base += 32) {
+    const int late = mine_s.first >= 0 || r0 <= cut.start(from_cta) ? 0 : decode4_part(G, D);          // the first CTA's part, where the row began inside it
+    for (int base = 0; base < owned; base += 32) {
       const int e = piece(base + first);
-      const bool works = mine < split && base + first < share;
+      const bool works = mine < split && base + first < owned;
       float M = -INFINITY, sum = 0.f;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
       if (works) {
         const int at_lse = G * D + kDecode4MaxGroup * warp + (base + first) / PIECES;
-#pragma unroll 4
-        for (int c = mine; c < n; c += split) {
-          const float* from = head_part + c * stride + (c == 0 ? late : 0);
-          const float lse = __ldcg(from + at_lse);
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(from + e * 4));
-          const float nm = fmaxf(M, lse), r = nm == -INFINITY ? 0.f : nm;
-          const float a = fast_exp2(M - r), f = fast_exp2(lse - r);
-          acc.x = fmaf(acc.x, a, f * v.x); acc.y = fmaf(acc.y, a, f * v.y); acc.z = fmaf(acc.z, a, f * v.z); acc.w = fmaf(acc.w, a, f * v.w);
-          sum = fmaf(sum, a, f);
-          M = nm;
+        constexpr int AT_ONCE = 8;                           // parts requested before the first is used
+        for (int c0 = mine; c0 < n; c0 += AT_ONCE * split) {
+          float lse[AT_ONCE], most = M;
+          float4 v[AT_ONCE];
+#pragma unroll
+          for (int k = 0; k < AT_ONCE; ++k) {
+            const int c = c0 + k * split;
+            const float* from = head_part + c * stride + (c == 0 ? late : 0);
+            lse[k] = c < n ? __ldcg(from + at_lse) : -INFINITY;
+            v[k] = c < n ? __ldcg(reinterpret_cast<const float4*>(from + e * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+#pragma unroll
+          for (int k = 0; k < AT_ONCE; ++k) most = fmaxf(most, lse[k]);
+          const float r = most == -INFINITY ? 0.f : most, a = fast_exp2(M - r);
+          acc.x *= a; acc.y *= a; acc.z *= a; acc.w *= a; sum *= a;
+          M = most;
+#pragma unroll
+          for (int k = 0; k < AT_ONCE; ++k) {
+            const float f = fast_exp2(lse[k] - r);
+            acc.x = fmaf(f, v[k].x, acc.x); acc.y = fmaf(f, v[k].y, acc.y); acc.z = fmaf(f, v[k].z, acc.z); acc.w = fmaf(f, v[k].w, acc.w);
+            sum += f;
+          }
         }
       }
       float top = M;
@@ -795,8 +864,8 @@ extern "C" int mvb_decode_attn4(const void* q, int64_t q_row_stride, const mvb_k
   if (num_seqs == 0) return kOk;
   if (!q || !out || !cache_seqlens || !block_table || !workspace) return kInvalidArgument;
   if (q_row_stride % 8 || out_row_stride % 8 || !is_aligned(q, 16) || !is_aligned(out, 16) || !is_aligned(workspace, 256)) return kMisaligned;
-  // lengths and tile numbers are 32-bit; the prefix sums of the lengths have the ring's room
-  if (static_cast<int64_t>(table_width) * cache->block_size > 0x7fffffffLL || num_seqs > 16384) return kUnsupportedShape;
+  // lengths and tile numbers are 32-bit
+  if (static_cast<int64_t>(table_width) * cache->block_size > 0x7fffffffLL || num_seqs > 65535) return kUnsupportedShape;
   const int64_t longest = table_width < cache->num_blocks ? table_width : cache->num_blocks;
   if (static_cast<double>(num_seqs) * hkv * longest * (cache->block_size / 32) > 2147483000.0) return kUnsupportedShape;
   if (workspace_bytes < decode4_bytes(num_seqs, hkv)) return kScratchTooSmall;

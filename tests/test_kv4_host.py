@@ -147,7 +147,7 @@ def test_decode_refusals():
     c = cache_struct()
     assert call(c, n=-1) == -1 and call(c, cap=-1.0) == -1 and call(c, cap=float("nan")) == -1 and call(c, tstride=3) == -1
     assert call(c, spans=A) == -1 and call(c, spans=A, budget=4, window=3) == -1 and call(c, ws=None) == -1 and call(c, q=None) == -1
-    assert call(c, hq=7) == -2 and call(c, hq=18) == -2 and call(c, n=20000, size=1 << 40) == -2
+    assert call(c, hq=7) == -2 and call(c, hq=18) == -2 and call(c, n=70000, size=1 << 40) == -2
     assert call(c, stride=1020) == -5 and call(c, q=A + 8) == -5 and call(c, ws=A + 128) == -5
     assert call(c, size=need - 1) == -7
     assert call(c, n=0) == 0
