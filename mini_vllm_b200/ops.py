@@ -1203,23 +1203,59 @@ def moe_gemm(x: torch.Tensor, weight: torch.Tensor, rows: ExpertRows, k: int,
 
 
 # ---- rotation in all its forms, and a paged cache of keys and values in 4 bits ------------------------------------------------------
-def _refuse(t: torch.Tensor, dtype, name: str, device: int) -> None:
+# A call of these is a few microseconds on the GPU where tokens are few, so its checks are written to cost little when all is well: one look
+# at each property, and what was wrong is found out afterwards.
+def _explain(t: torch.Tensor, dtype, device: int, name: str, what: str) -> None:
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor (the kernels have no CPU path)")
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    raise ValueError(f"{name} is on {t.device}; the current device is cuda:{device}")
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}; the current device is cuda:{device}")
+    raise ValueError(f"{name} must be {what}, got {tuple(t.shape)} with strides {t.stride()}")
 
 
-def _here(*named: tuple) -> None:
-    """Every (tensor or None, dtype, name) is a tensor of that type on the current device.  (None: not given.)"""
-    device = -1
-    for t, dtype, name in named:
-        if t is not None:
-            if device < 0 and t.is_cuda:
-                device = _device()
-            if t.dtype is not dtype or t.get_device() != device or device < 0:
-                _refuse(t, dtype, name, device)
+def _rows(t: torch.Tensor, dtype, device: int, shape: tuple, name: str) -> int:
+    """The token stride of a tensor [tokens, heads, size] of this shape with heads next to each other."""
+    if t.dtype is dtype and t.get_device() == device and t.shape == shape:
+        s = t.stride()
+        if s[2] == 1 and (s[1] == shape[2] or shape[1] == 1) or t.numel() == 0:
+            return s[0]
+    return _explain(t, dtype, device, name, f"[tokens, heads, head_dim] = {tuple(shape)} with contiguous heads")
+
+
+def _numbers(t: torch.Tensor, dtype, device: int, least: int, most: int, name: str) -> int:
+    """The address of a contiguous vector of ``least`` .. ``most`` numbers."""
+    if t.dtype is dtype and t.get_device() == device and least <= t.numel() <= most and t.is_contiguous():
+        return t.data_ptr()
+    return _explain(t, dtype, device, name, f"{least} contiguous numbers" + ("" if least == most else " or more"))
+
+
+def _dense(t: torch.Tensor, dtype, device: int, shape: tuple, name: str) -> int:
+    """The address of a contiguous tensor of this shape."""
+    if t.dtype is dtype and t.get_device() == device and t.shape == shape and t.is_contiguous():
+        return t.data_ptr()
+    return _explain(t, dtype, device, name, f"contiguous {tuple(shape)}")
+
+
+def _table(t: torch.Tensor, device: int, rows: int) -> tuple[int, int, int]:
+    """(address, row stride, width) of a block table with at least this many rows."""
+    if t.dtype is torch.int32 and t.get_device() == device:
+        shape, stride = t.shape, t.stride()
+        if len(shape) == 2 and stride[1] == 1 and shape[0] >= rows and shape[1] > 0:
+            return t.data_ptr(), (stride[0] if shape[0] > 1 else shape[1]), shape[1]
+    return _explain(t, torch.int32, device, "block_table", f"[{rows} sequences or more, blocks] with neighbouring blocks of a sequence next to each other")
+
+
+def _angles(t: torch.Tensor, device: int) -> tuple[int, int, int]:
+    """(address, positions, rotated channels) of a table of cosines and sines."""
+    if t.dtype is torch.float32 and t.get_device() == device and t.dim() == 2 and t.is_contiguous():
+        return t.data_ptr(), *t.shape
+    return _explain(t, torch.float32, device, "cos_sin", "contiguous [positions, rotated channels]")
+
+
+def _status(t: torch.Tensor | None, device: int) -> int | None:
+    return None if t is None else _numbers(t, torch.int32, device, 4, 4, "status")
 
 
 def _need_shape(ok: bool, what: str) -> None:
@@ -1227,27 +1263,7 @@ def _need_shape(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def _row_stride(t: torch.Tensor | None, shape: tuple, name: str) -> int:
-    """The token stride of a tensor [tokens, heads, size] of this shape with heads next to each other."""
-    if t is None:
-        return 0
-    if t.shape != shape:
-        raise ValueError(f"{name} must be [tokens, heads, head_dim] = {tuple(shape)}, got {tuple(t.shape)}")
-    s = t.stride()
-    if (s[2] != 1 or (s[1] != shape[2] and shape[1] != 1)) and t.numel():
-        raise ValueError(f"{name} must have contiguous heads")
-    return s[0]
-
-
-def _need_numbers(t: torch.Tensor, n: int, name: str) -> None:
-    if t.numel() != n or not t.is_contiguous():
-        raise ValueError(f"{name} must be one contiguous number per token, {n} of them")
-
-
-def _need_angles(cos_sin: torch.Tensor) -> tuple[int, int]:
-    if cos_sin.dim() != 2 or not cos_sin.is_contiguous():
-        raise ValueError("cos_sin must be [positions, rotated channels], contiguous")
-    return cos_sin.shape
+_BIG = 1 << 62
 
 
 def rotary(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tensor, cos_sin: torch.Tensor, interleaved: bool = False,
@@ -1258,25 +1274,32 @@ def rotary(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tens
     one = q if q is not None else k
     if one is None or (q is None and q_out is not None) or (k is None and k_out is not None):
         raise ValueError("rotary needs q or k, and each output its input")
-    dtype = one.dtype
+    dtype, device = one.dtype, _device() if one.is_cuda else -2
     if dtype not in _DTYPE:
         raise TypeError(f"q and k must be bfloat16 or float32, got {dtype}")
-    if q_out is None:
-        q_out = q
-    if k_out is None:
-        k_out = k
-    _here((q, dtype, "q"), (k, dtype, "k"), (q_out, dtype, "q_out"), (k_out, dtype, "k_out"), (positions, torch.int64, "positions"),
-          (cos_sin, torch.float32, "cos_sin"), (status, torch.int32, "status"))
-    if one.dim() != 3:
-        raise ValueError("q and k must be [tokens, heads, head_dim]")
+    _need_shape(one.dim() == 3, "q and k must be [tokens, heads, head_dim]")
     T, _, d = one.shape
-    hq, hkv = 0 if q is None else q.shape[1], 0 if k is None else k.shape[1]
-    strides = [_row_stride(t, (T, h, d), name) for t, h, name in ((q, hq, "q"), (k, hkv, "k"), (q_out, hq, "q_out"), (k_out, hkv, "k_out"))]
-    _need_numbers(positions, T, "positions")
-    max_pos, rot = _need_angles(cos_sin)
-    rc = _cabi.load().mvb_rotary(_ptr(q), strides[0], _ptr(k), strides[1], _ptr(q_out), strides[2], _ptr(k_out), strides[3],
-                                 positions.data_ptr(), cos_sin.data_ptr(), max_pos, T, hq, hkv, d, rot, 1 if interleaved else 0,
-                                 _DTYPE[dtype], _ptr(status), _stream())
+    hq = hkv = q_stride = k_stride = qo_stride = ko_stride = 0
+    q_ptr = k_ptr = qo_ptr = ko_ptr = None
+    if q is not None:
+        hq = q.shape[1]
+        q_stride, q_ptr = _rows(q, dtype, device, (T, hq, d), "q"), q.data_ptr()
+        if q_out is None:
+            q_out, qo_stride, qo_ptr = q, q_stride, q_ptr
+        else:
+            qo_stride, qo_ptr = _rows(q_out, dtype, device, (T, hq, d), "q_out"), q_out.data_ptr()
+    if k is not None:
+        _need_shape(k.dim() == 3, "q and k must be [tokens, heads, head_dim]")
+        hkv = k.shape[1]
+        k_stride, k_ptr = _rows(k, dtype, device, (T, hkv, d), "k"), k.data_ptr()
+        if k_out is None:
+            k_out, ko_stride, ko_ptr = k, k_stride, k_ptr
+        else:
+            ko_stride, ko_ptr = _rows(k_out, dtype, device, (T, hkv, d), "k_out"), k_out.data_ptr()
+    pos_ptr = _numbers(positions, torch.int64, device, T, T, "positions")
+    cs_ptr, max_pos, rot = _angles(cos_sin, device)
+    rc = _cabi.load().mvb_rotary(q_ptr, q_stride, k_ptr, k_stride, qo_ptr, qo_stride, ko_ptr, ko_stride, pos_ptr, cs_ptr, max_pos, T, hq, hkv, d,
+                                 rot, 1 if interleaved else 0, _DTYPE[dtype], _status(status, device), _stream())
     if rc:
         _cabi.check(rc, "mvb_rotary")
     LaunchCounter.total += 1 if T else 0
@@ -1305,9 +1328,7 @@ class KV4Cache:
             _need_shape(t.device == self.k_codes.device, f"{name} is on {t.device}, k_codes on {self.k_codes.device}")
         sizes = (shape[0], shape[2], shape[1], shape[3] * 2)       # blocks, tokens of a block, heads, channels
         object.__setattr__(self, "sizes", sizes)
-        args = _cabi.KV4Cache(*(t.data_ptr() for t in (self.k_codes, self.k_affine, self.v_codes, self.v_affine)), *sizes)
-        object.__setattr__(self, "_args", args)
-        object.__setattr__(self, "_ref", ctypes.byref(args))
+        object.__setattr__(self, "_made", ((), None, None))
 
     @classmethod
     def empty(cls, num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int, device) -> "KV4Cache":
@@ -1336,12 +1357,17 @@ class KV4Cache:
     def head_dim(self) -> int:
         return self.sizes[3]
 
-    def struct(self):
-        """The C argument."""
-        args = self._args
-        args.k_codes, args.k_affine = self.k_codes.data_ptr(), self.k_affine.data_ptr()
-        args.v_codes, args.v_affine = self.v_codes.data_ptr(), self.v_affine.data_ptr()
-        return self._ref
+    def struct(self, device: int):
+        """The C argument, for calls on a device; made anew when a tensor's memory has changed."""
+        if self.k_codes.get_device() != device:
+            _explain(self.k_codes, torch.uint8, device, "the cache", "")
+        at = (self.k_codes.data_ptr(), self.k_affine.data_ptr(), self.v_codes.data_ptr(), self.v_affine.data_ptr())
+        made = self._made
+        if made[0] != at:
+            args = _cabi.KV4Cache(*at, *self.sizes)
+            made = (at, ctypes.byref(args), args)
+            object.__setattr__(self, "_made", made)
+        return made[1]
 
 
 def rotary_kv4_write(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor | None, cos_sin: torch.Tensor | None,
@@ -1350,62 +1376,52 @@ def rotary_kv4_write(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, p
     """Turns ``q`` (in place or into ``q_out``) and ``k`` as ``rotary`` does, and writes ``k`` and ``v`` in 4 bits to their cache slots
     (-1: none); ``k_in_place``: the turned k also goes back to ``k``.  ``cos_sin`` None: nothing is turned.  bf16; the rotated channels a
     multiple of 16.  Returns the turned q."""
-    if q_out is None:
-        q_out = q
-    elif q is None:
+    if q is None and q_out is not None:
         raise ValueError("q_out needs q")
-    if cos_sin is None:
-        positions = None
-    elif positions is None:
-        raise ValueError("cos_sin needs positions")
-    bf16 = torch.bfloat16
-    _here((k, bf16, "k"), (v, bf16, "v"), (q, bf16, "q"), (q_out, bf16, "q_out"), (positions, torch.int64, "positions"),
-          (cos_sin, torch.float32, "cos_sin"), (slot_mapping, torch.int32, "slot_mapping"), (cache.k_codes, torch.uint8, "the cache"),
-          (status, torch.int32, "status"))
-    T, hq = k.shape[0], 0 if q is None else q.shape[1]
+    device, bf16 = _device() if k.is_cuda else -2, torch.bfloat16
+    _need_shape(k.dim() == 3, "k must be [tokens, heads, head_dim]")
+    T = k.shape[0]
     _, _, hkv, d = cache.sizes
-    k_stride, v_stride = _row_stride(k, (T, hkv, d), "k"), _row_stride(v, (T, hkv, d), "v")
-    q_stride, qo_stride = _row_stride(q, (T, hq, d), "q"), _row_stride(q_out, (T, hq, d), "q_out")
-    _need_numbers(slot_mapping, T, "slot_mapping")
-    max_pos = rot = 0
+    k_stride, v_stride = _rows(k, bf16, device, (T, hkv, d), "k"), _rows(v, bf16, device, (T, hkv, d), "v")
+    hq = q_stride = qo_stride = max_pos = rot = 0
+    q_ptr = qo_ptr = pos_ptr = cs_ptr = None
+    if q is not None:
+        _need_shape(q.dim() == 3, "q must be [tokens, heads, head_dim]")
+        hq = q.shape[1]
+        q_stride, q_ptr = _rows(q, bf16, device, (T, hq, d), "q"), q.data_ptr()
+        if q_out is None:
+            q_out, qo_stride, qo_ptr = q, q_stride, q_ptr
+        else:
+            qo_stride, qo_ptr = _rows(q_out, bf16, device, (T, hq, d), "q_out"), q_out.data_ptr()
     if cos_sin is not None:
-        _need_numbers(positions, T, "positions")
-        max_pos, rot = _need_angles(cos_sin)
-    rc = _cabi.load().mvb_rotary_kv4_write(
-        _ptr(q), q_stride, _ptr(q_out), qo_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride, _ptr(positions), _ptr(cos_sin), max_pos,
-        rot, 1 if interleaved else 0, slot_mapping.data_ptr(), cache.struct(), T, hq, 1 if k_in_place else 0, _ptr(status), _stream())
+        _need_shape(positions is not None, "cos_sin needs positions")
+        pos_ptr = _numbers(positions, torch.int64, device, T, T, "positions")
+        cs_ptr, max_pos, rot = _angles(cos_sin, device)
+    slots_ptr = _numbers(slot_mapping, torch.int32, device, T, T, "slot_mapping")
+    rc = _cabi.load().mvb_rotary_kv4_write(q_ptr, q_stride, qo_ptr, qo_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride, pos_ptr, cs_ptr,
+                                           max_pos, rot, 1 if interleaved else 0, slots_ptr, cache.struct(device), T, hq, 1 if k_in_place else 0,
+                                           _status(status, device), _stream())
     if rc:
         _cabi.check(rc, "mvb_rotary_kv4_write")
     LaunchCounter.total += 1 if T else 0
     return q_out
 
 
-def _need_table(block_table: torch.Tensor, rows: int) -> tuple[int, int]:
-    """(row stride, width) of a block table with at least this many rows."""
-    shape, stride = block_table.shape, block_table.stride()
-    if len(shape) != 2 or stride[1] != 1 or shape[0] < rows or shape[1] == 0:
-        raise ValueError("block_table must be [sequences, blocks] with neighbouring blocks of a sequence next to each other")
-    return max(stride[0], shape[1]) if shape[0] == 1 else stride[0], shape[1]
-
-
 def kv4_gather(cache: KV4Cache, cu_seqlens_k: torch.Tensor, block_table: torch.Tensor, num_rows: int, k_out: torch.Tensor | None = None,
                v_out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The cached contexts of a ragged step as dense bf16 rows ``[num_rows, Hkv, D]``, as ``prefill_attn`` reads them: sequence ``b`` from row
     ``cu_seqlens_k[b]`` on.  ``num_rows`` is the host's count of them; rows behind the last sequence stay as they are."""
-    _here((cu_seqlens_k, torch.int32, "cu_seqlens_k"), (block_table, torch.int32, "block_table"), (k_out, torch.bfloat16, "k_out"),
-          (v_out, torch.bfloat16, "v_out"), (cache.k_codes, torch.uint8, "the cache"), (status, torch.int32, "status"))
+    device, bf16 = _device() if cu_seqlens_k.is_cuda else -2, torch.bfloat16
     n = cu_seqlens_k.numel() - 1
-    _need_shape(n >= 0 and cu_seqlens_k.is_contiguous(), "cu_seqlens_k must be [sequences + 1], contiguous")
-    stride, width = _need_table(block_table, n)
+    cu_ptr = _numbers(cu_seqlens_k, torch.int32, device, 1, _BIG, "cu_seqlens_k")
+    table_ptr, stride, width = _table(block_table, device, n)
     shape = (num_rows, cache.sizes[2], cache.sizes[3])
     if k_out is None:
-        k_out = torch.empty(shape, dtype=torch.bfloat16, device=cu_seqlens_k.device)
+        k_out = torch.empty(shape, dtype=bf16, device=cu_seqlens_k.device)
     if v_out is None:
-        v_out = torch.empty(shape, dtype=torch.bfloat16, device=cu_seqlens_k.device)
-    _need_shape(k_out.shape == shape and k_out.is_contiguous() and v_out.shape == shape and v_out.is_contiguous(),
-                f"k_out and v_out must be contiguous {shape}")
-    rc = _cabi.load().mvb_kv4_gather(cache.struct(), cu_seqlens_k.data_ptr(), block_table.data_ptr(), stride, width, n, num_rows,
-                                     k_out.data_ptr(), v_out.data_ptr(), _ptr(status), _stream())
+        v_out = torch.empty(shape, dtype=bf16, device=cu_seqlens_k.device)
+    rc = _cabi.load().mvb_kv4_gather(cache.struct(device), cu_ptr, table_ptr, stride, width, n, num_rows, _dense(k_out, bf16, device, shape, "k_out"),
+                                     _dense(v_out, bf16, device, shape, "v_out"), _status(status, device), _stream())
     if rc:
         _cabi.check(rc, "mvb_kv4_gather")
     LaunchCounter.total += 1 if n and num_rows else 0
@@ -1425,24 +1441,26 @@ def decode_attn4(q: torch.Tensor, cache: KV4Cache, cache_seqlens: torch.Tensor, 
                  status: torch.Tensor | None = None, softcap: float = 0.0, out_scale: float = 1.0) -> torch.Tensor:
     """``decode_attn`` over a cache in 4 bits: ``q [B, Hq, D]`` bf16, one new token per sequence.  ``spans`` int32 ``[B, Hkv, budget]``
     (``kv4_select``): only these spans of 64 tokens are read, each listed once, entries below 0 skipped.  No plan is needed."""
-    bf16, i32 = torch.bfloat16, torch.int32
-    if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    _here((q, bf16, "q"), (cache_seqlens, i32, "cache_seqlens"), (block_table, i32, "block_table"), (workspace, torch.uint8, "workspace"),
-          (spans, i32, "spans"), (out, bf16, "out"), (cache.k_codes, torch.uint8, "the cache"), (status, i32, "status"))
+    device, bf16, i32 = _device() if q.is_cuda else -2, torch.bfloat16, torch.int32
     _, _, hkv, d = cache.sizes
     _need_shape(q.dim() == 3, "q must be [sequences, heads, head_dim]")
     B, hq, _ = q.shape
-    q_stride, out_stride = _row_stride(q, (B, hq, d), "q"), _row_stride(out, (B, hq, d), "out")
-    _need_shape(cache_seqlens.numel() >= B and cache_seqlens.is_contiguous(), "cache_seqlens must be one contiguous number per sequence")
-    stride, width = _need_table(block_table, B)
-    budget = 0
+    q_stride = _rows(q, bf16, device, (B, hq, d), "q")
+    if out is None:
+        out = torch.empty((B, hq, d), dtype=bf16, device=q.device)
+        out_stride = hq * d
+    else:
+        out_stride = _rows(out, bf16, device, (B, hq, d), "out")
+    lens_ptr = _numbers(cache_seqlens, i32, device, B, _BIG, "cache_seqlens")
+    table_ptr, stride, width = _table(block_table, device, B)
+    spans_ptr, budget = None, 0
     if spans is not None:
-        _need_shape(spans.dim() == 3 and spans.shape[:2] == (B, hkv) and spans.is_contiguous(), "spans must be contiguous [sequences, kv heads, budget]")
-        budget = spans.shape[2]
-    rc = _cabi.load().mvb_decode_attn4(
-        q.data_ptr(), q_stride, cache.struct(), cache_seqlens.data_ptr(), block_table.data_ptr(), stride, width, _ptr(spans), budget, B, hq,
-        scale, window_left, softcap, out_scale, out.data_ptr(), out_stride, workspace.data_ptr(), workspace.numel(), _ptr(status), _stream())
+        budget = spans.shape[-1]
+        spans_ptr = _dense(spans, i32, device, (B, hkv, budget), "spans")
+    ws_ptr = _numbers(workspace, torch.uint8, device, 0, _BIG, "workspace")
+    rc = _cabi.load().mvb_decode_attn4(q.data_ptr(), q_stride, cache.struct(device), lens_ptr, table_ptr, stride, width, spans_ptr, budget, B, hq,
+                                       scale, window_left, softcap, out_scale, out.data_ptr(), out_stride, ws_ptr, workspace.numel(),
+                                       _status(status, device), _stream())
     if rc:
         _cabi.check(rc, "mvb_decode_attn4")
     LaunchCounter.total += 1 if B else 0
@@ -1458,14 +1476,12 @@ def kv4_summaries(cache: KV4Cache) -> torch.Tensor:
 def kv4_summarise(cache: KV4Cache, slot_mapping: torch.Tensor, summaries: torch.Tensor, status: torch.Tensor | None = None) -> torch.Tensor:
     """Renews the bounds of the spans that a step has just written to: per channel the least and the greatest key over the span's rows up to
     the step's last one.  ``slot_mapping`` as for the write, a sequence's tokens next to each other and in order."""
-    _here((slot_mapping, torch.int32, "slot_mapping"), (summaries, torch.bfloat16, "summaries"), (cache.k_codes, torch.uint8, "the cache"),
-          (status, torch.int32, "status"))
+    device = _device() if slot_mapping.is_cuda else -2
     blocks, size, hkv, d = cache.sizes
-    _need_shape(summaries.shape == (blocks, hkv, size // 64, 2, d) and summaries.is_contiguous(),
-                "summaries must be contiguous [blocks, kv heads, block_size / 64, 2, head_dim], as the cache has them")
     T = slot_mapping.numel()
-    _need_numbers(slot_mapping, T, "slot_mapping")
-    rc = _cabi.load().mvb_kv4_summarise(cache.struct(), slot_mapping.data_ptr(), T, summaries.data_ptr(), _ptr(status), _stream())
+    slots_ptr = _numbers(slot_mapping, torch.int32, device, T, T, "slot_mapping")
+    to = _dense(summaries, torch.bfloat16, device, (blocks, hkv, size // 64, 2, d), "summaries")
+    rc = _cabi.load().mvb_kv4_summarise(cache.struct(device), slots_ptr, T, to, _status(status, device), _stream())
     if rc:
         _cabi.check(rc, "mvb_kv4_summarise")
     LaunchCounter.total += 1 if T else 0
@@ -1478,23 +1494,19 @@ def kv4_select(q: torch.Tensor, summaries: torch.Tensor, cache_seqlens: torch.Te
     head the ``budget`` (at least 2) spans with the greatest bound on ``q . k``, added up over the group's heads; the first and the last
     span are always among them, and of equal bounds the lower index is taken.  ``max_context``: the longest context that may come, where
     the table is wider than that (None: what the table holds; at most 1 M tokens)."""
-    _here((q, torch.bfloat16, "q"), (summaries, torch.bfloat16, "summaries"), (cache_seqlens, torch.int32, "cache_seqlens"),
-          (block_table, torch.int32, "block_table"), (out, torch.int32, "out"), (status, torch.int32, "status"))
-    _need_shape(q.dim() == 3 and summaries.dim() == 5 and summaries.is_contiguous(), "q must be [sequences, heads, head_dim], summaries contiguous "
-                "[blocks, kv heads, block_size / 64, 2, head_dim]")
+    device, bf16 = _device() if q.is_cuda else -2, torch.bfloat16
+    _need_shape(q.dim() == 3 and summaries.dim() == 5, "q must be [sequences, heads, head_dim], summaries [blocks, kv heads, block_size / 64, 2, head_dim]")
     B, hq, d = q.shape
-    q_stride = _row_stride(q, (B, hq, d), "q")
-    blocks, hkv, per_block = summaries.shape[:3]
-    _need_shape(per_block * 64 == block_size and summaries.shape[3:] == (2, d), f"summaries {tuple(summaries.shape)} are not those of blocks of "
-                f"{block_size} tokens and heads of {d}")
-    _need_shape(cache_seqlens.numel() >= B and cache_seqlens.is_contiguous(), "cache_seqlens must be one contiguous number per sequence")
-    stride, width = _need_table(block_table, B)
+    blocks, hkv = summaries.shape[:2]
+    q_stride = _rows(q, bf16, device, (B, hq, d), "q")
+    sum_ptr = _dense(summaries, bf16, device, (blocks, hkv, block_size // 64, 2, d), "summaries")
+    lens_ptr = _numbers(cache_seqlens, torch.int32, device, B, _BIG, "cache_seqlens")
+    table_ptr, stride, width = _table(block_table, device, B)
     if out is None:
         out = torch.empty((B, hkv, max(budget, 0)), dtype=torch.int32, device=q.device)
-    _need_shape(out.shape == (B, hkv, budget) and out.is_contiguous(), "out must be contiguous [sequences, kv heads, budget]")
-    rc = _cabi.load().mvb_kv4_select(q.data_ptr(), q_stride, summaries.data_ptr(), blocks, block_size, cache_seqlens.data_ptr(),
-                                     block_table.data_ptr(), stride, width, B, hq, hkv, d,
-                                     width * block_size if max_context is None else max_context, budget, out.data_ptr(), _ptr(status), _stream())
+    rc = _cabi.load().mvb_kv4_select(q.data_ptr(), q_stride, sum_ptr, blocks, block_size, lens_ptr, table_ptr, stride, width, B, hq, hkv, d,
+                                     width * block_size if max_context is None else max_context, budget,
+                                     _dense(out, torch.int32, device, (B, hkv, max(budget, 0)), "out"), _status(status, device), _stream())
     if rc:
         _cabi.check(rc, "mvb_kv4_select")
     LaunchCounter.total += 1 if B else 0
