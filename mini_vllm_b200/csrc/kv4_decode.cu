@@ -77,7 +77,7 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(                                                       // (not volatile: the compiler may interleave the products of a tile)
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -93,13 +93,15 @@ __device__ __forceinline__ float fast_log2(float x) {
   return y;
 }
 template <int N>
-__device__ __forceinline__ void lds_words(uint32_t addr, uint32_t (&w)[N]) {
+__device__ __forceinline__ void lds_words(const uint8_t* at, uint32_t (&w)[N]) {
   if constexpr (N == 1) {
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
+    w[0] = *reinterpret_cast<const uint32_t*>(at);
   } else if constexpr (N == 2) {
-    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+    const uint2 u = *reinterpret_cast<const uint2*>(at);
+    w[0] = u.x; w[1] = u.y;
   } else {
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
+    const uint4 u = *reinterpret_cast<const uint4*>(at);
+    w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
   }
 }
 
@@ -118,7 +120,8 @@ __device__ __forceinline__ uint32_t value_piece(int t, int piece) {
 // the token (of eight) that stands in row r of a fragment
 __device__ __forceinline__ int decode4_row(int r) { return r ^ ((r >> 1) & 1); }
 
-// The tiles of a (sequence, head) row, one after the other.
+// The tiles of a (sequence, head) row, one after the other.  Tile 0 holds no tokens: it stands for what a row costs besides them (its q, its
+// end; 1.7 us against 2.0 for a tile, with all SMs busy), so that warps with many short rows get no more work than the others.
 template <int TOK>
 struct Decode4Walk {
   int b, h, i, count, n;               // tile i of `count` of head h of sequence b, which has n tokens
@@ -130,8 +133,8 @@ struct Decode4Walk {
   }
   __device__ __forceinline__ static int tiles(const Decode4Params& p, int n) {
     if (n <= 0) return 0;
-    if (p.spans != nullptr) return (kKv4Span / TOK) * min(p.budget, (n + kKv4Span - 1) / kKv4Span);
-    return (n + TOK - 1) / TOK - first_tile(p, n);
+    if (p.spans != nullptr) return 1 + (kKv4Span / TOK) * min(p.budget, (n + kKv4Span - 1) / kKv4Span);
+    return 1 + (n + TOK - 1) / TOK - first_tile(p, n);
   }
   __device__ __forceinline__ void next(const Decode4Params& p) {
     if (++i < count) return;
@@ -310,11 +313,15 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
   auto look = [&]() {                                        // the next run; its block may still be on its way
     if (ft >= w1) return;
     Walk fs = fs_s[warp];                                    // the first tile that no run covers yet
+    if (fs.i == 0) {
+      fs.i = 1;
+      if (++ft >= w1) return;
+    }
     int known = run_s[warp].known, known_row = run_s[warp].known_row, run_token;
     const int32_t* table = p.block_table + fs.b * p.table_stride;
     int at, room;
     if (p.spans == nullptr) {
-      run_token = (Walk::first_tile(p, fs.n) + fs.i) * C::TOK;
+      run_token = (Walk::first_tile(p, fs.n) + fs.i - 1) * C::TOK;
       at = static_cast<int>(p.by_block.div(run_token));
       room = ((at + 1) * p.block_size - run_token) / C::TOK;
       if (known_row != fs.b || at < known || at >= known + 32) {
@@ -324,9 +331,9 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
     } else {
       constexpr int PER = kKv4Span / C::TOK;
       const int row = fs.b * p.hkv + fs.h;
-      at = fs.i / PER;
-      room = PER - fs.i % PER;
-      run_token = (fs.i % PER) * C::TOK;
+      at = (fs.i - 1) / PER;
+      room = PER - (fs.i - 1) % PER;
+      run_token = ((fs.i - 1) % PER) * C::TOK;
       if (known_row != row || at >= known + 32) {
         known = at; known_row = row;
         const int span = at + lane < p.budget ? __ldg(p.spans + static_cast<int64_t>(row) * p.budget + at + lane) : -1;
@@ -467,11 +474,12 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
     for (int j = 0; j < GRP; ++j) pm_a[j] = pm_b[j] = 0.f;
 
     for (; t < seg_end; ++t) {
+      if (t == row_t0) continue;                             // (the tile without tokens)
       cp_async_wait<NST - 2>();
       __syncwarp();                                          // the tile is there for every lane, and the one before has been read by all
       fetch();
       const int token0 = info_s[warp][stage];
-      const uint32_t at = ring + stage * C::STAGE;
+      const uint8_t* at = smem + warp * C::RING + stage * C::STAGE;
       stage = stage + 1 == NST ? 0 : stage + 1;
       if (token0 < 0) continue;
 
@@ -574,7 +582,7 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
         l_a += p0 + p2; l_b += p1 + p3;
         uint32_t v00[C::WV], v01[C::WV], v10[C::WV], v11[C::WV];
         const int u0 = 16 * s + vt0, u1 = 16 * s + vt1;
-        const uint32_t vat = at + C::CODES;
+        const uint8_t* vat = at + C::CODES;
         auto value = [&](int tok, uint32_t (&w)[C::WV]) {
           if constexpr (D == 256) lds_words<4>(vat + value_piece<D>(tok, g), w);
           else lds_words<C::WV>(vat + value_piece<D>(tok, D == 128 ? g >> 1 : g >> 2) + (D == 128 ? (g & 1) * 8 : (g & 3) * 4), w);
@@ -664,43 +672,53 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
     row_t0 = row_t1;
   }
   cp_async_wait<0>();
+  __syncwarp();
+  // a first part comes back to the ring's second place, so that what follows reads shared memory alone
+  constexpr int SECOND = kDecode4MaxGroup * D * 4;
+  static_assert(2 * SECOND <= C::RING, "two parts have to fit into a ring");
+  if (meta_s[warp][0][0] >= 0) {
+    const float* from = p.parts + (static_cast<int64_t>(cta) * (NW + 2) + warp) * decode4_part(G, D);
+    for (int e = lane; e < G * D / 4; e += 32)
+      *reinterpret_cast<float4*>(smem + warp * C::RING + SECOND + e * 16) = *reinterpret_cast<const float4*>(from + e * 4);
+  }
   __syncthreads();
 
   // ---- parts of rows, put together --------------------------------------------------------------------------------------------------
-  // The parts of a row are those of neighbouring warps, one of each: last parts in the rings, and perhaps a first part, in the workspace,
-  // of the last of these warps.  This code runs once, from a cold instruction cache and a load behind the other: one copy of it serves all
-  // jobs, and inside it everything that can be requested at once is.
+  // The parts of a row are those of neighbouring warps, one of each: last parts, and perhaps a first part of the last of these warps.  This
+  // code runs once, from a cold instruction cache and a load behind the other: one copy of it serves all jobs, and inside it what can be
+  // requested at once is.
   const Decode4Share mine_s = cut_s;
   const int t0 = mine_s.t0, t1 = mine_s.t1;
   const int* meta = &meta_s[0][0][0];
   const int of_lane = lane < NW ? lane : 0;
   const int row_f = lane < NW ? meta_s[of_lane][0][0] : -1, row_l = lane < NW ? meta_s[of_lane][1][0] : -1;
-  const float* first_parts = p.parts + static_cast<int64_t>(cta) * (NW + 2) * decode4_part(G, D);
   // four outputs of a row and the log2-sum-exp of their head, from the warps of the masks
   auto sum_parts = [&](uint32_t f, uint32_t l, int e, float& lse) -> float4 {
     const int head = e * 4 / D, wf = __ffs(f) - 1;           // (-1: no first part)
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f), acc = v;
-    if (wf >= 0) v = *reinterpret_cast<const float4*>(first_parts + wf * decode4_part(G, D) + e * 4);
-    float x[NW];
-#pragma unroll
-    for (int w = 0; w < NW; w += 4) *reinterpret_cast<float4*>(x + w) = *reinterpret_cast<const float4*>(&lse_s[1][head][w]);
+    const int lo = l != 0 ? __ffs(l) - 1 : 0, hi = 31 - __clz(l);            // (no last part: hi is -1)
     const float xf = wf >= 0 ? lse_s[0][head][wf] : -INFINITY;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float M = xf;
+    for (int w0 = lo; w0 <= hi; w0 += 4) {
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      if (((l >> w) & 1) == 0) x[w] = -INFINITY;
-      M = fmaxf(M, x[w]);
+      for (int k = 0; k < 4; ++k) M = fmaxf(M, w0 + k <= hi ? lse_s[1][head][w0 + k] : -INFINITY);       // (-inf: a warp without tiles)
     }
     const float r = M == -INFINITY ? 0.f : M;
     float sum = fast_exp2(xf - r);
-    acc.x = sum * v.x; acc.y = sum * v.y; acc.z = sum * v.z; acc.w = sum * v.w;
+    if (wf >= 0) {
+      const float4 y = *reinterpret_cast<const float4*>(smem + wf * C::RING + SECOND + e * 16);
+      acc.x = sum * y.x; acc.y = sum * y.y; acc.z = sum * y.z; acc.w = sum * y.w;
+    }
+    for (int w0 = lo; w0 <= hi; w0 += 4) {
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float a = fast_exp2(x[w] - r);
-      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (a > 0.f) y = *reinterpret_cast<const float4*>(smem + w * C::RING + e * 16);      // (a warp without a part has anything there)
-      acc.x = fmaf(a, y.x, acc.x); acc.y = fmaf(a, y.y, acc.y); acc.z = fmaf(a, y.z, acc.z); acc.w = fmaf(a, y.w, acc.w);
-      sum += a;
+      for (int k = 0; k < 4; ++k) {
+        const float x = w0 + k <= hi ? lse_s[1][head][w0 + k] : -INFINITY;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (x > -INFINITY) y = *reinterpret_cast<const float4*>(smem + (w0 + k) * C::RING + e * 16);
+        const float a = fast_exp2(x - r);
+        acc.x = fmaf(a, y.x, acc.x); acc.y = fmaf(a, y.y, acc.y); acc.z = fmaf(a, y.z, acc.z); acc.w = fmaf(a, y.w, acc.w);
+        sum += a;
+      }
     }
     const float inv = sum > 0.f ? 1.f / sum : 0.f;
     acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
@@ -867,7 +885,7 @@ extern "C" int mvb_decode_attn4(const void* q, int64_t q_row_stride, const mvb_k
   // lengths and tile numbers are 32-bit
   if (static_cast<int64_t>(table_width) * cache->block_size > 0x7fffffffLL || num_seqs > 65535) return kUnsupportedShape;
   const int64_t longest = table_width < cache->num_blocks ? table_width : cache->num_blocks;
-  if (static_cast<double>(num_seqs) * hkv * longest * (cache->block_size / 32) > 2147483000.0) return kUnsupportedShape;
+  if (static_cast<double>(num_seqs) * hkv * (longest * (cache->block_size / 32) + 1) > 2147483000.0) return kUnsupportedShape;
   if (workspace_bytes < decode4_bytes(num_seqs, hkv)) return kScratchTooSmall;
   const float kLog2e = 1.4426950408889634f;
   Decode4Params p;
