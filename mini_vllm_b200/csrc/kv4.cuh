@@ -43,14 +43,15 @@ __device__ __forceinline__ float kv4_min(uint32_t affine) { return __uint_as_flo
 // What the eight codes of a word stand for; the product is exact in fp32 and the sum is rounded once.  A code becomes a float as the last
 // bits of 2^23 + 16^i c, less 2^23 and over 16^i in one exact step: one integer instruction a code, the rest on the multipliers.
 __device__ __forceinline__ void kv4_values(uint32_t word, uint32_t affine, float (&v)[8]) {
-  const float s = kv4_scale(affine), m = kv4_min(affine);
+  const float2 s = make_float2(kv4_scale(affine), kv4_scale(affine)), m = make_float2(kv4_min(affine), kv4_min(affine));
   const uint32_t upper = word >> 16;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int place = 4 * (e >> 1);
-    const uint32_t x = (((e & 1) ? upper : word) & (15u << place)) | 0x4b000000u;
-    const float unit = 1.f / static_cast<float>(1u << place);
-    v[e] = fmaf(s, fmaf(__uint_as_float(x), unit, -8388608.f * unit), m);
+  for (int i = 0; i < 4; ++i) {                              // channels 2 i and 2 i + 1
+    const uint32_t mask = 15u << (4 * i);
+    const float unit = 1.f / static_cast<float>(1u << (4 * i)), less = -8388608.f * unit;
+    const float2 x = make_float2(__uint_as_float((word & mask) | 0x4b000000u), __uint_as_float((upper & mask) | 0x4b000000u));
+    const float2 y = fma_f32x2(s, fma_f32x2(x, make_float2(unit, unit), make_float2(less, less)), m);
+    v[2 * i] = y.x; v[2 * i + 1] = y.y;
   }
 }
 

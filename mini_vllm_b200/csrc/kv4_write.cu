@@ -36,14 +36,15 @@ struct Kv4WriteParams {
 // quotient: with f0 = t r the remainder t - f0 s takes 8 bits (s has 8) and is exact, f0 + r (t - f0 s) is within 2^-44 of t / s, and no
 // such quotient is that near the middle between two fp32 numbers.  So halves are halves and go to the even code.  Adding 1.5 * 2^23 rounds
 // to a whole number, which then stands in the float's last bits.
-__device__ __forceinline__ uint32_t kv4_codes(const float (&t)[8], float s, float r) {
+__device__ __forceinline__ uint32_t kv4_codes(const float2 (&t)[4], float s, float r) {
   constexpr float kRound = 12582912.f;
   constexpr uint32_t kPlaces = 0x11111111u;                  // one in each of the eight 4-bit places
+  const float2 r2 = make_float2(r, r), minus_s = make_float2(-s, -s), round2 = make_float2(kRound, kRound);
   uint32_t word = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float f0 = __fmul_rn(t[e], r), f = fmaf(fmaf(-f0, s, t[e]), r, f0);
-    word += __float_as_uint(__fadd_rn(f, kRound)) << kv4_shift(e);
+  for (int e = 0; e < 4; ++e) {
+    const float2 f0 = mul_f32x2(t[e], r2), f = add_f32x2(fma_f32x2(fma_f32x2(f0, minus_s, t[e]), r2, f0), round2);
+    word += (__float_as_uint(f.x) << kv4_shift(2 * e)) + (__float_as_uint(f.y) << kv4_shift(2 * e + 1));
   }
   return word - __float_as_uint(kRound) * kPlaces;           // modulo 2^32: the codes alone remain
 }
@@ -83,7 +84,7 @@ __global__ void __launch_bounds__(256, ITEMS == 4 ? 4 : 1) kv4_write_kernel(cons
   }
   const bool turns = p.cos_sin != nullptr && c * 8 < p.rot;  // this lane's channels are rotated
   bool ok = true;
-  float cs[8], sn[8];
+  float2 cs[4], sn[4];                                       // of channels 2 e and 2 e + 1 of the lane (neighbours: of pair e, twice)
   const bool second = !INTER && c * 8 >= half;               // halves: the lane holds the second one of its pairs
   const int partner = sub * LPH + (turns ? (second ? c - half / 8 : c + half / 8) : c);
   if (p.cos_sin != nullptr) {
@@ -92,10 +93,18 @@ __global__ void __launch_bounds__(256, ITEMS == 4 ? 4 : 1) kv4_write_kernel(cons
     if (!ok && lane == 0) report(p.dev_status, kDevBadPosition, t);
     if (turns && ok) {
       const float* tab = p.cos_sin + pos * p.rot + (INTER ? c * 4 : (second ? c * 8 - half : c * 8));
+      if constexpr (INTER) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(tab)), b = __ldg(reinterpret_cast<const float4*>(tab + half));
+        cs[0] = make_float2(a.x, a.x); cs[1] = make_float2(a.y, a.y); cs[2] = make_float2(a.z, a.z); cs[3] = make_float2(a.w, a.w);
+        sn[0] = make_float2(-b.x, b.x); sn[1] = make_float2(-b.y, b.y); sn[2] = make_float2(-b.z, b.z); sn[3] = make_float2(-b.w, b.w);
+      } else {
+        const float sign = second ? 1.f : -1.f;              // (a sign changes no rounding)
 #pragma unroll
-      for (int e = 0; e < (INTER ? 4 : 8); e += 4) {
-        *reinterpret_cast<float4*>(cs + e) = __ldg(reinterpret_cast<const float4*>(tab + e));
-        *reinterpret_cast<float4*>(sn + e) = __ldg(reinterpret_cast<const float4*>(tab + half + e));
+        for (int e = 0; e < 4; e += 2) {
+          const float4 a = __ldg(reinterpret_cast<const float4*>(tab + 2 * e)), b = __ldg(reinterpret_cast<const float4*>(tab + half + 2 * e));
+          cs[e] = make_float2(a.x, a.y); cs[e + 1] = make_float2(a.z, a.w);
+          sn[e] = make_float2(sign * b.x, sign * b.y); sn[e + 1] = make_float2(sign * b.z, sign * b.w);
+        }
       }
     }
   }
@@ -111,7 +120,7 @@ __global__ void __launch_bounds__(256, ITEMS == 4 ? 4 : 1) kv4_write_kernel(cons
   for (int i = 0; i < ITEMS; ++i) {
     const int row = row0 + i * RPW;
     const bool is_q = row < p.hq, is_v = row >= p.hq + p.hkv;
-    float y[8];
+    float2 y[4];
     {
       const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
       uint32_t o[4] = {0, 0, 0, 0};
@@ -120,27 +129,19 @@ __global__ void __launch_bounds__(256, ITEMS == 4 ? 4 : 1) kv4_write_kernel(cons
         for (int e = 0; e < 4; ++e) o[e] = __shfl_sync(FULL, w[e], partner);
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) { y[2 * e] = bf16_lo(w[e]); y[2 * e + 1] = bf16_hi(w[e]); }
+      for (int e = 0; e < 4; ++e) y[e] = make_float2(bf16_lo(w[e]), bf16_hi(w[e]));
       if (turns && ok && !is_v) {
-        if constexpr (INTER) {
+        // own cos +- other sin: two products and a sum, each rounded by itself (the paired instructions get fused)
+        uint32_t r[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float a = y[2 * e], b = y[2 * e + 1];
-            y[2 * e] = __fsub_rn(__fmul_rn(a, cs[e]), __fmul_rn(b, sn[e]));
-            y[2 * e + 1] = __fadd_rn(__fmul_rn(b, cs[e]), __fmul_rn(a, sn[e]));
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float other = (e & 1) ? bf16_hi(o[e >> 1]) : bf16_lo(o[e >> 1]);
-            const float a = __fmul_rn(y[e], cs[e]), b = __fmul_rn(other, sn[e]);
-            y[e] = second ? __fadd_rn(a, b) : __fsub_rn(a, b);
-          }
+        for (int e = 0; e < 4; ++e) {
+          const float2 other = INTER ? make_float2(y[e].y, y[e].x) : make_float2(bf16_lo(o[e]), bf16_hi(o[e]));
+          r[e] = pack_bf16(__fadd_rn(__fmul_rn(y[e].x, cs[e].x), __fmul_rn(other.x, sn[e].x)),
+                           __fadd_rn(__fmul_rn(y[e].y, cs[e].y), __fmul_rn(other.y, sn[e].y)));
         }
-        x[i] = make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
-        const uint32_t r[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        x[i] = make_uint4(r[0], r[1], r[2], r[3]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { y[2 * e] = bf16_lo(r[e]); y[2 * e + 1] = bf16_hi(r[e]); }
+        for (int e = 0; e < 4; ++e) y[e] = make_float2(bf16_lo(r[e]), bf16_hi(r[e]));
       }
     }
     if (row < rows && is_q) *reinterpret_cast<uint4*>(p.q_out + static_cast<int64_t>(t) * p.qo_stride + static_cast<int64_t>(row) * D + c * 8) = x[i];
@@ -156,15 +157,18 @@ __global__ void __launch_bounds__(256, ITEMS == 4 ? 4 : 1) kv4_write_kernel(cons
     const float lo = bf16_lo(pair), hi = -bf16_hi(pair);
     if (row >= rows || is_q) continue;
     const float scale = __bfloat162float(__float2bfloat16_rn(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f)));
-    float d[8];
+    float2 d[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) d[e] = __fsub_rn(y[e], lo);
+    for (int e = 0; e < 4; ++e) d[e] = add_f32x2(y[e], make_float2(-lo, -lo));
     uint32_t word = 0;
     if (scale > 0x1p-100f && scale < 0x1p100f) {             // the usual case: the reciprocal is a normal number, no code passes 15
       word = kv4_codes(d, scale, fast_rcp(scale));
     } else if (scale > 0.f) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) word |= (static_cast<uint32_t>(fminf(rintf(__fdiv_rn(d[e], scale)), 15.f)) & 15u) << kv4_shift(e);
+      for (int e = 0; e < 4; ++e) {
+        word |= (static_cast<uint32_t>(fminf(rintf(__fdiv_rn(d[e].x, scale)), 15.f)) & 15u) << kv4_shift(2 * e);
+        word |= (static_cast<uint32_t>(fminf(rintf(__fdiv_rn(d[e].y, scale)), 15.f)) & 15u) << kv4_shift(2 * e + 1);
+      }
     }
     const int h = row - p.hq - (is_v ? p.hkv : 0);
     const int64_t at = kv4_row(block, p.hkv, h, p.block_size, in_block);
@@ -185,6 +189,7 @@ struct Kv4GatherParams {
   int* dev_status;
 };
 
+// A lane takes eight channels of the key and of the value of a head, whose places in the cache differ by the base address only.
 template <int D, int ITEMS>
 __global__ void __launch_bounds__(256) kv4_gather_kernel(const Kv4GatherParams p) {
   constexpr int LPH = D / 8, RPW = 32 / LPH;
@@ -200,29 +205,29 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(const Kv4GatherParams p
   const int64_t block = col < p.table_width ? p.block_table[b * p.table_stride + col] : -1;
   const bool ok = block >= 0 && block < p.num_blocks;
   if (!ok && lane == 0) report(p.dev_status, kDevBadBlock, b);
-  const int in_block = token - col * p.block_size;
-  const int row0 = static_cast<int>(warp - t * p.by_token.n) * (RPW * ITEMS) + sub;
-  uint32_t word[ITEMS], affine[ITEMS];
+  const int head0 = static_cast<int>(warp - t * p.by_token.n) * (RPW * ITEMS) + sub;
+  const int64_t row = ok ? kv4_row(block, p.hkv, head0, p.block_size, token - col * p.block_size) : 0;
+  const uint32_t *kc = p.k_codes + row * (D / 8) + kv4_word<D>(c, true), *vc = p.v_codes + row * (D / 8) + kv4_word<D>(c, false);
+  const uint32_t *ka = p.k_affine + row * (D / 64) + (c >> 3), *va = p.v_affine + row * (D / 64) + (c >> 3);
+  const int64_t code_step = static_cast<int64_t>(RPW) * p.block_size * (D / 8), affine_step = static_cast<int64_t>(RPW) * p.block_size * (D / 64);
+  uint32_t word[ITEMS][2], affine[ITEMS][2];
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
-    const int row = row0 + i * RPW;
-    word[i] = affine[i] = 0;                                 // a bad block reads as zeros
-    if (row < 2 * p.hkv && ok) {
-      const bool is_v = row >= p.hkv;
-      const int64_t at = kv4_row(block, p.hkv, is_v ? row - p.hkv : row, p.block_size, in_block);
-      word[i] = __ldg((is_v ? p.v_codes : p.k_codes) + at * (D / 8) + kv4_word<D>(c, !is_v));
-      affine[i] = __ldg((is_v ? p.v_affine : p.k_affine) + at * (D / 64) + (c >> 3));
+    word[i][0] = word[i][1] = affine[i][0] = affine[i][1] = 0;           // a bad block reads as zeros
+    if (head0 + i * RPW < p.hkv && ok) {
+      word[i][0] = __ldg(kc + i * code_step); word[i][1] = __ldg(vc + i * code_step);
+      affine[i][0] = __ldg(ka + i * affine_step); affine[i][1] = __ldg(va + i * affine_step);
     }
   }
+  const int64_t to = (static_cast<int64_t>(t) * p.hkv + head0) * D + c * 8;
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
-    const int row = row0 + i * RPW;
-    if (row >= 2 * p.hkv) continue;
-    const bool is_v = row >= p.hkv;
+    if (head0 + i * RPW >= p.hkv) continue;
     float y[8];
-    kv4_values(word[i], affine[i], y);
-    __nv_bfloat16* dst = (is_v ? p.v_out : p.k_out) + (static_cast<int64_t>(t) * p.hkv + (is_v ? row - p.hkv : row)) * D;
-    store_vec<__nv_bfloat16, 8>(dst + c * 8, y);
+    kv4_values(word[i][0], affine[i][0], y);
+    store_vec<__nv_bfloat16, 8>(p.k_out + to + i * RPW * D, y);
+    kv4_values(word[i][1], affine[i][1], y);
+    store_vec<__nv_bfloat16, 8>(p.v_out + to + i * RPW * D, y);
   }
 }
 
@@ -304,8 +309,8 @@ extern "C" int mvb_kv4_gather(const mvb_kv4_cache* cache, const int32_t* cu_seql
   p.dev_status = dev_status;
   return by_head_dim(cache->head_dim, [&](auto tag) -> int {
     constexpr int D = decltype(tag)::value;
-    constexpr int RPW = 32 / (D / 8), ITEMS = 4;
-    const int64_t groups = (2 * static_cast<int64_t>(p.hkv) + RPW - 1) / RPW, per_token = (groups + ITEMS - 1) / ITEMS;
+    constexpr int RPW = 32 / (D / 8), ITEMS = D == 256 ? 2 : 4;
+    const int64_t groups = (static_cast<int64_t>(p.hkv) + RPW - 1) / RPW, per_token = (groups + ITEMS - 1) / ITEMS;
     const int64_t warps = per_token * num_rows;
     if (warps > 0x7fffffffLL - 8) return kUnsupportedShape;
     Kv4GatherParams r = p;
