@@ -29,6 +29,7 @@ struct Kv4WriteParams {
   int64_t num_slots;
   FastDiv by_block, by_token;
   int tokens, hq, hkv, block_size, rot, k_in_place;
+  int q_warps, k_warps;                // of a token
   int* dev_status;
 };
 
@@ -58,6 +59,7 @@ __device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&x);
 }
 
+// A warp works on queries, on keys or on values of its token: `by_token` counts the warps of a token, those of q first, then those of k.
 template <int D, bool INTER, int ITEMS>
 __global__ void __launch_bounds__(256, ITEMS == 4 ? 4 : 1) kv4_write_kernel(const Kv4WriteParams p) {
   constexpr int LPH = D / 8, RPW = 32 / LPH;                 // lanes of a row, rows a warp holds at once
@@ -66,88 +68,97 @@ __global__ void __launch_bounds__(256, ITEMS == 4 ? 4 : 1) kv4_write_kernel(cons
   const uint32_t warp = blockIdx.x * 8 + (threadIdx.x >> 5);
   const uint32_t t = p.by_token.div(warp);
   if (t >= static_cast<uint32_t>(p.tokens)) return;          // warp-uniform
-  const int rows = p.hq + 2 * p.hkv;
-  const int row0 = static_cast<int>(warp - t * p.by_token.n) * (RPW * ITEMS) + sub;
-  const int half = p.rot >> 1;
-
+  int part = static_cast<int>(warp - t * p.by_token.n);
+  const bool is_q = part < p.q_warps;
+  if (!is_q) part -= p.q_warps;
+  const bool is_v = !is_q && part >= p.k_warps;
+  if (is_v) part -= p.k_warps;
+  const int heads = is_q ? p.hq : p.hkv, head0 = part * (RPW * ITEMS) + sub;
+  const __nv_bfloat16* src = is_q ? p.q + static_cast<int64_t>(t) * p.q_stride
+                                  : is_v ? p.v + static_cast<int64_t>(t) * p.v_stride : p.k + static_cast<int64_t>(t) * p.k_stride;
+  src += static_cast<int64_t>(head0) * D + c * 8;
   uint4 x[ITEMS];
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
-    const int row = row0 + i * RPW;
     x[i] = make_uint4(0, 0, 0, 0);
-    if (row < rows) {
-      const __nv_bfloat16* src = row < p.hq ? p.q + static_cast<int64_t>(t) * p.q_stride + static_cast<int64_t>(row) * D
-                                 : row < p.hq + p.hkv ? p.k + static_cast<int64_t>(t) * p.k_stride + static_cast<int64_t>(row - p.hq) * D
-                                                      : p.v + static_cast<int64_t>(t) * p.v_stride + static_cast<int64_t>(row - p.hq - p.hkv) * D;
-      x[i] = *reinterpret_cast<const uint4*>(src + c * 8);
+    if (head0 + i * RPW < heads) x[i] = *reinterpret_cast<const uint4*>(src + i * RPW * D);
+  }
+  int64_t slot = -1;
+  if (!is_q) {
+    slot = p.slots[t];
+    if (slot < -1 || slot >= p.num_slots) {
+      if (lane == 0) report(p.dev_status, kDevBadSlot, t);
+      slot = -1;
     }
   }
-  const bool turns = p.cos_sin != nullptr && c * 8 < p.rot;  // this lane's channels are rotated
-  bool ok = true;
-  float2 cs[4], sn[4];                                       // of channels 2 e and 2 e + 1 of the lane (neighbours: of pair e, twice)
-  const bool second = !INTER && c * 8 >= half;               // halves: the lane holds the second one of its pairs
-  const int partner = sub * LPH + (turns ? (second ? c - half / 8 : c + half / 8) : c);
-  if (p.cos_sin != nullptr) {
+  if (p.cos_sin != nullptr && !is_v) {
+    const int half = p.rot >> 1;
+    const bool turns = c * 8 < p.rot;                        // this lane's channels are rotated
+    const bool second = !INTER && c * 8 >= half;             // halves: the lane holds the second one of its pairs
+    const int partner = sub * LPH + (turns ? (second ? c - half / 8 : c + half / 8) : c);
     const int64_t pos = p.positions[t];
-    ok = pos >= 0 && pos < p.max_pos;
+    const bool ok = pos >= 0 && pos < p.max_pos;
     if (!ok && lane == 0) report(p.dev_status, kDevBadPosition, t);
+    float cs[8], sn[8];                                      // of the lane's eight channels, the sine with the sign that the channel's product has
     if (turns && ok) {
       const float* tab = p.cos_sin + pos * p.rot + (INTER ? c * 4 : (second ? c * 8 - half : c * 8));
-      if constexpr (INTER) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(tab)), b = __ldg(reinterpret_cast<const float4*>(tab + half));
-        cs[0] = make_float2(a.x, a.x); cs[1] = make_float2(a.y, a.y); cs[2] = make_float2(a.z, a.z); cs[3] = make_float2(a.w, a.w);
-        sn[0] = make_float2(-b.x, b.x); sn[1] = make_float2(-b.y, b.y); sn[2] = make_float2(-b.z, b.z); sn[3] = make_float2(-b.w, b.w);
-      } else {
-        const float sign = second ? 1.f : -1.f;              // (a sign changes no rounding)
+      const float sign = second ? 1.f : -1.f;                // (a sign changes no rounding)
 #pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-          const float4 a = __ldg(reinterpret_cast<const float4*>(tab + 2 * e)), b = __ldg(reinterpret_cast<const float4*>(tab + half + 2 * e));
-          cs[e] = make_float2(a.x, a.y); cs[e + 1] = make_float2(a.z, a.w);
-          sn[e] = make_float2(sign * b.x, sign * b.y); sn[e + 1] = make_float2(sign * b.z, sign * b.w);
+      for (int e = 0; e < (INTER ? 4 : 8); e += 4) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(tab + e)), b = __ldg(reinterpret_cast<const float4*>(tab + half + e));
+        const float ca[4] = {a.x, a.y, a.z, a.w}, sa[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if constexpr (INTER) {
+            cs[2 * k] = cs[2 * k + 1] = ca[k];
+            sn[2 * k] = -sa[k]; sn[2 * k + 1] = sa[k];
+          } else {
+            cs[e + k] = ca[k];
+            sn[e + k] = sign * sa[k];
+          }
         }
       }
     }
-  }
-  int64_t slot = p.slots != nullptr ? p.slots[t] : -1;
-  if (slot < -1 || slot >= p.num_slots) {
-    if (lane == 0) report(p.dev_status, kDevBadSlot, t);
-    slot = -1;
-  }
-  const int64_t block = slot >= 0 ? p.by_block.div(static_cast<uint32_t>(slot)) : 0;
-  const int in_block = slot >= 0 ? static_cast<int>(slot - block * p.block_size) : 0;
-
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
-    const int row = row0 + i * RPW;
-    const bool is_q = row < p.hq, is_v = row >= p.hq + p.hkv;
-    float2 y[4];
-    {
-      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-      uint32_t o[4] = {0, 0, 0, 0};
+    for (int i = 0; i < ITEMS; ++i) {
+      uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w}, o[4] = {0, 0, 0, 0};
       if constexpr (!INTER) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = __shfl_sync(FULL, w[e], partner);
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = make_float2(bf16_lo(w[e]), bf16_hi(w[e]));
-      if (turns && ok && !is_v) {
-        // own cos +- other sin: two products and a sum, each rounded by itself (the paired instructions get fused)
-        uint32_t r[4];
+      if (turns && ok) {
+        // own cos +- other sin: two products and a sum, each rounded by itself (the paired instructions would be fused)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float2 other = INTER ? make_float2(y[e].y, y[e].x) : make_float2(bf16_lo(o[e]), bf16_hi(o[e]));
-          r[e] = pack_bf16(__fadd_rn(__fmul_rn(y[e].x, cs[e].x), __fmul_rn(other.x, sn[e].x)),
-                           __fadd_rn(__fmul_rn(y[e].y, cs[e].y), __fmul_rn(other.y, sn[e].y)));
+          const float a = bf16_lo(w[e]), b = bf16_hi(w[e]), other_a = INTER ? b : bf16_lo(o[e]), other_b = INTER ? a : bf16_hi(o[e]);
+          w[e] = pack_bf16(__fadd_rn(__fmul_rn(a, cs[2 * e]), __fmul_rn(other_a, sn[2 * e])),
+                           __fadd_rn(__fmul_rn(b, cs[2 * e + 1]), __fmul_rn(other_b, sn[2 * e + 1])));
         }
-        x[i] = make_uint4(r[0], r[1], r[2], r[3]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = make_float2(bf16_lo(r[e]), bf16_hi(r[e]));
+        x[i] = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
-    if (row < rows && is_q) *reinterpret_cast<uint4*>(p.q_out + static_cast<int64_t>(t) * p.qo_stride + static_cast<int64_t>(row) * D + c * 8) = x[i];
-    if (row < rows && !is_q && !is_v && p.k_in_place && turns && ok)
-      *reinterpret_cast<uint4*>(p.k + static_cast<int64_t>(t) * p.k_stride + static_cast<int64_t>(row - p.hq) * D + c * 8) = x[i];
-    if (slot < 0 || __all_sync(FULL, is_q || row >= rows)) continue;      // warp-uniform
+    if (!is_q && p.k_in_place && turns && ok) {
+      __nv_bfloat16* dst = p.k + static_cast<int64_t>(t) * p.k_stride + static_cast<int64_t>(head0) * D + c * 8;
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i)
+        if (head0 + i * RPW < heads) *reinterpret_cast<uint4*>(dst + i * RPW * D) = x[i];
+    }
+  }
+  if (is_q) {
+    __nv_bfloat16* dst = p.q_out + static_cast<int64_t>(t) * p.qo_stride + static_cast<int64_t>(head0) * D + c * 8;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+      if (head0 + i * RPW < heads) *reinterpret_cast<uint4*>(dst + i * RPW * D) = x[i];
+    return;
+  }
+  if (slot < 0) return;                                      // warp-uniform
+  const int64_t block = p.by_block.div(static_cast<uint32_t>(slot));
+  const int64_t at = kv4_row(block, p.hkv, head0, p.block_size, static_cast<int>(slot - block * p.block_size));
+  uint32_t* codes = reinterpret_cast<uint32_t*>(is_v ? p.v_codes : p.k_codes) + at * (D / 8) + kv4_word<D>(c, !is_v);
+  uint32_t* affine = (is_v ? p.v_affine : p.k_affine) + at * (D / 64) + (c >> 3);
+  const int64_t code_step = static_cast<int64_t>(RPW) * p.block_size * (D / 8), affine_step = static_cast<int64_t>(RPW) * p.block_size * (D / 64);
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
     // the group's least and greatest value, as the pair (least, -greatest): one minimum for both; every lane of the warp takes part
     const uint32_t least2 = min_bf16x2(min_bf16x2(x[i].x, x[i].y), min_bf16x2(x[i].z, x[i].w));
     const uint32_t most2 = max_bf16x2(max_bf16x2(x[i].x, x[i].y), max_bf16x2(x[i].z, x[i].w));
@@ -155,11 +166,11 @@ __global__ void __launch_bounds__(256, ITEMS == 4 ? 4 : 1) kv4_write_kernel(cons
 #pragma unroll
     for (int off = 1; off < 8; off <<= 1) pair = min_bf16x2(pair, __shfl_xor_sync(FULL, pair, off));
     const float lo = bf16_lo(pair), hi = -bf16_hi(pair);
-    if (row >= rows || is_q) continue;
     const float scale = __bfloat162float(__float2bfloat16_rn(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f)));
+    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
     float2 d[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) d[e] = add_f32x2(y[e], make_float2(-lo, -lo));
+    for (int e = 0; e < 4; ++e) d[e] = add_f32x2(make_float2(bf16_lo(w[e]), bf16_hi(w[e])), make_float2(-lo, -lo));
     uint32_t word = 0;
     if (scale > 0x1p-100f && scale < 0x1p100f) {             // the usual case: the reciprocal is a normal number, no code passes 15
       word = kv4_codes(d, scale, fast_rcp(scale));
@@ -170,11 +181,10 @@ __global__ void __launch_bounds__(256, ITEMS == 4 ? 4 : 1) kv4_write_kernel(cons
         word |= (static_cast<uint32_t>(fminf(rintf(__fdiv_rn(d[e].y, scale)), 15.f)) & 15u) << kv4_shift(2 * e + 1);
       }
     }
-    const int h = row - p.hq - (is_v ? p.hkv : 0);
-    const int64_t at = kv4_row(block, p.hkv, h, p.block_size, in_block);
-    uint32_t* codes = reinterpret_cast<uint32_t*>((is_v ? p.v_codes : p.k_codes) + at * (D / 2));
-    codes[kv4_word<D>(c, !is_v)] = word;
-    if ((c & 7) == 0) (is_v ? p.v_affine : p.k_affine)[at * (D / 64) + (c >> 3)] = pack_bf16(scale, lo);
+    if (head0 + i * RPW < heads) {
+      codes[i * code_step] = word;
+      if ((c & 7) == 0) affine[i * affine_step] = pack_bf16(scale, lo);
+    }
   }
 }
 
@@ -274,12 +284,13 @@ extern "C" int mvb_rotary_kv4_write(const void* q, int64_t q_row_stride, void* q
   return by_head_dim(d, [&](auto tag) -> int {
     constexpr int D = decltype(tag)::value;
     constexpr int RPW = 32 / (D / 8);
-    const int64_t groups = (static_cast<int64_t>(p.hq) + 2 * p.hkv + RPW - 1) / RPW;
+    auto warps_of = [&](int heads, int items) -> int { return (heads + RPW * items - 1) / (RPW * items); };
     // four rows in flight per lane once that still leaves every SM its 32 warps
-    const int items = num_tokens * ((groups + 3) / 4) >= static_cast<int64_t>(sm_count()) * 32 ? 4 : 1;
-    const int64_t per_token = (groups + items - 1) / items, warps = per_token * num_tokens;
-    if (warps > 0x7fffffffLL - 8) return kUnsupportedShape;
+    const int items = static_cast<int64_t>(num_tokens) * (warps_of(p.hq, 4) + 2 * warps_of(p.hkv, 4)) >= static_cast<int64_t>(sm_count()) * 32 ? 4 : 1;
     Kv4WriteParams r = p;
+    r.q_warps = warps_of(p.hq, items); r.k_warps = warps_of(p.hkv, items);
+    const int64_t per_token = r.q_warps + 2 * static_cast<int64_t>(r.k_warps), warps = per_token * num_tokens;
+    if (warps > 0x7fffffffLL - 8) return kUnsupportedShape;
     r.by_token = FastDiv(static_cast<uint32_t>(per_token));
     const unsigned grid = static_cast<unsigned>((warps + 7) / 8);
     if (items == 4 && interleaved) kv4_write_kernel<D, true, 4><<<grid, 256, 0, st>>>(r);
