@@ -236,13 +236,19 @@ __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(const Select
     const int s = threadIdx.x;
     const bool ends = s == 0 || s == count - 1;
     int better = s < count ? 0 : count;
-    if (s < count && !ends) {
-      const uint64_t mine = keys[s];
+    if (warp * 32 < count) {
+      const uint64_t own = s < count ? keys[s] : 0;
+      // spans before the warp's own count from equality on, those behind it above, and inside it depends on the lane
+      const int first = max(1, warp * 32), last = min(count - 1, warp * 32 + 32);
+#pragma unroll 8
+      for (int o = 1; o < first; ++o) better += keys[o] >= own;
 #pragma unroll 4
-      for (int o = 1; o < count - 1; ++o) {
+      for (int o = first; o < last; ++o) {
         const uint64_t k = keys[o];
-        better += k > mine || (k == mine && o < s);
+        better += k > own || (k == own && o < s);
       }
+#pragma unroll 8
+      for (int o = last; o < count - 1; ++o) better += keys[o] > own;
     }
     const bool take = ends || better < p.budget - 2;
     int total;
