@@ -21,8 +21,8 @@
 // warps a contiguous part of that.  A warp streams its tiles through a private ring in shared memory (cp.async, 16 bytes a lane, placed so
 // that the fragment loads meet no bank twice) and needs no other warp until its range is done.  Rows that lie within one warp's range go
 // straight to the output; parts of a row are put together by the CTA, and where a row crosses CTAs by the warps that arrive last.  Every
-// CTA works the split out for itself from the lengths (a scan in shared memory), so there is no plan to make, the grid does not depend on
-// data, and nothing ever waits for another CTA.
+// warp works the split out for itself from the lengths, so there is no plan to make, the grid does not depend on data, and nothing ever
+// waits for another CTA.
 #include "dtype.cuh"
 #include "host_util.cuh"
 #include "kv4.cuh"
@@ -38,17 +38,19 @@ template <int D>
 struct Decode4Cfg {
   static constexpr int TOK = 32;                             // tokens of a tile
   static constexpr int NW = D == 256 ? 8 : 16;               // warps of a CTA
-  static constexpr int NST = 3;                              // tiles in a warp's ring
+  static constexpr int NST = 2;                              // tiles in a warp's ring (three: 113 us instead of 111 for the ragged batch)
   static constexpr int CODES = TOK * D / 2, AFF = TOK * D / 16;
   static constexpr int STAGE = 2 * CODES + 2 * AFF;          // key codes, value codes, key affine, value affine
   static constexpr int RING = NST * STAGE;
   static constexpr int GRP = D / 64;                         // groups of channels
   static constexpr int WK = D / 32, WV = D / 64;             // 32-bit words of a lane: of a key, of a value
-  static constexpr size_t SMEM = static_cast<size_t>(NW) * RING;
+  static constexpr int PART = 8 * D * 4;                     // a part of a row: outputs of up to eight heads
+  static constexpr size_t SMEM = static_cast<size_t>(NW) * (RING + PART);
+  static_assert(PART <= RING, "a warp's last part takes the place of its ring");
 };
 
-// floats of a part: outputs of the group's heads, then their log2-sum-exps (where a CTA leaves a part for others, one copy for each warp
-// that merges a share of the channels)
+// floats of a part that a CTA leaves for others: outputs of the group's heads, then their log2-sum-exps, one copy for each warp that merges
+// a share of the channels
 __host__ __device__ __forceinline__ constexpr int decode4_part(int group, int d) {
   return group * d + kDecode4MaxGroup * (d == 256 ? Decode4Cfg<256>::NW : Decode4Cfg<128>::NW);
 }
@@ -65,7 +67,7 @@ struct Decode4Params {
   FastDiv by_block;
   int table_width, max_len, num_seqs, hkv, group, block_size, budget, window_left;
   float scale_log2, cap_in, cap_log2, out_scale;
-  float* parts;                        // [CTAs][NW + 2] parts: a warp's first row, then the CTA's first and last
+  float* parts;                        // [CTAs][2]: of the CTA's first row and of its last
   int32_t* arrivals;                   // [num_seqs * hkv][NW], zero between launches
   int* dev_status;
 };
@@ -226,7 +228,8 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
   }
   // Few rows: whole CTAs for each of them, in proportion to its tiles but one for a row of up to three tiles a warp, so that a CTA works on one
   // row and most need no other CTA.  Where some CTA would get much more than its share, or there are more rows than CTAs: the even cut.
-  // (8 rows of 22 tiles: 15.4 us cut evenly, XX by rows; 128 rows of up to 17 tiles of 256-wide heads: 18.9 and XX; 8 rows of 1280: 30.5 and XX.)
+  // (8 rows of 22 tiles: 15.4 us cut evenly, 11.5 by rows; 128 rows of up to 17 tiles of 256-wide heads: 18.9 and 13.6; 8 rows of 1280: 30.5
+  // and 26.4.)
   const int grid = gridDim.x, share = (total + grid - 1) / grid;
   const float part_of_grid = static_cast<float>(grid) / static_cast<float>(max(total, 1));
   auto ctas_of = [&](int v) -> int {                         // (a tile a warp at least: no CTA is left without one)
@@ -532,7 +535,7 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          x[s][i] *= (i & 1) ? f_b : f_a;
+          x[s][i] *= (i & 1) ? f_b : f_a;                    // (rounded here: the weights' differences have to be those of one set of scores)
           if constexpr (CAP) x[s][i] = fmaf(-2.f * p.cap_log2, fast_rcp(1.f + fast_exp2(x[s][i] * p.cap_in)), p.cap_log2);
         }
         if (!whole) {                                        // tokens out of sight: no weight, whatever their rows hold
@@ -632,13 +635,13 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
     const bool complete = row_t0 >= w0 && row_t1 <= w1;
     float* part = nullptr;
     if (!complete) {
-      // the warp's last part can take the place of its ring, an earlier one (its first row's end) goes to the workspace
+      // the warp's last part can take the place of its ring, an earlier one (its first row's end) has a place of its own
       if (seg_end == w1) {
         cp_async_wait<0>();
         __syncwarp();
         part = reinterpret_cast<float*>(smem + warp * C::RING);
       } else {
-        part = p.parts + (static_cast<int64_t>(cta) * (NW + 2) + warp) * decode4_part(G, D);
+        part = reinterpret_cast<float*>(smem + NW * C::RING + warp * C::PART);
       }
       if (lane == 0) {
         const int slot = seg_end == w1 ? 1 : 0;
@@ -672,15 +675,6 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
     row_t0 = row_t1;
   }
   cp_async_wait<0>();
-  __syncwarp();
-  // a first part comes back to the ring's second place, so that what follows reads shared memory alone
-  constexpr int SECOND = kDecode4MaxGroup * D * 4;
-  static_assert(2 * SECOND <= C::RING, "two parts have to fit into a ring");
-  if (meta_s[warp][0][0] >= 0) {
-    const float* from = p.parts + (static_cast<int64_t>(cta) * (NW + 2) + warp) * decode4_part(G, D);
-    for (int e = lane; e < G * D / 4; e += 32)
-      *reinterpret_cast<float4*>(smem + warp * C::RING + SECOND + e * 16) = *reinterpret_cast<const float4*>(from + e * 4);
-  }
   __syncthreads();
 
   // ---- parts of rows, put together --------------------------------------------------------------------------------------------------
@@ -706,7 +700,7 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
     const float r = M == -INFINITY ? 0.f : M;
     float sum = fast_exp2(xf - r);
     if (wf >= 0) {
-      const float4 y = *reinterpret_cast<const float4*>(smem + wf * C::RING + SECOND + e * 16);
+      const float4 y = *reinterpret_cast<const float4*>(smem + NW * C::RING + wf * C::PART + e * 16);
       acc.x = sum * y.x; acc.y = sum * y.y; acc.z = sum * y.z; acc.w = sum * y.w;
     }
     for (int w0 = lo; w0 <= hi; w0 += 4) {
@@ -760,7 +754,7 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
     } else if (lane == job - 2) {
       mine_row = row; mine_first = r0; mine_last = r1;
     }
-    float* to = p.parts + (static_cast<int64_t>(cta) * (NW + 2) + NW + (r0 <= t0 ? 0 : 1)) * decode4_part(G, D);
+    float* to = p.parts + (static_cast<int64_t>(cta) * 2 + (r0 <= t0 ? 0 : 1)) * decode4_part(G, D);
     for (; at < end; at += 32) {
       const int e = job < 2 ? at : piece(at);
       float lse;
@@ -798,8 +792,8 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
     const int from_cta = __shfl_sync(FULL, c1, i), row = __shfl_sync(FULL, mine_row, i), r0 = __shfl_sync(FULL, mine_first, i);
     // a lane takes a piece, or the piece of every n-th part where a warp's share leaves lanes over
     const int lanes = min(owned, 32), split = 32 / lanes, mine = lane / lanes, first = lane - mine * lanes;
-    const float* head_part = p.parts + (static_cast<int64_t>(from_cta) * (NW + 2) + NW) * decode4_part(G, D);
-    const int64_t stride = static_cast<int64_t>(NW + 2) * decode4_part(G, D);
+    const float* head_part = p.parts + static_cast<int64_t>(from_cta) * 2 * decode4_part(G, D);
+    const int64_t stride = 2 * decode4_part(G, D);
     const int late = mine_s.first >= 0 || r0 <= cut.start(from_cta) ? 0 : decode4_part(G, D);          // the first CTA's part, where the row began inside it
     for (int base = 0; base < owned; base += 32) {
       const int e = piece(base + first);
@@ -850,12 +844,8 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
 
 // The parts have the room that the largest head shape needs, so that the counters lie at the same place for every shape and batch: one
 // workspace may serve different calls one after the other and the counters are zero between them.
-constexpr size_t decode4_parts_bytes(int d, int nw) {
-  return sizeof(float) * kDecode4MaxCtas * (nw + 2) * decode4_part(kDecode4MaxGroup, d);
-}
-constexpr size_t kDecode4Parts = decode4_parts_bytes(256, Decode4Cfg<256>::NW) > decode4_parts_bytes(128, Decode4Cfg<128>::NW)
-                                     ? decode4_parts_bytes(256, Decode4Cfg<256>::NW) : decode4_parts_bytes(128, Decode4Cfg<128>::NW);
-static_assert(kDecode4Parts % 256 == 0, "");
+constexpr size_t kDecode4Parts = sizeof(float) * kDecode4MaxCtas * 2 * decode4_part(kDecode4MaxGroup, 256);
+static_assert(kDecode4Parts % 256 == 0 && decode4_part(kDecode4MaxGroup, 256) >= decode4_part(kDecode4MaxGroup, 128), "");
 
 static size_t decode4_bytes(int64_t seqs, int hkv) {
   return kDecode4Parts + (sizeof(int32_t) * static_cast<size_t>(seqs) * hkv * Decode4Cfg<128>::NW + 255) / 256 * 256;
