@@ -11,6 +11,7 @@ Gemma3, ``query_pre_attn_scalar``, ``sliding_window``, ``rope_local_base_freq``)
 """
 from __future__ import annotations
 
+import logging
 import os
 from dataclasses import dataclass
 from types import SimpleNamespace
@@ -19,6 +20,8 @@ from typing import Any, Optional, Set
 import torch
 
 from .native import read_native
+
+log = logging.getLogger(__name__)
 
 
 @dataclass
@@ -99,8 +102,14 @@ def _flatten_hf(cfg) -> SimpleNamespace:
     out = SimpleNamespace(**{n: getattr(cfg, n) for n in names if hasattr(cfg, n)})
     rp = getattr(cfg, "rope_parameters", None)
     scaling = getattr(cfg, "rope_scaling", None) or (rp.get("full_attention", rp) if isinstance(rp, dict) else None)
-    if isinstance(scaling, dict) and scaling.get("rope_type", scaling.get("type", "default")) != "default":
-        out.rope_scaling = dict(scaling)
+    if isinstance(scaling, dict):
+        kind = scaling.get("rope_type", scaling.get("type", "default"))
+        if kind in ("linear", "yarn", "llama3"):
+            out.rope_scaling = dict(scaling)
+            if out.rope_scaling.get("original_max_position_embeddings") is None:
+                out.rope_scaling["original_max_position_embeddings"] = getattr(out, "max_position_embeddings", None)
+        elif kind != "default":
+            log.warning("rope scaling of type %r is not known and left out", kind)
     if isinstance(rp, dict):
         if "rope_theta" in rp and not hasattr(out, "rope_theta"):
             out.rope_theta = rp["rope_theta"]

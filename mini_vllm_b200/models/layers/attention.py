@@ -119,6 +119,8 @@ class FlashAttention(nn.Module):
                 self.source is None and not self.lends and self._extras(None) is None)
 
     def _write_kv4(self, ctx: Context, q, k, v, positions, cos_sin) -> None:
+        if self._extras(None) is not None or self.lends:
+            raise ValueError("a cache in 4 bits goes with plain attention: no sinks, biases, kept tokens or lent keys")
         if ctx.prefill and ctx.block_table is None:
             raise ValueError("a cache in 4 bits needs the step's block table: prompts read their keys and values back from it")
         ops.rotary_kv4_write(q, k, v, positions, cos_sin, ctx.slot_mapping, self.kv4, status=ctx.status)

@@ -1459,7 +1459,7 @@ def decode_attn4(q: torch.Tensor, cache: KV4Cache, cache_seqlens: torch.Tensor, 
         spans_ptr = _dense(spans, i32, device, (B, hkv, budget), "spans")
     ws_ptr = _numbers(workspace, torch.uint8, device, 0, _BIG, "workspace")
     rc = _cabi.load().mvb_decode_attn4(q.data_ptr(), q_stride, cache.struct(device), lens_ptr, table_ptr, stride, width, spans_ptr, budget, B, hq,
-                                       scale, window_left, softcap, out_scale, out.data_ptr(), out_stride, ws_ptr, workspace.numel(),
+                                       float(scale), window_left, float(softcap), float(out_scale), out.data_ptr(), out_stride, ws_ptr, workspace.numel(),
                                        _status(status, device), _stream())
     if rc:
         _cabi.check(rc, "mvb_decode_attn4")

@@ -66,7 +66,11 @@ def test_scaling_comes_out_of_a_hugging_face_config():
     assert not hasattr(_flatten_hf(cfg), "rope_scaling")
     cfg.rope_parameters = {**YARN, "rope_theta": 1e6}
     flat = _flatten_hf(cfg)
-    assert flat.rope_scaling["factor"] == 4.0 and flat.rope_theta == 1e6
+    assert flat.rope_scaling["factor"] == 4.0 and flat.rope_theta == 1e6 and flat.rope_scaling["original_max_position_embeddings"] == 8192
+    cfg.rope_parameters = {"rope_type": "yarn", "factor": 2.0, "rope_theta": 1e6}
+    assert _flatten_hf(cfg).rope_scaling["original_max_position_embeddings"] == cfg.max_position_embeddings
+    cfg.rope_parameters = {"rope_type": "dynamic", "factor": 2.0, "rope_theta": 1e6}
+    assert not hasattr(_flatten_hf(cfg), "rope_scaling")            # (left out, as it always was)
 
 
 # ---- configuration and handle ---------------------------------------------------------------------------------------------------------
@@ -101,6 +105,24 @@ def test_layout_is_a_permutation_and_values_come_back(d, keys):
     spread = g.amax(-1, keepdim=True) - g.amin(-1, keepdim=True)
     # half a code, and the scale's own rounding over 15 codes
     assert ((g - z).abs() <= spread / 15 * (0.5 + 16 * 2.0 ** -8)).all()
+
+
+def test_layer_refuses_what_four_bits_do_not_serve():
+    from mini_vllm_b200.executor.context import Context
+    from mini_vllm_b200.models.layers.attention import FlashAttention
+    layer = FlashAttention(4, 128, 1.0, 2)
+    assert layer.takes_kv4(torch.bfloat16) and not layer.takes_kv4(torch.float32)
+    assert not FlashAttention(4, 64, 1.0, 2).takes_kv4(torch.bfloat16) and not FlashAttention(18, 128, 1.0, 2).takes_kv4(torch.bfloat16)
+    layer.kv4 = ops.KV4Cache.empty(1, 128, 2, 128, "cpu")
+    x = torch.zeros(3, 2, 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="block table"):
+        layer(Context(prefill=True), x, x, x)
+    with pytest.raises(ValueError, match="no norms"):
+        layer.forward_fused(Context(prefill=True), x, x, x, torch.zeros(3, dtype=torch.int64), None, norm=(128, 1e-6))
+    layer.sinks = torch.zeros(4)
+    assert not layer.takes_kv4(torch.bfloat16)
+    with pytest.raises(ValueError, match="no sinks"):
+        layer(Context(prefill=False), x, x, x)
 
 
 # ---- refusals at the C entries (nothing is launched: no address is followed) ---------------------------------------------------------------
