@@ -670,7 +670,7 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
         if (complete) store_vec<__nv_bfloat16, 8>(p.out + b * p.out_stride + (static_cast<int64_t>(h) * G + head) * D + 64 * j + 8 * g, y);
         else store_f32<8>(part + head * D + 64 * j + 8 * g, y);
       }
-      if (!complete && g == 0) lse_s[seg_end == w1 ? 1 : 0][head][warp] = l > 0.f ? m + fast_log2(l) : -INFINITY;
+      if (!complete && g == 0) lse_s[seg_end == w1 ? 1 : 0][head][warp] = l == 0.f ? -INFINITY : m + fast_log2(l);    // (NaN stays NaN)
     }
     row_t0 = row_t1;
   }
@@ -716,7 +716,7 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
     }
     const float inv = sum > 0.f ? 1.f / sum : 0.f;
     acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
-    lse = sum > 0.f ? M + fast_log2(sum) : -INFINITY;
+    lse = sum == 0.f ? -INFINITY : M + fast_log2(sum);
     return acc;
   };
   auto put = [&](int row, int e, const float4& y, float f) {

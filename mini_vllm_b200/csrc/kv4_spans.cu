@@ -149,8 +149,8 @@ __device__ __forceinline__ int block_prefix(int v, int* scratch, int& total) {
 // A cluster of CL blocks per (KV head, sequence).  Its blocks share the spans and send their sums' bits, as keys that ascend with the sum, to the
 // first one, which finds the budget-th greatest by radix selection, eight bits at a time from the first one in which keys differ, and
 // writes the chosen indices in order (of equal sums the lower ones).  Eight lanes take a span, so that a warp has four spans in flight.
-// 4 sequences of 9000-40000 tokens, 8 KV heads: 67 us with one block and one span a warp, 11.4 with eight blocks and
-// eight spans a warp.
+// Bound by latency for few rows (4 sequences of 9000-40000 tokens, 8 KV heads: 11 us, 67 with one block and one span a warp), by the fp64 sums
+// for many.
 template <int D>
 __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(const SelectParams p) {
   constexpr uint32_t FULL = 0xffffffffu;
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(const Select
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane & 7;
   const int n = p.seqlens[b];
   int32_t* out = p.out + (static_cast<int64_t>(b) * p.hkv + h) * p.budget;
-  int count = n > 0 ? (n + kKv4Span - 1) / kKv4Span : 0;
+  int count = n > 0 ? (n - 1) / kKv4Span + 1 : 0;
   const int per_block = p.block_size / kKv4Span;
   if (count > p.max_spans) {                                 // longer than the caller said, or than its block list holds
     if (threadIdx.x == 0) report(p.dev_status, kDevBadLength, b);
@@ -233,7 +233,10 @@ __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(const Select
     __syncthreads();
   }
   // ---- the first block: which of the inner spans -------------------------------------------------------------------------------------
-  if (count <= kSelectThreads) {                             // a thread has a span and counts the better ones: no passes, one prefix sum
+  // Up to 256 spans a thread has one and counts the better ones: no passes, one prefix sum.  That takes every warp the whole list, so blocks
+  // that share an SM with others do it up to 128 (8 pairs of 250 spans: 8.6 us against 10.1 by radix; 768 pairs of 90 spans 23.3 and 24.5, of
+  // 250 54.9 and 51.0)
+  if (count <= (cl > 1 ? kSelectThreads : kSelectThreads / 2)) {
     const int s = threadIdx.x;
     const bool ends = s == 0 || s == count - 1;
     int better = s < count ? 0 : count;
@@ -333,8 +336,9 @@ extern "C" int mvb_kv4_summarise(const mvb_kv4_cache* cache, const int32_t* slot
   p.num_slots = cache->num_blocks * cache->block_size;
   p.tokens = num_tokens; p.hkv = cache->num_kv_heads; p.block_size = cache->block_size; p.dev_status = dev_status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // a block for each (token, head) up to a few per SM's place for them; more are mostly prompts
-  const bool few = static_cast<int64_t>(num_tokens) * cache->num_kv_heads <= 4096;
+  // a block for each (token, head) of a step of few, a warp for each of many (decoding, 8 heads of 128, eight warps and one: 32 sequences 2.9
+  // and 5.1 us, 128 5.5 and 5.3, 1024 27 and 18; prompts: 64 tokens 2.5 and 4.5, 512 4.6 and 4.5, 8192 39 and 15)
+  const bool few = static_cast<int64_t>(num_tokens) * cache->num_kv_heads <= 1024;
   const dim3 grid(few ? num_tokens : (static_cast<unsigned>(num_tokens) + 7) / 8, cache->num_kv_heads);
   auto launch = [&](auto tag) -> int {
     constexpr int D = decltype(tag)::value;
@@ -372,9 +376,12 @@ extern "C" int mvb_kv4_select(const void* q, int64_t q_row_stride, const void* s
   p.dev_status = dev_status;
   const size_t smem = sizeof(uint64_t) * static_cast<size_t>(spans_most);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // blocks enough for every SM to have two, a cluster of at most eight for one (sequence, head)
+  // a cluster of at most eight blocks for one (sequence, head): up to 5/3 blocks per SM, and 44 spans of the longest context for each.  128-wide
+  // heads, clusters of 1, 2, 4, 8: 32 pairs of 16 K tokens 16.7, 11.5, 8.6, 10.6 us, of 40 K 34.6, 22.2, 16.4, 14.8; 72 of 40 K 35.1, 22.5, 21.4,
+  // 22.7; 128 of 16 K 17.0, 14.6, 16.6, 25.2; 256 of 16 K 22.0, 26.4, 27.6, 43.4
+  const int64_t pairs = static_cast<int64_t>(num_kv_heads) * num_seqs;
   int cl = 1;
-  while (cl < 8 && static_cast<int64_t>(num_kv_heads) * num_seqs * cl < 2 * sm_count()) cl *= 2;
+  while (cl < 8 && pairs * cl * 3 < 5 * sm_count() && spans_most >= 88 * cl) cl *= 2;
   auto launch = [&](auto tag) -> int {
     constexpr int D = decltype(tag)::value;
     struct Tag {};

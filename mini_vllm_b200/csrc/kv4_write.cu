@@ -211,8 +211,8 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(const Kv4GatherParams p
   if (static_cast<int>(t) >= total) return;                  // rows behind the last sequence are left as they are
   const int b = seq_of_row(p.cu, p.num_seqs, t);
   const int token = static_cast<int>(t) - p.cu[b];
-  const int col = p.by_block.div(token);
-  const int64_t block = col < p.table_width ? p.block_table[b * p.table_stride + col] : -1;
+  const int col = p.by_block.div(max(token, 0));             // (negative: a list of lengths that does not begin at 0)
+  const int64_t block = token >= 0 && col < p.table_width ? p.block_table[b * p.table_stride + col] : -1;
   const bool ok = block >= 0 && block < p.num_blocks;
   if (!ok && lane == 0) report(p.dev_status, kDevBadBlock, b);
   const int head0 = static_cast<int>(warp - t * p.by_token.n) * (RPW * ITEMS) + sub;
@@ -285,8 +285,9 @@ extern "C" int mvb_rotary_kv4_write(const void* q, int64_t q_row_stride, void* q
     constexpr int D = decltype(tag)::value;
     constexpr int RPW = 32 / (D / 8);
     auto warps_of = [&](int heads, int items) -> int { return (heads + RPW * items - 1) / (RPW * items); };
-    // four rows in flight per lane once that still leaves every SM its 32 warps
-    const int items = static_cast<int64_t>(num_tokens) * (warps_of(p.hq, 4) + 2 * warps_of(p.hkv, 4)) >= static_cast<int64_t>(sm_count()) * 32 ? 4 : 1;
+    // four rows in flight per lane where that still leaves every SM 12 warps, one where there are few tokens (8 KV heads of 128, one and four
+    // rows: 96 tokens 2.5 and 3.1 us; 512 tokens with 32 heads of queries 5.4 and 4.4, with 16 4.4 and 3.8; 16384 with 32 131 and 87)
+    const int items = static_cast<int64_t>(num_tokens) * (warps_of(p.hq, 4) + 2 * warps_of(p.hkv, 4)) >= static_cast<int64_t>(sm_count()) * 12 ? 4 : 1;
     Kv4WriteParams r = p;
     r.q_warps = warps_of(p.hq, items); r.k_warps = warps_of(p.hkv, items);
     const int64_t per_token = r.q_warps + 2 * static_cast<int64_t>(r.k_warps), warps = per_token * num_tokens;

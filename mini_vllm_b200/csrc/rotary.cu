@@ -124,8 +124,10 @@ static int launch_rotary(RotaryParams& p, bool inter, cudaStream_t stream) {
   p.rot_units = vec && inter ? p.rot / V : p.rot / 2 / v;
   p.units = p.rot_units + (in_place ? 0 : (p.d - p.rot) / v);
   const int heads = p.hq + p.hkv;
-  // four heads a thread where that still leaves every SM its 2048 threads, one where there are few tokens
-  const bool many = vec && static_cast<int64_t>((heads + 3) / 4) * p.units * p.tokens >= static_cast<int64_t>(sm_count()) * 2048;
+  // four heads a thread where that still leaves every SM 512 threads, one where there are few tokens (32 + 8 heads of 128, whole heads turned
+  // by neighbours, one and four heads: 96 tokens 2.0 and 2.4 us, 512 3.6 and 3.4, 1024 5.7 and 4.9, 16384 73 and 55; by halves 2.1 and 2.8, 3.2
+  // and 3.4, 5.1 and 4.8, 66 and 58)
+  const bool many = vec && static_cast<int64_t>((heads + 3) / 4) * p.units * p.tokens >= static_cast<int64_t>(sm_count()) * 512;
   const int64_t per_token = static_cast<int64_t>(many ? (heads + 3) / 4 : heads) * p.units;
   if (per_token > 0x7fffffffLL / (p.tokens > 0 ? p.tokens : 1)) return kUnsupportedShape;
   p.total = per_token * p.tokens;

@@ -121,6 +121,10 @@ def test_gather(cuda, d, hkv, size):
     assert status[0].item() == 2 and status[1].item() == 4
     first = int(cu[4]) + size
     assert (k[first:first + size] == 0).all() and (v[first:first + size] == 0).all()
+    late, status = (cu + 3).to(torch.int32), ops.new_status(cuda)   # lists that do not begin at 0: the rows before them read as zeros
+    k, v = ops.kv4_gather(on(cuda, cache), late.to(cuda), table.to(cuda), total + 3, status=status)
+    assert status[0].item() == 2 and status[1].item() == 0 and (k[:3] == 0).all() and (v[:3] == 0).all()
+    assert torch.equal(k[3:].cpu(), out[0][:total].cpu()) and torch.equal(v[3:].cpu(), out[1][:total].cpu())
 
 
 # ---- attention of single tokens ---------------------------------------------------------------------------------------------------------
@@ -237,6 +241,23 @@ def test_decode_reports_bad_blocks_and_lengths(cuda):
     assert status[0].item() == 5 and status[1].item() == 0
 
 
+@pytest.mark.parametrize("n", [20, 700, 9000])
+def test_decode_a_query_that_is_not_a_number_stays_one_heads_matter(cuda, n):
+    """Within one warp, over the warps of a CTA and over CTAs."""
+    g, hq, hkv, d = gen(n), 4, 2, 128
+    table, blocks = kh.block_lists(g, [n, n], 256)
+    cache = kh.make_cache(g, blocks, hkv, 256, d)
+    q = torch.randn(2, hq, d, generator=g).to(BF)
+    want, big = kh.decode(q, cache, table, [n, n], d ** -0.5)
+    q[1, 2, 77] = float("nan")
+    got = ops.decode_attn4(q.to(cuda), on(cuda, cache), torch.tensor([n, n], dtype=torch.int32, device=cuda), table.to(cuda), d ** -0.5, -1,
+                           ops.decode4_workspace(2, hq, hkv, d, cuda))
+    assert torch.isnan(got[1, 2]).all()
+    others = torch.ones(2, hq, dtype=torch.bool)
+    others[1, 2] = False
+    kh.assert_decode(got.cpu()[others], want[others], big[others], "the other heads")
+
+
 def test_decode_capture_replay_and_two_graphs_of_one_workspace(cuda):
     """Lengths change between replays of a captured step; two graphs take turns on one workspace and another stream."""
     g, hq, hkv, d, most = gen(12), 8, 2, 128, [2000, 700, 90, 300]
@@ -345,6 +366,22 @@ def test_selection(cuda, hq, hkv, d, size, budget):
     assert torch.equal(ops.kv4_select(*one).cpu(), want[7:8])
     ops.kv4_select(*args, max_context=20000, status=status)
     assert status[0].item() == 5 and status[1].item() == 10
+    longest = args[2].clone()
+    longest[10] = 2 ** 31 - 1                                       # longer than its list of blocks holds: cut there
+    status = ops.new_status(cuda)
+    cut = ops.kv4_select(*args[:2], longest, *args[3:], status=status)[10]
+    assert status[0].item() == 5 and status[1].item() == 10 and (cut[:, -1] == table.shape[1] * (size // 64) - 1).all()
+
+
+def test_selection_for_many_sequences(cuda):
+    """More rows than SMs, on both sides of the 128 spans that such rows are ranked up to."""
+    g, hkv, d, size, budget = gen(77), 8, 64, 256, 20
+    lens = [64 * n + i % 3 for i, n in enumerate([1, 20, 21, 126, 127, 128, 129, 200, 255, 256, 257] * 3)]
+    table, blocks = kh.block_lists(g, lens, size)
+    summaries = torch.randn(blocks, hkv, size // 64, 2, d, generator=g).to(BF).sort(3).values
+    q = torch.randn(len(lens), 16, d, generator=g).to(BF)
+    got = ops.kv4_select(q.to(cuda), summaries.to(cuda), torch.tensor(lens, dtype=torch.int32, device=cuda), table.to(cuda), size, budget)
+    assert torch.equal(got.cpu(), kh.select(q, summaries, table, lens, budget))
 
 
 @pytest.mark.parametrize("count", [40, 500])
