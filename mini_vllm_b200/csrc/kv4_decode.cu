@@ -16,13 +16,17 @@
 // token's values), with size = max(scale, 2^-20 |minimum|, 2^-100), which bounds every p s by 2^6 and every p m by 2^26; a minimum that
 // large leaves nothing of its codes in the bf16 output.
 //
-// Bound by memory, on paper 4608 bytes against some 450 warp instructions per 32 tokens of a 128-wide head.  Work is tiles of 32 tokens of
-// one (sequence, head), numbered sequence by sequence and head by head, and cut evenly: each CTA takes a contiguous range, each of its
-// warps a contiguous part of that.  A warp streams its tiles through a private ring in shared memory (cp.async, 16 bytes a lane, placed so
-// that the fragment loads meet no bank twice) and needs no other warp until its range is done.  Rows that lie within one warp's range go
-// straight to the output; parts of a row are put together by the CTA, and where a row crosses CTAs by the warps that arrive last.  Every
-// warp works the split out for itself from the lengths, so there is no plan to make, the grid does not depend on data, and nothing ever
-// waits for another CTA.
+// On paper bound by memory: a tile of 32 tokens of a 128-wide head is 4608 bytes.  Its 675 warp instructions, most of them on the integer
+// pipe, bring instruction issue near: 240 sequences of 128-8192 tokens, 16 heads on 8, 0.51 GB in 111 us, 4.6 TB/s (0.71 of what a copy reaches),
+// 62 % of the issue slots, the integer pipe at 58 %.  A few rows are bound by the chain of dependent loads (lengths, block lists, tiles, parts):
+// one context of 700 tokens 12 us.
+//
+// Work is tiles of 32 tokens of one (sequence, head), numbered sequence by sequence and head by head.  Each CTA takes a contiguous range (all
+// alike, or, where there are few rows, a share of one of them), each of its warps a contiguous part of that.  A warp streams its tiles
+// through a private ring in shared memory (cp.async, 16 bytes a lane, placed so that the fragment loads meet no bank twice) and needs no
+// other warp until its range is done.  Rows that lie within one warp's range go straight to the output; parts of a row are put together by
+// the CTA, and where a row crosses CTAs by the warps that arrive last.  Every warp works the split out for itself from the lengths, so
+// there is no plan to make, the grid does not depend on data, and nothing ever waits for another CTA.
 #include "dtype.cuh"
 #include "host_util.cuh"
 #include "kv4.cuh"
@@ -228,8 +232,8 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
   }
   // Few rows: whole CTAs for each of them, in proportion to its tiles but one for a row of up to three tiles a warp, so that a CTA works on one
   // row and most need no other CTA.  Where some CTA would get much more than its share, or there are more rows than CTAs: the even cut.
-  // (8 rows of 22 tiles: 15.4 us cut evenly, 11.5 by rows; 128 rows of up to 17 tiles of 256-wide heads: 18.9 and 13.6; 8 rows of 1280: 30.5
-  // and 26.4.)
+  // (8 rows of 22 tiles: 15.4 us cut evenly, 11.8 by rows; 128 rows of up to 17 tiles of 256-wide heads: 18.9 and 13.7; 8 rows of 1280: 30.5
+  // and 24.9.)
   const int grid = gridDim.x, share = (total + grid - 1) / grid;
   const float part_of_grid = static_cast<float>(grid) / static_cast<float>(max(total, 1));
   auto ctas_of = [&](int v) -> int {                         // (a tile a warp at least: no CTA is left without one)
