@@ -149,8 +149,8 @@ __device__ __forceinline__ int block_prefix(int v, int* scratch, int& total) {
 // A cluster of CL blocks per (KV head, sequence).  Its blocks share the spans and send their sums' bits, as keys that ascend with the sum, to the
 // first one, which finds the budget-th greatest by radix selection, eight bits at a time from the first one in which keys differ, and
 // writes the chosen indices in order (of equal sums the lower ones).  Eight lanes take a span, so that a warp has four spans in flight.
-// Bound by latency for few rows (4 sequences of 9000-40000 tokens, 8 KV heads: 11 us, 67 with one block and one span a warp), by the fp64 sums
-// for many.
+// Bound by latency: for few rows by the chain of loads, sums and ranking (4 sequences of 9000-40000 tokens, 8 KV heads: 11 us, 67 with one block
+// and one span a warp), for many by the same chain in every block, loads and barriers at 45 % of the issue slots (96 sequences: 26 us).
 template <int D>
 __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(const SelectParams p) {
   constexpr uint32_t FULL = 0xffffffffu;
