@@ -622,7 +622,7 @@ int mvb_row_norm_rope_kv_write(int dtype, void* q, int64_t q_row_stride, void* k
  *   num_kv_heads.  spans (NULL: all tokens): int32 [num_seqs, num_kv_heads, budget], the 64-token spans that a head's queries read, each once;
  *   entries below 0 are skipped (not with a window).  A sequence of no tokens, or none that is read, gives zeros.  workspace of
  *   mvb_decode_attn4_workspace_bytes, 256-byte aligned, zeroed once by the caller and left zeroed where it has to be; calls that share it
- *   must not overlap.
+ *   must not overlap.  out lies apart from q.
  * mvb_kv4_summarise: bounds of the keys of the spans that a step's tokens were written to: summaries bf16 [num_blocks, num_kv_heads,
  *   block_size / 64, 2, head_dim], least and greatest key per channel over the span's rows up to the step's last one.  The tokens of a
  *   sequence stand next to each other, in order.

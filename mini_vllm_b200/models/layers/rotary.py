@@ -24,7 +24,8 @@ def scaled_frequencies(rotary_dim: int, rope_theta: float, scaling: dict) -> tup
     * ``default``: as trained;
     * ``linear``: every position counts as ``1 / factor``;
     * ``yarn``: pairs that turn less than ``beta_slow`` times over ``original_max_position_embeddings`` are slowed by ``factor``, those that turn
-      more than ``beta_fast`` times stay, a ramp over the pairs' numbers between; vectors grow by ``attention_factor`` or ``0.1 ln(factor) + 1``;
+      more than ``beta_fast`` times stay, a ramp over the pairs' numbers between; vectors grow by ``attention_factor``, or by ``g(1)`` with
+      ``g(m) = 0.1 m ln(factor) + 1``, or by ``g(mscale) / g(mscale_all_dim)`` where both are given; ``truncate`` False: the ramp's ends are not rounded;
     * ``llama3``: pairs with wavelengths above ``original / low_freq_factor`` are slowed by ``factor``, those below ``original /
       high_freq_factor`` stay, blended by the wavelength between.
     """
@@ -44,12 +45,15 @@ def scaled_frequencies(rotary_dim: int, rope_theta: float, scaling: dict) -> tup
         keep = ((turns - low) / (high - low)).clamp(0, 1)
         return freq / factor * (1 - keep) + freq * keep, 1.0
     pair = lambda turns: rotary_dim * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(rope_theta))   # the pair that turns so often
-    low = max(math.floor(pair(float(scaling.get("beta_fast") or 32))), 0)
-    high = min(math.ceil(pair(float(scaling.get("beta_slow") or 1))), rotary_dim - 1)
+    whole = scaling.get("truncate", True)                    # the ramp goes from pair to pair
+    low, high = pair(float(scaling.get("beta_fast") or 32)), pair(float(scaling.get("beta_slow") or 1))
+    low, high = max(math.floor(low) if whole else low, 0), min(math.ceil(high) if whole else high, rotary_dim - 1)
     slowed = ((torch.arange(rotary_dim // 2, dtype=torch.double, device="cpu") - low) / max(high - low, 0.001)).clamp(0, 1)
     grow = scaling.get("attention_factor")
     if grow is None:
-        grow = 0.1 * math.log(factor) + 1 if factor > 1 else 1.0
+        growth = lambda m: 0.1 * m * math.log(factor) + 1 if factor > 1 else 1.0
+        m, m_all = scaling.get("mscale"), scaling.get("mscale_all_dim")
+        grow = growth(float(m)) / growth(float(m_all)) if m and m_all else growth(1.0)
     return freq / factor * slowed + freq * (1 - slowed), float(grow)
 
 

@@ -1440,7 +1440,8 @@ def decode_attn4(q: torch.Tensor, cache: KV4Cache, cache_seqlens: torch.Tensor, 
                  workspace: torch.Tensor, spans: torch.Tensor | None = None, out: torch.Tensor | None = None,
                  status: torch.Tensor | None = None, softcap: float = 0.0, out_scale: float = 1.0) -> torch.Tensor:
     """``decode_attn`` over a cache in 4 bits: ``q [B, Hq, D]`` bf16, one new token per sequence.  ``spans`` int32 ``[B, Hkv, budget]``
-    (``kv4_select``): only these spans of 64 tokens are read, each listed once, entries below 0 skipped.  No plan is needed."""
+    (``kv4_select``): only these spans of 64 tokens are read, each listed once, entries below 0 skipped.  No plan is needed.  ``out`` lies
+    apart from ``q``, which several blocks read."""
     device, bf16, i32 = _device() if q.is_cuda else -2, torch.bfloat16, torch.int32
     _, _, hkv, d = cache.sizes
     _need_shape(q.dim() == 3, "q must be [sequences, heads, head_dim]")
@@ -1451,6 +1452,7 @@ def decode_attn4(q: torch.Tensor, cache: KV4Cache, cache_seqlens: torch.Tensor, 
         out_stride = hq * d
     else:
         out_stride = _rows(out, bf16, device, (B, hq, d), "out")
+        _need_shape(out.data_ptr() != q.data_ptr() or B == 0, "out must lie apart from q")
     lens_ptr = _numbers(cache_seqlens, i32, device, B, _BIG, "cache_seqlens")
     table_ptr, stride, width = _table(block_table, device, B)
     spans_ptr, budget = None, 0

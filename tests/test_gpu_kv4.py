@@ -303,7 +303,7 @@ def test_wrappers_refuse(cuda):
         with pytest.raises(TypeError):
             bad()
     for bad in (lambda: dec(q=q[..., :64]), lambda: dec(cache_seqlens=i32[:1]), lambda: dec(block_table=table[:1]), lambda: dec(block_table=table.t()[::2]),
-                lambda: dec(spans=spans[:1]), lambda: dec(out=q[:1]), lambda: wr(k=q), lambda: wr(v=k[:1]), lambda: wr(slot_mapping=i32[:1]),
+                lambda: dec(spans=spans[:1]), lambda: dec(out=q[:1]), lambda: dec(out=q), lambda: wr(k=q), lambda: wr(v=k[:1]), lambda: wr(slot_mapping=i32[:1]),
                 lambda: wr(cos_sin=cs[:, ::2]), lambda: wr(positions=None), lambda: wr(q=None, q_out=q), lambda: sel(block_size=128), lambda: sel(summaries=s[:, :, :, :1]),
                 lambda: sel(out=spans), lambda: ops.kv4_summarise(c, i32, s[:2]), lambda: ops.kv4_gather(c, i32, table, 4, k_out=k),
                 lambda: dec(q=q[0]), lambda: dec(q=torch.zeros(2, 128, 4, dtype=BF, device=cuda).transpose(1, 2))):

@@ -26,7 +26,8 @@ LLAMA3 = {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_fr
 
 
 @pytest.mark.parametrize("scaling,head_dim,partial", [(YARN, 128, 1.0), ({**YARN, "beta_fast": 16, "beta_slow": 2}, 64, 1.0), (LLAMA3, 128, 1.0),
-                                                      ({"rope_type": "linear", "factor": 4.0}, 128, 0.5)])
+                                                      ({"rope_type": "linear", "factor": 4.0}, 128, 0.5), ({**YARN, "truncate": False}, 128, 1.0),
+                                                      ({**YARN, "mscale": 1.0, "mscale_all_dim": 0.707}, 64, 1.0), ({**YARN, "attention_factor": 1.5}, 64, 1.0)])
 def test_frequencies_are_those_of_hugging_face(scaling, head_dim, partial):
     from transformers.modeling_rope_utils import ROPE_INIT_FUNCTIONS
     from transformers import LlamaConfig
