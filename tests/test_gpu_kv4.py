@@ -498,3 +498,31 @@ def test_a_step_of_all_of_them(cuda):
         want = kh.select(q, tight, table, seen, budget)
         assert torch.equal(spans.cpu(), want)
         kh.assert_decode(out, *kh.decode(q, plain, table, seen, d ** -0.5, spans=want), f"step {k}")
+
+
+def test_a_cache_whose_offsets_pass_32_bits(cuda):
+    """The last blocks of 18 M slots (2.3 GB of codes a side) hold and give what the first ones do, bit for bit."""
+    g, hq, hkv, d, size, blocks, n = gen(40), 8, 1, 256, 256, 70000, 1500
+    cache = ops.KV4Cache.empty(blocks, size, hkv, d, cuda)
+    summaries, ws = ops.kv4_summaries(cache), ops.decode4_workspace(2, hq, hkv, d, cuda)
+    x = torch.randn(n, hq + 2 * hkv, d, generator=g).to(BF).to(cuda)
+    pos = torch.arange(n, device=cuda)
+    cos = build_cos_sin_cache(d, n, 1e4).to(cuda)
+    used = -(-n // size)
+    near = torch.arange(used, dtype=torch.int32, device=cuda)[None]
+    far = blocks - 1 - near
+    assert blocks * size * (d // 2) > 2 ** 31
+    got = []
+    for table in (near, far):
+        slots = (table[0].repeat_interleave(size) * size + torch.arange(size, dtype=torch.int32, device=cuda).repeat(used))[:n].contiguous()
+        q = ops.rotary_kv4_write(x[:, :hq], x[:, hq:hq + 1], x[:, hq + 1:], pos, cos, slots, cache, q_out=torch.empty(n, hq, d, dtype=BF, device=cuda))
+        ops.kv4_summarise(cache, slots, summaries)
+        lens, last, status = torch.tensor([n], dtype=torch.int32, device=cuda), q[-1:], ops.new_status(cuda)
+        spans = ops.kv4_select(last, summaries, lens, table, size, 6, status=status)
+        rows = ops.kv4_gather(cache, torch.tensor([0, n], dtype=torch.int32, device=cuda), table, n, status=status)
+        got.append((spans, *rows, ops.decode_attn4(last, cache, lens, table, d ** -0.5, -1, ws, status=status),
+                    ops.decode_attn4(last, cache, lens, table, d ** -0.5, -1, ws, spans=spans, status=status)))
+        ops.check_status(status)
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert torch.equal(got[1][2].cpu(), kh.stored(x[:, hq + 1:].cpu(), False, torch.float32).to(BF))
