@@ -17,7 +17,7 @@
 // large leaves nothing of its codes in the bf16 output.
 //
 // On paper bound by memory: a tile of 32 tokens of a 128-wide head is 4608 bytes.  Its 675 warp instructions, most of them on the integer
-// pipe, bring instruction issue near: 240 sequences of 128-8192 tokens, 16 heads on 8, 0.51 GB in 111 us, 4.6 TB/s (0.71 of what a copy reaches),
+// pipe, bring instruction issue near: 240 sequences of 128-8192 tokens, 16 heads on 8, 0.51 GB in 109 us, 4.7 TB/s (0.72 of what a copy reaches),
 // 62 % of the issue slots, the integer pipe at 58 %.  A few rows are bound by the chain of dependent loads (lengths, block lists, tiles, parts):
 // one context of 700 tokens 12 us.
 //
@@ -42,7 +42,7 @@ template <int D>
 struct Decode4Cfg {
   static constexpr int TOK = 32;                             // tokens of a tile
   static constexpr int NW = D == 256 ? 8 : 16;               // warps of a CTA
-  static constexpr int NST = 2;                              // tiles in a warp's ring (three: 113 us instead of 111 for the ragged batch)
+  static constexpr int NST = 2;                              // tiles in a warp's ring, one of them being computed (three: 113 us instead of 111 for the ragged batch)
   static constexpr int CODES = TOK * D / 2, AFF = TOK * D / 16;
   static constexpr int STAGE = 2 * CODES + 2 * AFF;          // key codes, value codes, key affine, value affine
   static constexpr int RING = NST * STAGE;
@@ -187,7 +187,6 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int total_s;
   __shared__ Decode4Share cut_s;
-  __shared__ int info_s[NW][NST];                            // first token of the tile in a stage, -1: nothing to read
   __shared__ int meta_s[NW][2][3];                           // a warp's parts: row (-1: none), the row's first tile and the one behind its last
   __shared__ Walk fs_s[NW], cs_s[NW];                        // a warp's fetching and computing side
   __shared__ Decode4Run run_s[NW];
@@ -233,7 +232,7 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
   // Few rows: whole CTAs for each of them, in proportion to its tiles but one for a row of up to three tiles a warp, so that a CTA works on one
   // row and most need no other CTA.  Where some CTA would get much more than its share, or there are more rows than CTAs: the even cut.
   // (8 rows of 22 tiles: 15.4 us cut evenly, 11.8 by rows; 128 rows of up to 17 tiles of 256-wide heads: 18.9 and 13.7; 8 rows of 1280: 30.5
-  // and 24.9.)
+  // and 24.8.)
   const int grid = gridDim.x, share = (total + grid - 1) / grid;
   const float part_of_grid = static_cast<float>(grid) / static_cast<float>(max(total, 1));
   auto ctas_of = [&](int v) -> int {                         // (a tile a warp at least: no CTA is left without one)
@@ -359,7 +358,8 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
   };
   int f_stage = 0, f_left = 0, f_token = 0, f_n = 0;
   int64_t f_off = -1;                                        // of the codes, in bytes; < 0: nothing to read
-  auto fetch = [&]() {
+  auto fetch = [&]() -> int {                                // the tile's first token, -1: nothing to read
+    int first = -1;
     if (ft < w1) {
       if (f_left == 0) {                                     // on to the run that look() found
         const Decode4Run run = run_s[warp];
@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
         f_off = ok ? kv4_row(block, p.hkv, run.h, p.block_size, in_block) * (D / 2) : -1;
       }
       const bool ok = f_off >= 0 && f_token < f_n;
-      if (lane == 0) info_s[warp][f_stage] = ok ? f_token : -1;
+      first = ok ? f_token : -1;
       if (ok) {
         const uint8_t* k = p.k_codes + f_off + lane * 16;
         const uint8_t* v = p.v_codes + f_off + lane * 16;
@@ -408,6 +408,7 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
       if (--f_left == 0) look();
     }
     cp_async_commit();
+    return first;
   };
   // q of a row, requested before anything that waits: word j of a lane is channels 8 (4 j + c4) .. of head g of the group
   uint4 qw[C::WK];
@@ -421,8 +422,8 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
   if (w0 < w1) ask_q(cs.b, cs.h);
   if (lane == 0) cs_s[warp] = cs;
   look();
-#pragma unroll
-  for (int i = 0; i < NST - 1; ++i) fetch();
+  static_assert(NST == 2, "one tile is on its way while another is computed");
+  int on_its_way = fetch();
 
   // ---- the computing side -----------------------------------------------------------------------------------------------------------
   const int kt = decode4_row(g);                             // this lane's token of eight, in the roles of a key's row and of a score's
@@ -484,8 +485,8 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
       if (t == row_t0) continue;                             // (the tile without tokens)
       cp_async_wait<NST - 2>();
       __syncwarp();                                          // the tile is there for every lane, and the one before has been read by all
-      fetch();
-      const int token0 = info_s[warp][stage];
+      const int token0 = on_its_way;
+      on_its_way = fetch();
       const uint8_t* at = smem + warp * C::RING + stage * C::STAGE;
       stage = stage + 1 == NST ? 0 : stage + 1;
       if (token0 < 0) continue;
