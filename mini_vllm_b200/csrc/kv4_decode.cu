@@ -19,7 +19,7 @@
 // On paper bound by memory: a tile of 32 tokens of a 128-wide head is 4608 bytes.  Its 675 warp instructions, most of them on the integer
 // pipe, bring instruction issue near: 240 sequences of 128-8192 tokens, 16 heads on 8, 0.51 GB in 109 us, 4.7 TB/s (0.72 of what a copy reaches),
 // 62 % of the issue slots, the integer pipe at 58 %.  A few rows are bound by the chain of dependent loads (lengths, block lists, tiles, parts):
-// one context of 700 tokens 12 us.
+// one context of 700 tokens 10 us.
 //
 // Work is tiles of 32 tokens of one (sequence, head), numbered sequence by sequence and head by head.  Each CTA takes a contiguous range (all
 // alike, or, where there are few rows, a share of one of them), each of its warps a contiguous part of that.  A warp streams its tiles
@@ -38,10 +38,12 @@ namespace mvb {
 constexpr int kDecode4MaxGroup = 8;
 constexpr int kDecode4MaxCtas = 160;
 
-template <int D>
+constexpr int kDecode4MaxWarps = 16;
+
+template <int D, int W>
 struct Decode4Cfg {
   static constexpr int TOK = 32;                             // tokens of a tile
-  static constexpr int NW = D == 256 ? 8 : 16;               // warps of a CTA
+  static constexpr int NW = W;                               // warps of a CTA
   static constexpr int NST = 2;                              // tiles in a warp's ring, one of them being computed (three: 113 us instead of 111 for the ragged batch)
   static constexpr int CODES = TOK * D / 2, AFF = TOK * D / 16;
   static constexpr int STAGE = 2 * CODES + 2 * AFF;          // key codes, value codes, key affine, value affine
@@ -56,7 +58,7 @@ struct Decode4Cfg {
 // floats of a part that a CTA leaves for others: outputs of the group's heads, then their log2-sum-exps, one copy for each warp that merges
 // a share of the channels
 __host__ __device__ __forceinline__ constexpr int decode4_part(int group, int d) {
-  return group * d + kDecode4MaxGroup * (d == 256 ? Decode4Cfg<256>::NW : Decode4Cfg<128>::NW);
+  return group * d + kDecode4MaxGroup * kDecode4MaxWarps;
 }
 
 struct Decode4Params {
@@ -72,7 +74,7 @@ struct Decode4Params {
   int table_width, max_len, num_seqs, hkv, group, block_size, budget, window_left;
   float scale_log2, cap_in, cap_log2, out_scale;
   float* parts;                        // [CTAs][2]: of the CTA's first row and of its last
-  int32_t* arrivals;                   // [num_seqs * hkv][NW], zero between launches
+  int32_t* arrivals;                   // [num_seqs * hkv][warps], zero between launches
   int* dev_status;
 };
 
@@ -178,9 +180,9 @@ struct Decode4Share {
   int t0, t1, first, parts;
 };
 
-template <int D, bool CAP>
-__global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(const Decode4Params p) {
-  using C = Decode4Cfg<D>;
+template <int D, bool CAP, int W>
+__global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const Decode4Params p) {
+  using C = Decode4Cfg<D, W>;
   using Walk = Decode4Walk<C::TOK>;
   constexpr int NW = C::NW, NT = NW * 32, NST = C::NST, GRP = C::GRP;
   constexpr uint32_t FULL = 0xffffffffu, LO = 0x000f000fu, HI = 0x00f000f0u, BYTE = 0x00ff00ffu;
@@ -231,8 +233,8 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
   }
   // Few rows: whole CTAs for each of them, in proportion to its tiles but one for a row of up to three tiles a warp, so that a CTA works on one
   // row and most need no other CTA.  Where some CTA would get much more than its share, or there are more rows than CTAs: the even cut.
-  // (8 rows of 22 tiles: 15.4 us cut evenly, 11.8 by rows; 128 rows of up to 17 tiles of 256-wide heads: 18.9 and 13.7; 8 rows of 1280: 30.5
-  // and 24.8.)
+  // (Cut evenly and by rows: 8 rows of 22 tiles, sixteen warps, 15.4 and 11.8 us; 128 rows of up to 17 tiles of 256-wide heads 18.9 and 13.7; 8 rows
+  // of 1280, sixteen warps, 30.5 and 24.8.)
   const int grid = gridDim.x, share = (total + grid - 1) / grid;
   const float part_of_grid = static_cast<float>(grid) / static_cast<float>(max(total, 1));
   auto ctas_of = [&](int v) -> int {                         // (a tile a warp at least: no CTA is left without one)
@@ -850,10 +852,10 @@ __global__ void __launch_bounds__(Decode4Cfg<D>::NW * 32, 1) kv4_decode_kernel(c
 // The parts have the room that the largest head shape needs, so that the counters lie at the same place for every shape and batch: one
 // workspace may serve different calls one after the other and the counters are zero between them.
 constexpr size_t kDecode4Parts = sizeof(float) * kDecode4MaxCtas * 2 * decode4_part(kDecode4MaxGroup, 256);
-static_assert(kDecode4Parts % 256 == 0 && decode4_part(kDecode4MaxGroup, 256) >= decode4_part(kDecode4MaxGroup, 128), "");
+static_assert(kDecode4Parts % 256 == 0, "the counters lie at a multiple of 256 bytes");
 
 static size_t decode4_bytes(int64_t seqs, int hkv) {
-  return kDecode4Parts + (sizeof(int32_t) * static_cast<size_t>(seqs) * hkv * Decode4Cfg<128>::NW + 255) / 256 * 256;
+  return kDecode4Parts + (sizeof(int32_t) * static_cast<size_t>(seqs) * hkv * kDecode4MaxWarps + 255) / 256 * 256;
 }
 
 }  // namespace mvb
@@ -899,17 +901,28 @@ extern "C" int mvb_decode_attn4(const void* q, int64_t q_row_stride, const mvb_k
   p.dev_status = dev_status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int grid = sm_count() < kDecode4MaxCtas ? sm_count() : kDecode4MaxCtas;
-  auto launch = [&](auto tag, auto cap) -> int {
-    constexpr int D = decltype(tag)::value;
-    using C = Decode4Cfg<D>;
+  // Sixteen warps keep an SM's pipes busier, eight have twice the registers and are quicker from the first load to the last part (and take a
+  // shorter row by themselves): eight up to 200 tiles an SM (80 of 64-wide heads), as far as the call can tell; always eight for heads of 256,
+  // whose fragments need the registers.  8 heads of 128, sixteen and eight: 1 context of 700 tokens 11.7 and 9.4 us, of 40000 21.7 and 19.4, 32 of
+  // 1000 22.2 and 19.7, 32 of 4000 39.1 and 38.7, 4 of 40000 45.3 and 47.1, 64 of 4000 61 and 65.  2 heads of 64: 1 of 40000 16.8 and 13.8, 32 of
+  // 4000 16.6 and 16.3, 16 of 16000 20.2 and 21.1
+  int64_t most = longest * cache->block_size / 32 + 1;       // tiles of a row
+  if (window_left >= 0 && (static_cast<int64_t>(window_left) + 1) / 32 + 2 < most) most = (static_cast<int64_t>(window_left) + 1) / 32 + 2;
+  if (spans != nullptr && static_cast<int64_t>(budget) * (kKv4Span / 32) < most) most = static_cast<int64_t>(budget) * (kKv4Span / 32);
+  const bool few = static_cast<int64_t>(num_seqs) * hkv * most <= static_cast<int64_t>(sm_count()) * (cache->head_dim == 64 ? 80 : 200);
+  auto launch = [&](auto tag, auto cap, auto warps) -> int {
+    constexpr int D = decltype(tag)::value, W = decltype(warps)::value;
+    using C = Decode4Cfg<D, W>;
     struct Tag {};
-    const int r = opt_in_dynamic_smem<Tag>(reinterpret_cast<const void*>(&kv4_decode_kernel<D, decltype(cap)::value>), C::SMEM);
+    const int r = opt_in_dynamic_smem<Tag>(reinterpret_cast<const void*>(&kv4_decode_kernel<D, decltype(cap)::value, W>), C::SMEM);
     if (r != kOk) return r;
-    kv4_decode_kernel<D, decltype(cap)::value><<<grid, C::NW * 32, C::SMEM, st>>>(p);
+    kv4_decode_kernel<D, decltype(cap)::value, W><<<grid, C::NW * 32, C::SMEM, st>>>(p);
     return cudaGetLastError() == cudaSuccess ? kOk : kLaunchFailed;
   };
-  auto by_cap = [&](auto tag) -> int { return softcap > 0.f ? launch(tag, std::true_type{}) : launch(tag, std::false_type{}); };
-  if (cache->head_dim == 64) return by_cap(std::integral_constant<int, 64>{});
-  if (cache->head_dim == 128) return by_cap(std::integral_constant<int, 128>{});
-  return by_cap(std::integral_constant<int, 256>{});
+  auto by_cap = [&](auto tag, auto warps) -> int { return softcap > 0.f ? launch(tag, std::true_type{}, warps) : launch(tag, std::false_type{}, warps); };
+  const std::integral_constant<int, 8> eight{};
+  const std::integral_constant<int, 16> sixteen{};
+  if (cache->head_dim == 64) return few ? by_cap(std::integral_constant<int, 64>{}, eight) : by_cap(std::integral_constant<int, 64>{}, sixteen);
+  if (cache->head_dim == 128) return few ? by_cap(std::integral_constant<int, 128>{}, eight) : by_cap(std::integral_constant<int, 128>{}, sixteen);
+  return by_cap(std::integral_constant<int, 256>{}, eight);
 }

@@ -128,7 +128,7 @@ def test_gather(cuda, d, hkv, size):
 
 
 # ---- attention of single tokens ---------------------------------------------------------------------------------------------------------
-def run_decode(cuda, lens, hq, hkv, d, size=256, window=-1, cap=0.0, spans=None, seed=0, v_size=1.0, width=None, workspace=None, change=None, q_scale=1.0):
+def run_decode(cuda, lens, hq, hkv, d, size=256, window=-1, cap=0.0, spans=None, seed=0, v_size=1.0, width=None, workspace=None, change=None, q_scale=1.0, pool=0):
     g = gen(seed)
     table, blocks = kh.block_lists(g, lens, size, width)
     cache = kh.make_cache(g, blocks, hkv, size, d, v_size)
@@ -143,7 +143,13 @@ def run_decode(cuda, lens, hq, hkv, d, size=256, window=-1, cap=0.0, spans=None,
     packed = torch.zeros(len(lens), hq * d + 16, dtype=BF, device=cuda)                 # rows further apart than they are long
     qd = packed[:, 8:8 + hq * d].view(len(lens), hq, d)
     qd.copy_(q)
-    got = ops.decode_attn4(qd, on(cuda, cache), torch.tensor(lens, dtype=torch.int32, device=cuda), table.to(cuda), d ** -0.5, window, ws,
+    dev = on(cuda, cache)
+    if pool > blocks:                                               # more blocks than anyone holds
+        big_one = ops.KV4Cache.empty(pool, size, hkv, d, cuda)
+        for to, rows in ((big_one.k_codes, dev.k_codes), (big_one.k_affine, dev.k_affine), (big_one.v_codes, dev.v_codes), (big_one.v_affine, dev.v_affine)):
+            to[:blocks] = rows
+        dev = big_one
+    got = ops.decode_attn4(qd, dev, torch.tensor(lens, dtype=torch.int32, device=cuda), table.to(cuda), d ** -0.5, window, ws,
                            spans=None if spans is None else spans.to(cuda), out=out, status=status, softcap=cap)
     ops.check_status(status)
     assert got is out
@@ -216,6 +222,29 @@ def test_decode_one_workspace_for_every_shape(cuda):
     ws = ops.decode4_workspace(64, 16, 8, 256, cuda)
     for hq, hkv, d in ((16, 8, 128), (8, 1, 256), (2, 2, 64), (32, 8, 256), (16, 8, 128)):
         run_decode(cuda, [3000, 40, 900], hq, hkv, d, workspace=ws, seed=d)
+
+
+WIDE = dict(width=2000, pool=2000)                                  # room for contexts of half a million tokens: sixteen warps a block
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 128), (16, 8, 128), (8, 2, 64), (14, 2, 64)])
+@pytest.mark.parametrize("lens", [[1], [700], [9000], [9000] + [3] * 40 + [0, 700], [40] * 150, [300, 0, 280, 310, 0] * 20, [31, 32, 33, 63, 64, 65, 255, 256, 257, 0]])
+def test_decode_with_room_for_long_contexts(cuda, lens, hq, hkv, d):
+    run_decode(cuda, lens, hq, hkv, d, seed=len(lens), **WIDE)
+
+
+def test_decode_both_kinds_of_blocks_on_one_workspace(cuda):
+    ws = ops.decode4_workspace(64, 16, 8, 256, cuda)
+    for more in ({}, WIDE, {}, dict(WIDE, cap=30.0), dict(cap=30.0), WIDE):
+        run_decode(cuda, [3000, 40, 900, 0], 16, 8, 128, workspace=ws, seed=9, **more)
+
+
+def test_decode_windows_and_spans_of_many_sequences(cuda):
+    g, lens = gen(6), [(i * 37) % 400 + 1 for i in range(240)]
+    run_decode(cuda, lens, 16, 8, 128, window=600, width=40, pool=600, seed=5)
+    spans = torch.stack([torch.stack([torch.cat([torch.randperm(-(-n // 64), generator=g)[:4].int(), torch.full((60,), -1, dtype=torch.int32)])[:12] for _ in range(8)])
+                         if n > 192 else torch.cat([torch.arange(-(-n // 64)), torch.full((12,), -1)])[:12].int().repeat(8, 1) for n in lens]).contiguous()
+    run_decode(cuda, lens, 16, 8, 128, spans=spans, seed=5)
 
 
 def test_decode_same_bits_every_time(cuda):
