@@ -905,11 +905,12 @@ extern "C" int mvb_decode_attn4(const void* q, int64_t q_row_stride, const mvb_k
   // shorter row by themselves): eight up to 200 tiles an SM (80 of 64-wide heads), as far as the call can tell; always eight for heads of 256,
   // whose fragments need the registers.  8 heads of 128, sixteen and eight: 1 context of 700 tokens 11.7 and 9.4 us, of 40000 21.7 and 19.4, 32 of
   // 1000 22.2 and 19.7, 32 of 4000 39.1 and 38.7, 4 of 40000 45.3 and 47.1, 64 of 4000 61 and 65.  2 heads of 64: 1 of 40000 16.8 and 13.8, 32 of
-  // 4000 16.6 and 16.3, 16 of 16000 20.2 and 21.1
+  // 4000 16.6 and 16.3, 16 of 16000 20.2 and 21.1.  Lists of spans, a run of loads more for every two tiles, half of that: 8 heads of 128, 64 spans
+  // for 1 sequence 14.1 and 11.2, 16 for 48 27.4 and 25.5, 16 for 96 38.4 and 39.9, 64 for 64 73 and 81
   int64_t most = longest * cache->block_size / 32 + 1;       // tiles of a row
   if (window_left >= 0 && (static_cast<int64_t>(window_left) + 1) / 32 + 2 < most) most = (static_cast<int64_t>(window_left) + 1) / 32 + 2;
   if (spans != nullptr && static_cast<int64_t>(budget) * (kKv4Span / 32) < most) most = static_cast<int64_t>(budget) * (kKv4Span / 32);
-  const bool few = static_cast<int64_t>(num_seqs) * hkv * most <= static_cast<int64_t>(sm_count()) * (cache->head_dim == 64 ? 80 : 200);
+  const bool few = static_cast<int64_t>(num_seqs) * hkv * most <= static_cast<int64_t>(sm_count()) * (cache->head_dim == 64 ? 80 : 200) / (spans != nullptr ? 2 : 1);
   auto launch = [&](auto tag, auto cap, auto warps) -> int {
     constexpr int D = decltype(tag)::value, W = decltype(warps)::value;
     using C = Decode4Cfg<D, W>;
