@@ -16,9 +16,9 @@
 // token's values), with size = max(scale, 2^-20 |minimum|, 2^-100), which bounds every p s by 2^6 and every p m by 2^26; a minimum that
 // large leaves nothing of its codes in the bf16 output.
 //
-// On paper bound by memory: a tile of 32 tokens of a 128-wide head is 4608 bytes.  Its 675 warp instructions, most of them on the integer
+// On paper bound by memory: a tile of 32 tokens of a 128-wide head is 4608 bytes.  Its 655 warp instructions, most of them on the integer
 // pipe, bring instruction issue near: 240 sequences of 128-8192 tokens, 16 heads on 8, 0.51 GB in 109 us, 4.7 TB/s (0.72 of what a copy reaches),
-// 62 % of the issue slots, the integer pipe at 58 %.  A few rows are bound by the chain of dependent loads (lengths, block lists, tiles, parts):
+// 64 % of the issue slots, the integer pipe at 60 %.  A few rows are bound by the chain of dependent loads (lengths, block lists, tiles, parts):
 // one context of 700 tokens 10 us.
 //
 // Work is tiles of 32 tokens of one (sequence, head), numbered sequence by sequence and head by head.  Each CTA takes a contiguous range (all
