@@ -93,6 +93,10 @@ class Config:
             raise ValueError("kv_cache_block_size must be a multiple of 128 (the prefill KV tile)")
 
 
+def _rope_kind(parameters) -> str:
+    return parameters.get("rope_type", parameters.get("type", "default")) if isinstance(parameters, dict) else "default"
+
+
 def _flatten_hf(cfg) -> SimpleNamespace:
     """Copy the attributes the engine reads; newer transformers keep the RoPE bases in rope_parameters."""
     names = ["architectures", "num_hidden_layers", "num_attention_heads", "num_key_value_heads", "head_dim",
@@ -101,9 +105,13 @@ def _flatten_hf(cfg) -> SimpleNamespace:
              "sliding_window", "rope_theta", "rope_local_base_freq"]
     out = SimpleNamespace(**{n: getattr(cfg, n) for n in names if hasattr(cfg, n)})
     rp = getattr(cfg, "rope_parameters", None)
-    scaling = getattr(cfg, "rope_scaling", None) or (rp.get("full_attention", rp) if isinstance(rp, dict) else None)
+    # where layers of several kinds rotate (Gemma3), each kind has parameters of its own; newer transformers have both names for one thing
+    scaling = rp or getattr(cfg, "rope_scaling", None)
     if isinstance(scaling, dict):
-        kind = scaling.get("rope_type", scaling.get("type", "default"))
+        if _rope_kind(scaling.get("sliding_attention")) != "default":
+            log.warning("rope scaling of the layers with a window is left out: %r", scaling["sliding_attention"])
+        scaling = scaling.get("full_attention", scaling)
+        kind = _rope_kind(scaling)
         if kind in ("linear", "yarn", "llama3"):
             out.rope_scaling = dict(scaling)
             if out.rope_scaling.get("original_max_position_embeddings") is None:
