@@ -11,13 +11,14 @@
 // channel have to meet in a register: a byte permutation, and the high codes of a byte are never masked out, their sums are those of
 // whole bytes less those of the low codes), and scales and minima cost a few per token.  q is brought to [2^14, 2^15)
 // by a power of two per head so that fp16 holds every bf16 exactly down to 2^-29 of the greatest; the channels whose codes sit at bits 4-7
-// (16 times as large) have it divided by 16.  Scores, softmax statistics and outputs are fp32; the weights p s are rounded once, to fp16,
-// an eighth of what bf16 weights would lose.  They never overflow: the softmax's reference is the greatest score + log2(size of the
-// token's values), with size = max(scale, 2^-20 |minimum|, 2^-100), which bounds every p s by 2^6 and every p m by 2^26; a minimum that
-// large leaves nothing of its codes in the bf16 output.
+// (16 times as large) have it divided by 16.  Scores, softmax statistics and outputs are fp32; the weights p s are rounded once, to fp16.  Every
+// group of channels and head has a power of two of its own on them, moved when the group's greatest weight would pass 2^14: they never
+// overflow, and a group keeps its bits whatever the sizes of other groups, tokens and heads (scales from 2^-120 on; p itself is at most 2^-14, so
+// that a warp's sum of p m is finite too, for 16 K tokens of the largest values there are).  A rounding of p s meets the codes, up to 15 of them, while p m is exact: next to the plain form's error that is
+// 2^-11 sum p (15 s) more at most.
 //
 // On paper bound by memory: a tile of 32 tokens of a 128-wide head is 4608 bytes.  Its 655 warp instructions, most of them on the integer
-// pipe, bring instruction issue near: 240 sequences of 128-8192 tokens, 16 heads on 8, 0.51 GB in 109 us, 4.7 TB/s (0.72 of what a copy reaches),
+// pipe, bring instruction issue near: 240 sequences of 128-8192 tokens, 16 heads on 8, 0.51 GB in 114 us, 4.5 TB/s (0.69 of what a copy reaches),
 // 64 % of the issue slots, the integer pipe at 60 %.  A few rows are bound by the chain of dependent loads (lengths, block lists, tiles, parts):
 // one context of 700 tokens 10 us.
 //
@@ -99,6 +100,23 @@ __device__ __forceinline__ float fast_log2(float x) {
   float y;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// Powers of two, as their exponents say: of a whole number (0 below 2^-126, at most 2^127; of one that is not a number 0), one over 2^-126 .. 2^126,
+// and what brings the greatest of a group's weights to 2^8 .. 2^9
+constexpr float kMostUp = 0x1p126f;
+__device__ __forceinline__ float pow2_whole(float x) {
+  return __uint_as_float(static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(x, -127.f), 127.f)) + 127) << 23);
+}
+__device__ __forceinline__ float pow2_inverse(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
+__device__ __forceinline__ float up_for(float most) {
+  const int e = static_cast<int>(__float_as_uint(most) >> 23) - 127;
+  return __uint_as_float(static_cast<uint32_t>(127 + max(min(8 - e, 126), -102)) << 23);
+}
+// the outputs of a group's channels, by a factor for each of the two heads
+template <int N>
+__device__ __forceinline__ void scale_group(float (&o)[N][4], int j, float a, float b) {
+#pragma unroll
+  for (int i = 4 * j; i < 4 * j + 4; ++i) { o[i][0] *= a; o[i][1] *= b; o[i][2] *= a; o[i][3] *= b; }
 }
 template <int N>
 __device__ __forceinline__ void lds_words(const uint8_t* at, uint32_t (&w)[N]) {
@@ -478,10 +496,11 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const Decode4Para
       f_b = __shfl_sync(FULL, f, 8 * c4 + 4);
     }
     float o[4 * C::WV][4], l_a = 0.f, l_b = 0.f, m_a = -INFINITY, m_b = -INFINITY, pm_a[GRP], pm_b[GRP];
+    float2 up[GRP];                                          // what the group's weights are multiplied by, of the two heads
 #pragma unroll
     for (int i = 0; i < 4 * C::WV; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
-    for (int j = 0; j < GRP; ++j) pm_a[j] = pm_b[j] = 0.f;
+    for (int j = 0; j < GRP; ++j) { pm_a[j] = pm_b[j] = 0.f; up[j] = make_float2(kMostUp, kMostUp); }
 
     for (; t < seg_end; ++t) {
       if (t == row_t0) continue;                             // (the tile without tokens)
@@ -558,38 +577,75 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const Decode4Para
             for (int j = 0; j < GRP; ++j) va[s][1][j] = 0u;
           }
         }
-        float big0 = 0x1p-100f, big1 = 0x1p-100f;
-#pragma unroll
-        for (int j = 0; j < GRP; ++j) {
-          big0 = fmax3(big0, kv4_scale(va[s][0][j]), fabsf(kv4_min(va[s][0][j])) * 0x1p-20f);
-          big1 = fmax3(big1, kv4_scale(va[s][1][j]), fabsf(kv4_min(va[s][1][j])) * 0x1p-20f);
-        }
-        big0 = fast_log2(big0); big1 = fast_log2(big1);
-        ta = fmax3(ta, x[s][0] + big0, x[s][2] + big1);
-        tb = fmax3(tb, x[s][1] + big0, x[s][3] + big1);
+        ta = fmax3(ta, x[s][0], x[s][2]);
+        tb = fmax3(tb, x[s][1], x[s][3]);
       }
-      // ---- the running reference: moved only when a weight would pass 2^6, which fp16 holds with room to spare ----------------------------
-      if (__any_sync(FULL, ta > m_a + 6.f || tb > m_b + 6.f)) {
+      // ---- the running reference, a whole number at least 14 above every score: weights stay below 2^-14, and old ones change by powers of two.
+      // What the groups' weights are multiplied by moves against it, so that what has been added up stays as it is ----------------------------
+      if (__any_sync(FULL, ta > m_a - 14.f || tb > m_b - 14.f)) {
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) {
           ta = fmaxf(ta, __shfl_xor_sync(FULL, ta, off));
           tb = fmaxf(tb, __shfl_xor_sync(FULL, tb, off));
         }
-        ta = fmaxf(m_a, ta); tb = fmaxf(m_b, tb);
-        const float alpha_a = ta == -INFINITY ? 1.f : fast_exp2(m_a - ta), alpha_b = tb == -INFINITY ? 1.f : fast_exp2(m_b - tb);
+        ta = fmaxf(m_a, ceilf(ta) + 20.f); tb = fmaxf(m_b, ceilf(tb) + 20.f);
+        const float less_a = pow2_whole(m_a - ta), less_b = pow2_whole(m_b - tb), more_a = pow2_whole(ta - m_a), more_b = pow2_whole(tb - m_b);
         m_a = ta; m_b = tb;
-        l_a *= alpha_a; l_b *= alpha_b;
+        l_a *= less_a; l_b *= less_b;
 #pragma unroll
-        for (int j = 0; j < GRP; ++j) { pm_a[j] *= alpha_a; pm_b[j] *= alpha_b; }
-#pragma unroll
-        for (int i = 0; i < 4 * C::WV; ++i) { o[i][0] *= alpha_a; o[i][1] *= alpha_b; o[i][2] *= alpha_a; o[i][3] *= alpha_b; }
+        for (int j = 0; j < GRP; ++j) {
+          pm_a[j] *= less_a; pm_b[j] *= less_b;
+          const float2 to = make_float2(fminf(up[j].x * more_a, kMostUp), fminf(up[j].y * more_b, kMostUp));
+          scale_group(o, j, to.x * pow2_inverse(up[j].x) * less_a, to.y * pow2_inverse(up[j].y) * less_b);
+          up[j] = to;
+        }
       }
       const float ra = m_a == -INFINITY ? 0.f : m_a, rb = m_b == -INFINITY ? 0.f : m_b;
-      // ---- weights: transposed, as the B operand of the values --------------------------------------------------------------------
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const float p0 = fast_exp2(x[s][0] - ra), p1 = fast_exp2(x[s][1] - rb), p2 = fast_exp2(x[s][2] - ra), p3 = fast_exp2(x[s][3] - rb);
-        l_a += p0 + p2; l_b += p1 + p3;
+        x[s][0] = fast_exp2(x[s][0] - ra); x[s][1] = fast_exp2(x[s][1] - rb); x[s][2] = fast_exp2(x[s][2] - ra); x[s][3] = fast_exp2(x[s][3] - rb);
+        l_a += x[s][0] + x[s][2]; l_b += x[s][1] + x[s][3];
+      }
+      // ---- weights p s to fp16, each group's in a range of its own: its greatest is brought to 2^8 .. 2^9 when it would pass 2^14 ----------
+      uint32_t w[2][GRP][2];
+#pragma unroll 1
+      for (bool again = true;;) {
+        float most = 0.f;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+          for (int j = 0; j < GRP; ++j) {
+            const float s0 = kv4_scale(va[s][0][j]), s1 = kv4_scale(va[s][1][j]);
+            const float2 w0 = mul_f32x2(mul_f32x2(make_float2(x[s][0], x[s][1]), up[j]), make_float2(s0, s0));
+            const float2 w1 = mul_f32x2(mul_f32x2(make_float2(x[s][2], x[s][3]), up[j]), make_float2(s1, s1));
+            most = fmax3(fmax3(most, w0.x, w0.y), w1.x, w1.y);
+            w[s][j][0] = pack_f16(w0.x, w0.y); w[s][j][1] = pack_f16(w1.x, w1.y);
+          }
+        }
+        if (!__any_sync(FULL, most > 0x1p14f) || !again) break;             // (a weight that is not finite stays so)
+        again = false;
+#pragma unroll
+        for (int j = 0; j < GRP; ++j) {
+          float a = 0.f, b = 0.f;                            // the tile's greatest p s, of both heads
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const float s0 = kv4_scale(va[s][0][j]), s1 = kv4_scale(va[s][1][j]);
+            a = fmax3(a, x[s][0] * s0, x[s][2] * s1);
+            b = fmax3(b, x[s][1] * s0, x[s][3] * s1);
+          }
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) {
+            a = fmaxf(a, __shfl_xor_sync(FULL, a, off));
+            b = fmaxf(b, __shfl_xor_sync(FULL, b, off));
+          }
+          const float2 to = make_float2(fminf(up[j].x, up_for(a)), fminf(up[j].y, up_for(b)));
+          scale_group(o, j, to.x * pow2_inverse(up[j].x), to.y * pow2_inverse(up[j].y));
+          up[j] = to;
+        }
+      }
+      // ---- transposed, as the B operand of the values -----------------------------------------------------------------------------------
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
         uint32_t v00[C::WV], v01[C::WV], v10[C::WV], v11[C::WV];
         const int u0 = 16 * s + vt0, u1 = 16 * s + vt1;
         const uint8_t* vat = at + C::CODES;
@@ -600,10 +656,10 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const Decode4Para
         value(u0, v00); value(u1, v01); value(u0 + 8, v10); value(u1 + 8, v11);
 #pragma unroll
         for (int j = 0; j < GRP; ++j) {
-          const float s0 = kv4_scale(va[s][0][j]), s1 = kv4_scale(va[s][1][j]), m0 = kv4_min(va[s][0][j]), m1 = kv4_min(va[s][1][j]);
-          pm_a[j] = fmaf(p0, m0, fmaf(p2, m1, pm_a[j]));
-          pm_b[j] = fmaf(p1, m0, fmaf(p3, m1, pm_b[j]));
-          const uint32_t b0 = movmatrix_trans(pack_f16(p0 * s0, p1 * s0)), b1 = movmatrix_trans(pack_f16(p2 * s1, p3 * s1));
+          const float m0 = kv4_min(va[s][0][j]), m1 = kv4_min(va[s][1][j]);
+          pm_a[j] = fmaf(x[s][0], m0, fmaf(x[s][2], m1, pm_a[j]));
+          pm_b[j] = fmaf(x[s][1], m0, fmaf(x[s][3], m1, pm_b[j]));
+          const uint32_t b0 = movmatrix_trans(w[s][j][0]), b1 = movmatrix_trans(w[s][j][1]);
           const uint32_t xl = __byte_perm(v00[j], v01[j], 0x5410), yl = __byte_perm(v00[j], v01[j], 0x7632);
           const uint32_t xh = __byte_perm(v10[j], v11[j], 0x5410), yh = __byte_perm(v10[j], v11[j], 0x7632);
           // channels 0, 1 of the lane's word by their own codes, 2, 3 by whole bytes c + 16 c' (less those of 0, 1 at the end); 4 .. 7 alike
@@ -665,14 +721,15 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const Decode4Para
       const float inv = l > 0.f ? (complete ? p.out_scale : 1.f) / l : 0.f;
 #pragma unroll
       for (int j = 0; j < C::WV; ++j) {
+        const float by = 0x1p24f * pow2_inverse(side ? up[j].y : up[j].x), by16 = by * 0.0625f;
         float y[8];                                          // channels 64 j + 8 g ..: rows g (even) and g + 8 (odd) of four tiles
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float add = side ? pm_b[j] : pm_a[j];
           const float* even = o[4 * j + (i & 2)];
           const float* at = o[4 * j + i];
-          y[2 * i] = (i & 1) ? fmaf(at[side] - even[side], 0x1p20f, add) * inv : fmaf(at[side], 0x1p24f, add) * inv;
-          y[2 * i + 1] = (i & 1) ? fmaf(at[2 + side] - even[2 + side], 0x1p20f, add) * inv : fmaf(at[2 + side], 0x1p24f, add) * inv;
+          y[2 * i] = (i & 1) ? fmaf(at[side] - even[side], by16, add) * inv : fmaf(at[side], by, add) * inv;
+          y[2 * i + 1] = (i & 1) ? fmaf(at[2 + side] - even[2 + side], by16, add) * inv : fmaf(at[2 + side], by, add) * inv;
         }
         if (complete) store_vec<__nv_bfloat16, 8>(p.out + b * p.out_stride + (static_cast<int64_t>(h) * G + head) * D + 64 * j + 8 * g, y);
         else store_f32<8>(part + head * D + 64 * j + 8 * g, y);

@@ -1,0 +1,117 @@
+"""The 4-bit cache (CUDA) where its users rarely go."""
+import pytest
+import torch
+
+from mini_vllm_b200 import ops
+from tests import kv4_helpers as kh
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+NAN, INF = float("nan"), float("inf")
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def on(cuda, cache) -> ops.KV4Cache:
+    return ops.KV4Cache(*(t.to(cuda) for t in cache))
+
+
+def call(cuda, q, cache, table, lens, window=-1, spans=None, room=None, status=None):
+    """``room``: blocks in the pool and columns in the table, more than anyone holds."""
+    dev, (blocks, hkv, size), d = on(cuda, cache), cache[0].shape[:3], q.shape[2]
+    if room is not None:
+        wide = torch.full((table.shape[0], room), -1, dtype=torch.int32)
+        wide[:, :table.shape[1]] = table
+        big, table = ops.KV4Cache.empty(room, size, hkv, d, cuda), wide
+        for to, rows in zip((big.k_codes, big.k_affine, big.v_codes, big.v_affine), (dev.k_codes, dev.k_affine, dev.v_codes, dev.v_affine)):
+            to[:blocks] = rows
+        dev = big
+    ws = ops.decode4_workspace(len(lens), q.shape[1], hkv, d, cuda)
+    return ops.decode_attn4(q.to(cuda), dev, torch.tensor(lens, dtype=torch.int32, device=cuda), table.to(cuda), d ** -0.5, window, ws,
+                            spans=None if spans is None else spans.to(cuda), status=status).double().cpu()
+
+
+# ---- groups of unequal size ---------------------------------------------------------------------------------------------------------------
+def group_bound(q, cache, table, lens):
+    """Per sequence, head and group of 64 channels, the bound that goes with that group alone.  With p the softmax: a weight p s to fp16 is off
+    by 2^-11 of itself and meets codes of at most 15: 2^-11 sum p (15 s).  Scores are fp32 sums, good to 2^-14, and with them each weight, twice
+    (numerator and sum): 2^-13 sum p |v|.  Weights below fp16's normal numbers are off by 2^-25, the group's greatest being 2^8 at least:
+    2^-33 of the greatest p (15 s) for each token.  Sums run in fp32, a step for 16 tokens, each good to 2^-23: n 2^-27 of what is added up."""
+    hkv, d = cache[0].shape[1], q.shape[2]
+    group, out = q.shape[1] // hkv, torch.zeros(*q.shape[:2], d // 64, dtype=kh.F64)
+    for b, n in enumerate(lens):
+        k, v = kh.context(cache, table, b, n)
+        size = cache[0].shape[2]
+        s = cache[3][table[b, :-(-n // size)].long()].transpose(0, 1).flatten(1, 2)[:, :n, :, 0].to(kh.F64) * 15
+        for h in range(hkv):
+            p = torch.softmax(q[b, h * group:(h + 1) * group].to(kh.F64) @ k[h].T * d ** -0.5, -1)
+            v_size = v[h].abs().unflatten(-1, (-1, 64)).amax(-1)
+            sums = p @ s[h], p @ v_size
+            out[b, h * group:(h + 1) * group] = ((2.0 ** -11 + n * 2.0 ** -27) * sums[0] + (2.0 ** -13 + n * 2.0 ** -27) * sums[1] +
+                                                 n * 2.0 ** -33 * (p[..., None] * s[h]).amax(1))
+    return out
+
+
+def check_groups(cuda, change, hq, hkv, d, lens, seed, **kw):
+    g = gen(seed)
+    table, blocks = kh.block_lists(g, lens, 256)
+    cache = kh.make_cache(g, blocks, hkv, 256, d)
+    change(cache, table)
+    kh.poison(cache, table, lens, 256)
+    q = torch.randn(len(lens), hq, d, generator=g).to(BF)
+    got, (want, _) = call(cuda, q, cache, table, lens, **kw), kh.decode(q, cache, table, lens, d ** -0.5)
+    assert torch.isfinite(got).all()
+    bound = want.abs() * 2.0 ** -8 + group_bound(q, cache, table, lens).repeat_interleave(64, -1)
+    worst = ((got - want).abs() / bound.clamp(min=1e-300)).unflatten(-1, (-1, 64)).amax((0, 1, 3))
+    assert (worst <= 1.0).all(), f"of the bound, per group: {worst.tolist()}"
+
+
+@pytest.mark.parametrize("r", [0, 12, 16, 20, 26, 60, 100])
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 128), (4, 1, 256)])
+def test_a_small_group_beside_a_large_one(cuda, hq, hkv, d, r):
+    def change(cache, table):
+        cache[3][..., 1, :] *= 2.0 ** -r
+    check_groups(cuda, change, hq, hkv, d, [650, 33, 1], seed=r)
+    check_groups(cuda, change, hq, hkv, d, [3000, 700], seed=r, room=2000)
+
+
+@pytest.mark.parametrize("r", [18, 40, 110])
+def test_one_token_with_a_large_group(cuda, r):
+    """Its other group and all other tokens' are what they were."""
+    def change(cache, table):
+        cache[3][table[0, 0], :, 70, 0] *= 2.0 ** r
+        cache[3][table[1, 0], :, 5, 0] *= 2.0 ** r
+    check_groups(cuda, change, 8, 2, 128, [700, 40, 9], seed=r)
+
+
+@pytest.mark.parametrize("up", [True, False])
+def test_groups_that_grow_and_shrink_along_a_row(cuda, up):
+    """Every tile's first group 2^4 larger, its second 2^4 smaller than the tile's before."""
+    def change(cache, table):
+        size, n = 256, 640
+        step = (torch.arange(3 * size) // 32 - 10).clamp(-10, 10) * (4 if up else -4)
+        for i in range(3):
+            f = torch.exp2(step[i * size:(i + 1) * size].float())[None, :, None]
+            cache[3][table[0, i], :, :, 0] = (cache[3][table[0, i], :, :, 0].float() * f).to(BF)
+            cache[3][table[0, i], :, :, 1] = (cache[3][table[0, i], :, :, 1].float() / f).to(BF)
+    check_groups(cuda, change, 4, 2, 128, [640], seed=3)
+    check_groups(cuda, change, 1, 1, 128, [640], seed=4)
+
+
+@pytest.mark.parametrize("bad", [NAN, INF, -INF])
+@pytest.mark.parametrize("n", [20, 700, 9000])
+def test_a_value_that_is_not_a_number_is_its_groups_matter(cuda, n, bad):
+    g, hq, hkv, d = gen(n), 4, 2, 128
+    table, blocks = kh.block_lists(g, [n, n], 256)
+    cache = kh.make_cache(g, blocks, hkv, 256, d)
+    q = torch.randn(2, hq, d, generator=g).to(BF)
+    want, big = kh.decode(q, cache, table, [n, n], d ** -0.5)
+    t = n // 2
+    cache[3][table[1, t // 256], 1, t % 256, 0] = torch.tensor([abs(bad), 0.5 if bad == INF else bad]).to(BF)     # what a write makes of it
+    got = call(cuda, q, cache, table, [n, n])
+    assert not torch.isfinite(got[1, 2:, :64]).any()
+    others = torch.ones(2, hq, 2, dtype=torch.bool)
+    others[1, 2:, 0] = False
+    kh.assert_decode(got.unflatten(-1, (2, 64))[others], want.unflatten(-1, (2, 64))[others], big[..., None].expand(2, hq, 2)[others], "the other groups")
