@@ -188,7 +188,7 @@ struct Decode4Cut {
   __device__ __forceinline__ int of(int tile) const { return tile < rest * (per + 1) ? tile / (per + 1) : (tile - rest) / per; }
 };
 
-// a run of tiles of head h of sequence b (n tokens): its first token (behind the span's, with a list of spans) and which lane has its block
+// a run of tiles of head h of sequence b (n tokens): its first token (behind the span's, with a list of spans) and which lane has its block (none: -1)
 struct Decode4Run {
   int known, known_row, sel, token, tiles, b, h, n;
 };
@@ -210,6 +210,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const Decode4Para
   __shared__ int meta_s[NW][2][3];                           // a warp's parts: row (-1: none), the row's first tile and the one behind its last
   __shared__ Walk fs_s[NW], cs_s[NW];                        // a warp's fetching and computing side
   __shared__ Decode4Run run_s[NW];
+  __shared__ int before_s[NW];                               // entries that name a span in front of the known ones
   __shared__ __align__(16) float lse_s[2][kDecode4MaxGroup][NW];            // log2-sum-exps of the warps' first and last parts, -inf: none
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c4 = lane & 3;
@@ -331,7 +332,8 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const Decode4Para
   const uint32_t ring = smem_u32(smem) + warp * C::RING;
   int ft = w0;                                               // the next tile to fetch
   // A run: tiles that lie one behind the other in memory (of one block, or of one span).  Where the runs lie is known 32 at a time: lane i
-  // has the block of table column known + i or, with a list of spans, the first token and the block of its entry known + i.
+  // has the block of table column known + i or, with a list of spans, the first token and the block of its entry known + i (no token: the
+  // entry names no span of the sequence).  The i-th span of a row is the list's i-th entry that names one, wherever it stands.
   // What only changes from run to run is kept in shared memory.
   int u_block = -1, u_token = -1;
   if (lane == 0) { fs_s[warp] = cs; run_s[warp].known = 0; run_s[warp].known_row = -1; }
@@ -356,18 +358,28 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const Decode4Para
       }
     } else {
       constexpr int PER = kKv4Span / C::TOK;
-      const int row = fs.b * p.hkv + fs.h;
-      at = (fs.i - 1) / PER;
+      const int row = fs.b * p.hkv + fs.h, nth = (fs.i - 1) / PER;
       room = PER - (fs.i - 1) % PER;
       run_token = ((fs.i - 1) % PER) * C::TOK;
-      if (known_row != row || at >= known + 32) {
-        known = at; known_row = row;
-        const int span = at + lane < p.budget ? __ldg(p.spans + static_cast<int64_t>(row) * p.budget + at + lane) : -1;
+      int before = before_s[warp];
+      if (known_row != row) { known = -32; before = 0; u_token = -1; known_row = row; }
+      uint32_t named = __ballot_sync(FULL, u_token >= 0);
+      bool more = false;
+      while (nth >= before + __popc(named) && known + 32 < p.budget) {
+        before += __popc(named);
+        known += 32;
+        const int span = known + lane < p.budget ? __ldg(p.spans + static_cast<int64_t>(row) * p.budget + known + lane) : -1;
         const bool fits = span <= (fs.n - 1) / kKv4Span;
         if (!fits) report(p.dev_status, kDevBadLength, fs.b);
         u_token = span >= 0 && fits ? span * kKv4Span : -1;
-        u_block = u_token >= 0 ? __ldg(table + p.by_block.div(u_token)) : -1;
+        named = __ballot_sync(FULL, u_token >= 0);
+        more = true;
       }
+      if (more) {
+        u_block = u_token >= 0 ? __ldg(table + p.by_block.div(u_token)) : -1;
+        if (lane == 0) before_s[warp] = before;
+      }
+      at = known + __ffs(__ballot_sync(FULL, u_token >= 0 && __popc(named & ((1u << lane) - 1)) == nth - before)) - 1;    // (known - 1: there is none)
     }
     const int tiles = min(room, fs.count - fs.i), b = fs.b, h = fs.h, n = fs.n;
     fs.i += tiles - 1;
@@ -383,13 +395,13 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const Decode4Para
     if (ft < w1) {
       if (f_left == 0) {                                     // on to the run that look() found
         const Decode4Run run = run_s[warp];
-        const int block = __shfl_sync(FULL, u_block, run.sel);
+        const int block = __shfl_sync(FULL, u_block, run.sel & 31);
         f_token = run.token; f_left = run.tiles; f_n = run.n;
         bool ok = true;
         if (p.spans != nullptr) {
-          const int base = __shfl_sync(FULL, u_token, run.sel);
-          f_token += base;
-          ok = base >= 0;
+          const int base = __shfl_sync(FULL, u_token, run.sel & 31);
+          ok = run.sel >= 0 && base >= 0;
+          f_token = ok ? f_token + base : 0;
         }
         if (ok && (block < 0 || block >= p.num_blocks)) {
           if (lane == 0) report(p.dev_status, kDevBadBlock, run.b);

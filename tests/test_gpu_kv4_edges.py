@@ -115,3 +115,42 @@ def test_a_value_that_is_not_a_number_is_its_groups_matter(cuda, n, bad):
     others = torch.ones(2, hq, 2, dtype=torch.bool)
     others[1, 2:, 0] = False
     kh.assert_decode(got.unflatten(-1, (2, 64))[others], want.unflatten(-1, (2, 64))[others], big[..., None].expand(2, hq, 2)[others], "the other groups")
+
+
+# ---- lists of spans with gaps -------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("budget", [5, 31, 40, 100])
+@pytest.mark.parametrize("hq,hkv,d,size", [(8, 2, 128, 256), (2, 1, 256, 64), (8, 2, 64, 64)])
+def test_spans_behind_gaps(cuda, hq, hkv, d, size, budget):
+    """Entries below 0 anywhere in a list, more of them than the sequence has spans."""
+    g, lens = gen(budget), [1, 64, 100, 700, 0, 5000, 130, 1300]
+    spans = torch.full((len(lens), hkv, budget), -1, dtype=torch.int32)
+    for b, n in enumerate(lens):
+        count = -(-n // 64)
+        for h in range(hkv):
+            m = int(torch.randint(0, min(count, budget) + 1, (1,), generator=g))
+            at = torch.randperm(budget, generator=g)[:m]
+            spans[b, h, at] = torch.randperm(count, generator=g)[:m].int() if m else spans[b, h, at]
+    if budget == 5:
+        spans[2] = torch.tensor([-1, -1, 0, 1, -1])
+        spans[0] = torch.tensor([-1, -1, -1, -1, 0])
+    table, blocks = kh.block_lists(g, lens, size)
+    cache = kh.make_cache(g, blocks, hkv, size, d)
+    kh.poison(cache, table, lens, size)
+    q = torch.randn(len(lens), hq, d, generator=g).to(BF)
+    want, big = kh.decode(q, cache, table, lens, d ** -0.5, spans=spans)
+    for room in (None, 2000):
+        status = ops.new_status(cuda)
+        got = call(cuda, q, cache, table, lens, spans=spans, room=room, status=status)
+        ops.check_status(status)
+        kh.assert_decode(got, want, big, f"budget {budget}")
+
+
+def test_spans_outside_the_sequence_in_front_of_others(cuda):
+    g = gen(2)
+    table, blocks = kh.block_lists(g, [100], 64)
+    cache = kh.make_cache(g, blocks, 1, 64, 128)
+    q, spans = torch.randn(1, 2, 128, generator=g).to(BF), torch.tensor([[[9, 2, 1, 1 << 20, 0]]], dtype=torch.int32)
+    status = ops.new_status(cuda)
+    got = call(cuda, q, cache, table, [100], spans=spans, status=status)
+    assert status[0].item() == 5 and status[1].item() == 0
+    kh.assert_decode(got, *kh.decode(q, cache, table, [100], 128 ** -0.5), "both spans")
