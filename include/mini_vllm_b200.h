@@ -607,7 +607,8 @@ int mvb_row_norm_rope_kv_write(int dtype, void* q, int64_t q_row_stride, void* k
  *   head_dim / 64, 2], for each group of 64 channels of a row its (scale, minimum): code c stands for minimum + scale * c, with scale =
  *   bf16((greatest - least) * fp32(1/15)) and c = round((x - least) / scale) held to 0..15.  head_dim 64, 128 or 256; block_size a multiple
  *   of 64; 16-byte aligned; slots below 2^31.  Channel 8 L + e lies in bits 4 (e / 2) + 16 (e % 2) of a 32-bit word: word (D / 32) (L % 4) +
- *   L / 4 of a row of keys, word (D / 64) (L % 8) + L / 8 of a row of values.  Values are finite, with a spread inside a group that is too.
+ *   L / 4 of a row of keys, word (D / 64) (L % 8) + L / 8 of a row of values.  A group of values that are not all
+ *   finite, or whose spread is not, is read as values that are not: one NaN makes all 64 NaN.
  * mvb_rotary: the first rotary_dim (even) channels of every head of q [num_tokens, num_q_heads, head_dim] and k turned by the angles of
  *   cos_sin fp32 [max_pos, rotary_dim] (cosines, then sines): pairs (2i, 2i + 1) if interleaved, else (i, i + rotary_dim / 2); the others
  *   carried along.  *_out the same as q and k (in place) or apart from them.  dtype as elsewhere; num_q_heads or num_kv_heads 0: without.
@@ -627,7 +628,8 @@ int mvb_row_norm_rope_kv_write(int dtype, void* q, int64_t q_row_stride, void* k
  *   block_size / 64, 2, head_dim], least and greatest key per channel over the span's rows up to the step's last one.  The tokens of a
  *   sequence stand next to each other, in order.
  * mvb_kv4_select: per sequence and KV head the `budget` (>= 2) spans with the greatest sum over the group's heads and the channels of
- *   max(q least, q greatest), the first and the last span always among them, of equal sums the lower index; ascending, -1 behind them.
+ *   max(q least, q greatest), the first and the last span always among them, of equal sums the lower index, those that are not numbers
+ *   in front of all others; ascending, -1 behind them.
  *   max_tokens: the longest context that may come (at most 1048576, and what the table holds); a longer one is reported and cut there.
  */
 typedef struct mvb_kv4_cache {

@@ -2,6 +2,7 @@
 //
 // A row is one token's key (or value) of one KV head: D channels in groups of 64.  With m and M a group's least and greatest value,
 //     minimum m,   scale s = bf16((M - m) * fp32(1/15)),   code c = round((x - m) / s) held to 0..15,   the row stands for m + s c.
+// A value that is not finite makes m or s so: no channel of its group is read as a number that could pass for one.
 // Codes lie in [blocks, kv heads, block_size, D / 2] bytes, (s, m) as a bf16 pair in [blocks, kv heads, block_size, D / 64, 2]: a head's
 // tokens are contiguous inside a block, so 32 tokens of a head are one piece of memory.  4.5 bits a value, against 16.
 //

@@ -14,6 +14,18 @@
 
 namespace mvb {
 
+// of two numbers; of anything and what is not one, that
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
 struct SummariseParams {
   const uint32_t *k_codes, *k_affine;
   const int32_t* slots;
@@ -67,7 +79,7 @@ __global__ void __launch_bounds__(256) kv4_summarise_kernel(const SummariseParam
         float y[8];
         kv4_values(word[i], affine[i], y);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) { lo[e] = fminf(lo[e], y[e]); hi[e] = fmaxf(hi[e], y[e]); }
+        for (int e = 0; e < 8; ++e) { lo[e] = min_nan(lo[e], y[e]); hi[e] = max_nan(hi[e], y[e]); }
       }
     }
   }
@@ -75,8 +87,8 @@ __global__ void __launch_bounds__(256) kv4_summarise_kernel(const SummariseParam
   for (int off = LPH; off < 32; off <<= 1) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      lo[e] = fminf(lo[e], __shfl_xor_sync(FULL, lo[e], off));
-      hi[e] = fmaxf(hi[e], __shfl_xor_sync(FULL, hi[e], off));
+      lo[e] = min_nan(lo[e], __shfl_xor_sync(FULL, lo[e], off));
+      hi[e] = max_nan(hi[e], __shfl_xor_sync(FULL, hi[e], off));
     }
   }
   __nv_bfloat16* out = p.summaries + ((block * p.hkv + h) * (p.block_size / kKv4Span) + span) * (2 * D);
@@ -95,7 +107,7 @@ __global__ void __launch_bounds__(256) kv4_summarise_kernel(const SummariseParam
       const int side = i / D, e = i % D;
       float y = part_s[0][side][e];
 #pragma unroll
-      for (int w = 1; w < WARPS; ++w) y = side ? fmaxf(y, part_s[w][side][e]) : fminf(y, part_s[w][side][e]);
+      for (int w = 1; w < WARPS; ++w) y = side ? max_nan(y, part_s[w][side][e]) : min_nan(y, part_s[w][side][e]);
       out[i] = __float2bfloat16_rn(y);
     }
   }
@@ -117,8 +129,9 @@ constexpr int kSelectThreads = 256;
 constexpr int kSelectMaxSpans = 16384;       // keys of 8 bytes in shared memory: a context of 1 M tokens
 constexpr int kSelectMaxGroup = 8;
 
-// ascending with the sum, whatever its sign
+// ascending with the sum, whatever its sign; a sum that is not a number comes before all others, so that what made it is read
 __device__ __forceinline__ uint64_t order_key(double x) {
+  if (x != x) return ~0ull;
   const uint64_t b = static_cast<uint64_t>(__double_as_longlong(x));
   return (b >> 63) ? ~b : b | 0x8000000000000000ull;
 }

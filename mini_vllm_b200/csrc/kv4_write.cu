@@ -53,12 +53,13 @@ __device__ __forceinline__ uint32_t kv4_codes(const float2 (&t)[4], float s, flo
   return word - __float_as_uint(kRound) * kPlaces;           // modulo 2^32: the codes alone remain
 }
 
+// (what is not a number stays so: it has to reach the scale and the minimum)
 __device__ __forceinline__ uint32_t min_bf16x2(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 x = __hmin2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  const __nv_bfloat162 x = __hmin2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
   return *reinterpret_cast<const uint32_t*>(&x);
 }
 __device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 x = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  const __nv_bfloat162 x = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
   return *reinterpret_cast<const uint32_t*>(&x);
 }
 

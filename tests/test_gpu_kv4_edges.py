@@ -100,6 +100,32 @@ def test_groups_that_grow_and_shrink_along_a_row(cuda, up):
     check_groups(cuda, change, 1, 1, 128, [640], seed=4)
 
 
+# ---- what is not a number -------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("bad", [NAN, -NAN, INF, -INF])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_rows_that_are_not_numbers_stay_visible(cuda, d, bad):
+    """A NaN makes its whole group of 64 one; an infinity leaves no channel of its group finite.  Every other group is what it was."""
+    g, n, hkv = gen(d), 90, 2
+    x = torch.randn(n, 2 * hkv, d, generator=g).to(BF)
+    hit = torch.zeros(n, 2 * hkv, d // 64, dtype=torch.bool)
+    for t, h, c in ((0, 0, 0), (5, 1, d - 1), (6, 2, 17), (40, 3, d // 2), (89, 0, d - 7), (88, 2, 63)):
+        x[t, h, c] = bad
+        hit[t, h, c // 64] = True
+    cache = ops.KV4Cache.empty(2, 64, hkv, d, cuda)
+    slots, dev = torch.arange(n, dtype=torch.int32, device=cuda), x.to(cuda)
+    ops.rotary_kv4_write(None, dev[:, :hkv], dev[:, hkv:], None, None, slots, cache)
+    k, v = ops.kv4_gather(cache, torch.tensor([0, n], dtype=torch.int32, device=cuda), torch.tensor([[0, 1]], dtype=torch.int32, device=cuda), n)
+    got = torch.cat([k, v], 1).cpu().unflatten(-1, (-1, 64))
+    if bad != bad:
+        assert torch.isnan(got[hit]).all()
+    else:
+        assert not torch.isfinite(got[hit]).any()
+    clean = x.clone()
+    clean[~torch.isfinite(clean)] = 0
+    want = torch.cat([kh.stored(clean[:, :hkv], True, torch.float32), kh.stored(clean[:, hkv:], False, torch.float32)], 1).to(BF).unflatten(-1, (-1, 64))
+    assert torch.equal(got[~hit], want[~hit])
+
+
 @pytest.mark.parametrize("bad", [NAN, INF, -INF])
 @pytest.mark.parametrize("n", [20, 700, 9000])
 def test_a_value_that_is_not_a_number_is_its_groups_matter(cuda, n, bad):
@@ -115,6 +141,28 @@ def test_a_value_that_is_not_a_number_is_its_groups_matter(cuda, n, bad):
     others = torch.ones(2, hq, 2, dtype=torch.bool)
     others[1, 2:, 0] = False
     kh.assert_decode(got.unflatten(-1, (2, 64))[others], want.unflatten(-1, (2, 64))[others], big[..., None].expand(2, hq, 2)[others], "the other groups")
+
+
+def test_a_key_that_is_not_a_number_reaches_its_queries_and_is_chosen(cuda):
+    g, hq, hkv, d, n = gen(3), 4, 2, 128, 64 * 40
+    x = torch.randn(n, 2 * hkv, d, generator=g).to(BF)
+    x[64 * 17 + 3, 1, 100] = NAN                                    # a key of the second head
+    dev, slots = x.to(cuda), torch.arange(n, dtype=torch.int32, device=cuda)
+    cache = ops.KV4Cache.empty(n // 256, 256, hkv, d, cuda)
+    ops.rotary_kv4_write(None, dev[:, :hkv], dev[:, hkv:], None, None, slots, cache)
+    summaries = ops.kv4_summarise(cache, slots, ops.kv4_summaries(cache))
+    q = torch.randn(3, hq, d, generator=g).to(BF).to(cuda)
+    lens = torch.tensor([n, 64 * 17 + 3, n], dtype=torch.int32, device=cuda)             # (the second sequence ends in front of it)
+    table = torch.arange(n // 256, dtype=torch.int32, device=cuda).repeat(3, 1)
+    ws = ops.decode4_workspace(3, hq, hkv, d, cuda)
+    out = ops.decode_attn4(q, cache, lens, table, d ** -0.5, -1, ws)
+    nan = torch.isnan(out).all(-1).cpu()
+    assert nan.tolist() == [[False, False, True, True], [False] * 4, [False, False, True, True]] and not torch.isnan(out[nan.logical_not().to(cuda)]).any()
+    spans = ops.kv4_select(q[:1], summaries, lens[:1], table[:1], 256, 4).cpu()
+    assert 17 in spans[0, 1].tolist()
+    few = ops.kv4_summarise(cache, slots[64 * 17:64 * 17 + 64], ops.kv4_summaries(cache))    # by eight warps a span, as by one
+    assert torch.equal(few[4, :, 1].view(torch.int16), summaries[4, :, 1].view(torch.int16))
+    assert torch.isnan(summaries[4, 1, 1, :, 64:]).all() and not torch.isnan(summaries[4, 1, 1, :, :64]).any()
 
 
 # ---- lists of spans with gaps -------------------------------------------------------------------------------------------------------------
