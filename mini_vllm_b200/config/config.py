@@ -12,6 +12,7 @@ Gemma3, ``query_pre_attn_scalar``, ``sliding_window``, ``rope_local_base_freq``)
 from __future__ import annotations
 
 import logging
+import math
 import os
 from dataclasses import dataclass
 from types import SimpleNamespace
@@ -77,6 +78,7 @@ class Config:
                 self.hf_config = _flatten_hf(AutoConfig.from_pretrained(path))
         if self.dtype is not None:
             self.hf_config.dtype = self.dtype
+        _reach(self.hf_config, self.max_model_len)
         if self.eos_token_ids is None:
             eos = getattr(self.hf_config, "eos_token_id", None)
             if eos is None:
@@ -91,6 +93,18 @@ class Config:
             raise ValueError("decode_spans needs kv_cache_bits=4, and at least 2 spans (the first and the last one are always read)")
         if self.kv_cache_block_size % 128 != 0:
             raise ValueError("kv_cache_block_size must be a multiple of 128 (the prefill KV tile)")
+
+
+def _reach(hf, max_model_len: int) -> None:
+    """``max_position_embeddings`` as far as a scaled rotation goes: ``factor`` times the trained length.  Checkpoints with linear scaling mostly
+    give the scaled length already, so there the factor counts only as far as ``max_model_len`` asks for it."""
+    scaling, most = getattr(hf, "rope_scaling", None), getattr(hf, "max_position_embeddings", None)
+    if not isinstance(scaling, dict) or most is None or _rope_kind(scaling) == "default":
+        return
+    if scaling.get("original_max_position_embeddings") is None:
+        hf.rope_scaling = scaling = {**scaling, "original_max_position_embeddings": most}
+    far = math.ceil(float(scaling["factor"]) * scaling["original_max_position_embeddings"])
+    hf.max_position_embeddings = max(most, min(far, max_model_len) if _rope_kind(scaling) == "linear" else far)
 
 
 def _rope_kind(parameters) -> str:

@@ -37,11 +37,23 @@ class Engine:
         self.scheduler = Scheduler(config)
         self.metrics = Metrics()
 
-    def submit(self, tokens: list[int], sampling_params: SamplingParams) -> Request:
-        limit = getattr(getattr(self.config, "hf_config", None), "learned_positions", None)      # a position table has an end (the last token needs none)
+    def _check_length(self, tokens: list[int], sampling_params: SamplingParams) -> None:
+        """Position tables have an end (the last token needs no position)."""
+        limit = getattr(getattr(self.config, "hf_config", None), "learned_positions", None)
         if limit is not None and len(tokens) + sampling_params.max_tokens - 1 > limit:
             raise ValueError(f"{len(tokens)} prompt tokens and {sampling_params.max_tokens} new ones need more than the model's "
                              f"{limit} positions")
+        # so have a rotation's; a request that may stop in front of it is taken
+        limit = getattr(getattr(self, "executor", None), "max_positions", None)
+        if limit is None:
+            return
+        stops = bool(self.config.eos_token_ids) and not sampling_params.ignore_eos
+        if len(tokens) + (0 if stops else sampling_params.max_tokens - 1) > limit:
+            raise ValueError(f"{len(tokens)} prompt tokens and {sampling_params.max_tokens} new ones need more than the {limit} positions "
+                             "that the model's rotation reaches")
+
+    def submit(self, tokens: list[int], sampling_params: SamplingParams) -> Request:
+        self._check_length(tokens, sampling_params)
         req = Request(tokens, sampling_params)
         self.scheduler.submit(req)
         return req
@@ -190,6 +202,8 @@ class Engine:
     def generate(self, prompts: list[list[int]], sampling_params, use_tqdm: bool = True) -> list[dict]:
         if not isinstance(sampling_params, list):
             sampling_params = [sampling_params] * len(prompts)
+        for prompt, sp in zip(prompts, sampling_params):       # (all of them before the first is taken)
+            self._check_length(prompt, sp)
         reqs = [self.submit(prompt, sp) for prompt, sp in zip(prompts, sampling_params)]
         if not use_tqdm and self._schedule_is_token_independent(sampling_params):
             self._generate_pipelined(reqs)

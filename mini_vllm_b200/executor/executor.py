@@ -17,6 +17,7 @@ import torch
 
 from .. import ops
 from ..engine.request import Request
+from ..models.layers.rotary import RotaryEmbedding
 from ..models.layers.sampler import Sampler
 from ..models.loader import load_model
 from ..scheduler.batch import Batch
@@ -78,6 +79,8 @@ class Executor:
             config.num_state_slots = None
         self.attention_layers = [m for m in self.model.modules() if hasattr(m, "k_cache") and hasattr(m, "v_cache")]
         self.latent_layers = [m for m in self.model.modules() if hasattr(m, "latent_cache")]     # (those with latents of their own)
+        # positions that every rotation's table has; None: nothing is rotated
+        self.max_positions = min((m.max_position_embeddings for m in self.model.modules() if isinstance(m, RotaryEmbedding)), default=None)
         self.item_rows = 0                     # query-block size of the prefill kernel's work items for this model
         for m in (self.attention_layers + self.latent_layers)[:1]:
             # (a head layout the kernel does not take: no list, the plain grid)
