@@ -157,7 +157,7 @@ class Executor:
         layers, cfg = self.attention_layers, self.config
         if not layers or self.latent_layers or self.recurrent or not all(m.takes_kv4(cfg.hf_config.dtype) for m in layers):
             raise ValueError("kv_cache_bits=4 needs bf16 attention layers of 128 or 256 channels a head throughout, without sinks, biases by "
-                             "distance, kept tokens, gates or borrowed keys")
+                             "distance, kept tokens, head gates, norms beside the rotation or borrowed keys")
         tokens = sum(ops.KV4Cache.token_bytes(m.num_kv_heads, m.head_dim) for m in layers) * self.block_size
         bounds = sum(m.num_kv_heads * (self.block_size // 64) * 4 * m.head_dim for m in layers if m.window_left < 0)
         return tokens + (bounds if cfg.decode_spans else 0)

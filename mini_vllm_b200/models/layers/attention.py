@@ -84,6 +84,7 @@ class FlashAttention(nn.Module):
         self.sinks = self.slopes = None   # fp32 [num_heads] each, set by whoever owns them
         self.__dict__["source"] = source  # (not a submodule of this one)
         self.lends = False                # some later layer reads this one's keys and values
+        self.dressed = False              # whoever owns it hands ``forward_fused`` norms or a head gate
         # in the caches' place, one in 4 bits; with decode_spans > 0 also the bounds of its spans of 64 tokens: a decode step then reads only so
         # many of them per sequence and KV head (layers without a window)
         self.kv4: ops.KV4Cache | None = None
@@ -116,7 +117,7 @@ class FlashAttention(nn.Module):
     def takes_kv4(self, dtype: torch.dtype) -> bool:
         """Whether a cache in 4 bits can stand in for this layer's keys and values."""
         return (dtype == torch.bfloat16 and self.head_dim in (128, 256) and self.num_heads <= 8 * self.num_kv_heads and
-                self.source is None and not self.lends and self._extras(None) is None)
+                self.source is None and not self.lends and not self.dressed and self._extras(None) is None)
 
     def _write_kv4(self, ctx: Context, q, k, v, positions, cos_sin) -> None:
         if self._extras(None) is not None or self.lends:

@@ -127,6 +127,7 @@ class AttentionBranch(Branch):
         self.attn = FlashAttention(heads, padded, scale, kv_heads, (-1 if window is None else window - 1, -1),
                                    softcap=softcap or 0.0, out_scale=factor, keep_first=keep_first,
                                    source=None if source is None else source.attn)
+        self.attn.dressed = gate == "head" or norm_eps is not None or row_eps is not None
         if sink is not None:
             self.attn.sinks = weight_f32(heads)
         if slopes is not None:
