@@ -50,6 +50,9 @@ class Config:
     # extension (with kv_cache_bits=4): a decode step reads this many spans of 64 tokens per sequence and KV head, those whose bounds promise the
     # greatest scores, in layers without a window (None: all tokens)
     decode_spans: Optional[int] = None
+    # with kv_cache_bits=4: context tokens that the prompts of a step may have together, for which the executor keeps memory to unpack them (it sets
+    # this; a single prompt may always come)
+    max_prompt_keys: Optional[int] = None
     num_state_slots: Optional[int] = None    # recurrent models: sequences that can hold state (None: max_num_batched_seqs)
 
     # executor

@@ -131,7 +131,10 @@ class Executor:
         if kv4:
             block_bytes = self._kv4_block_bytes()
         room = int(total * cfg.gpu_memory_utilization - (total - free) - peak + current)
-        fit = room // block_bytes if block_bytes else cfg.kv_cache_num_blocks
+        if kv4:
+            fit, cfg.max_prompt_keys = self._kv4_blocks_and_keys(room, block_bytes)
+        else:
+            fit = room // block_bytes if block_bytes else cfg.kv_cache_num_blocks
         if fit <= 0:
             raise RuntimeError("no memory left for the KV cache")
         cfg.kv_cache_num_blocks = min(fit, cfg.kv_cache_num_blocks)
@@ -161,6 +164,22 @@ class Executor:
         tokens = sum(ops.KV4Cache.token_bytes(m.num_kv_heads, m.head_dim) for m in layers) * self.block_size
         bounds = sum(m.num_kv_heads * (self.block_size // 64) * 4 * m.head_dim for m in layers if m.window_left < 0)
         return tokens + (bounds if cfg.decode_spans else 0)
+
+    def _kv4_blocks_and_keys(self, room: int, block_bytes: int) -> tuple[int, int]:
+        """How many blocks fit beside the memory that a step's prompts take to unpack their contexts, layer by layer, and how many context tokens
+        that memory is for: those of one context as long as the pool or the rotation's tables let it become, and no fewer than a step's tokens."""
+        cfg, size = self.config, self.block_size
+        row_bytes = max(4 * m.num_kv_heads * m.head_dim for m in self.attention_layers)              # a bf16 key and value of each head
+        longest = cfg.kv_cache_num_blocks * size if self.max_positions is None else self.max_positions
+
+        def keys(blocks: int) -> int:
+            return max(cfg.max_num_batched_tokens, min(longest, blocks * size))
+
+        low, high = 0, cfg.kv_cache_num_blocks                        # the most blocks with blocks * block_bytes + keys * row_bytes <= room
+        while low < high:
+            mid = (low + high + 1) // 2
+            low, high = (mid, high) if mid * block_bytes + keys(mid) * row_bytes <= room else (low, mid - 1)
+        return low, keys(low)
 
     def _bind_kv4(self) -> None:
         """One cache in 4 bits per layer, all of the same number of blocks, served by the same block tables."""

@@ -32,6 +32,8 @@ class Scheduler:
     def __init__(self, config):
         self.max_num_batched_seqs = config.max_num_batched_seqs
         self.max_num_batched_tokens = config.max_num_batched_tokens
+        # context tokens that the prompts of a step may have together; with whole prompts the token budget, which counts cached ones too, is the bound
+        self.max_prompt_keys = getattr(config, "max_prompt_keys", None)
         self.eos_token_ids = config.eos_token_ids
         self.mixed_steps = bool(getattr(config, "enable_mixed_steps", False))
         self.chunked = bool(getattr(config, "enable_chunked_prefill", False))
@@ -76,11 +78,16 @@ class Scheduler:
 
     def _schedule_portions(self, max_seqs: int, budget: int):
         """Chunked prefill: fill the token budget with the rest of prompts under way, then with new ones."""
-        bm, picked, total = self.block_manager, [], 0
+        bm, picked, total, keys = self.block_manager, [], 0, 0
+        # a request's context after its portion at most (a waiting one's cached prefix is not known yet)
+        fits = lambda req, cached: (not picked or self.max_prompt_keys is None or
+                                    keys + min(len(req.tokens), cached + budget) <= self.max_prompt_keys)
         while len(picked) < max_seqs and budget > 0:
             if len(picked) < len(self.prefilling):
                 req = self.prefilling[len(picked)]
-            elif self.waiting and bm.can_allocate_new_block(self.waiting[0]):
+                if not fits(req, req.num_cached_tokens):
+                    break
+            elif self.waiting and fits(self.waiting[0], len(self.waiting[0].tokens) if bm.support_prefix_cache else 0) and bm.can_allocate_new_block(self.waiting[0]):
                 req = self.waiting.popleft()
                 bm.allocate_blocks_for_prefill(req)
                 req.state = Request.RUNNING
@@ -91,6 +98,7 @@ class Scheduler:
             req.portion_end = req.num_cached_tokens + portion
             budget -= portion
             total += portion
+            keys += req.portion_end
             picked.append(req)
         if not picked:
             return None
