@@ -614,8 +614,8 @@ int mvb_row_norm_rope_kv_write(int dtype, void* q, int64_t q_row_stride, void* k
  *   carried along.  *_out the same as q and k (in place) or apart from them.  dtype as elsewhere; num_q_heads or num_kv_heads 0: without.
  *   A position outside the table is reported and its token left unturned.
  * mvb_rotary_kv4_write: bf16; q turned into q_out (may be q; num_q_heads 0: none), k turned and quantised, v quantised, into slot
- *   slot_mapping[token] (-1: not cached); k_in_place: k is turned in place too.  cos_sin NULL: nothing is turned.  rotary_dim a multiple
- *   of 16.  A slot given twice in one call: either token's row.
+ *   slot_mapping[token] (-1: not cached); k_in_place: k is turned in place too, and v lies apart from it.  cos_sin NULL: nothing is
+ *   turned.  rotary_dim a multiple of 16.  Slots are distinct: one given twice in a call holds parts of both rows.
  * mvb_kv4_gather: the cached rows of sequence b, tokens 0 .. cu_seqlens_k[b + 1] - cu_seqlens_k[b], as dense bf16 rows k_out, v_out
  *   [num_rows, num_kv_heads, head_dim] from row cu_seqlens_k[b] on; rows behind the last sequence stay as they are; a block id outside the
  *   pool is reported and reads as zeros.

@@ -269,6 +269,7 @@ extern "C" int mvb_rotary_kv4_write(const void* q, int64_t q_row_stride, void* q
     if (rotary_dim > d || rotary_dim % 16 != 0) return kUnsupportedShape;
   }
   if (num_tokens == 0) return kOk;
+  if (k == v && k_in_place && cos_sin != nullptr) return kInvalidArgument;   // (values are read by other warps than those that turn the keys)
   if (!k || !v || !slot_mapping || (num_q_heads > 0 && (!q || !q_out))) return kInvalidArgument;
   if ((num_q_heads > 0 && (q_row_stride % 8 || q_out_row_stride % 8)) || k_row_stride % 8 || v_row_stride % 8) return kMisaligned;
   if (!is_aligned(k, 16) || !is_aligned(v, 16) || !is_aligned(cos_sin, 16) || (num_q_heads > 0 && (!is_aligned(q, 16) || !is_aligned(q_out, 16))))

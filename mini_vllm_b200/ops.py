@@ -1374,7 +1374,7 @@ def rotary_kv4_write(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, p
                      slot_mapping: torch.Tensor, cache: KV4Cache, interleaved: bool = False, q_out: torch.Tensor | None = None,
                      k_in_place: bool = False, status: torch.Tensor | None = None) -> torch.Tensor | None:
     """Turns ``q`` (in place or into ``q_out``) and ``k`` as ``rotary`` does, and writes ``k`` and ``v`` in 4 bits to their cache slots
-    (-1: none); ``k_in_place``: the turned k also goes back to ``k``.  ``cos_sin`` None: nothing is turned.  bf16; the rotated channels a
+    (-1: none; each slot once); ``k_in_place``: the turned k also goes back to ``k``, and ``v`` lies apart from it.  ``cos_sin`` None: nothing is turned.  bf16; the rotated channels a
     multiple of 16.  Returns the turned q."""
     if q is None and q_out is not None:
         raise ValueError("q_out needs q")
