@@ -1220,7 +1220,7 @@ def _rows(t: torch.Tensor, dtype, device: int, shape: tuple, name: str) -> int:
     if t.dtype is dtype and t.get_device() == device and t.shape == shape:
         s = t.stride()
         if s[2] == 1 and (s[1] == shape[2] or shape[1] == 1) or t.numel() == 0:
-            return s[0]
+            return s[0] if shape[0] > 1 else shape[1] * shape[2]               # (no row lies behind a single one, whatever its stride)
     return _explain(t, dtype, device, name, f"[tokens, heads, head_dim] = {tuple(shape)} with contiguous heads")
 
 

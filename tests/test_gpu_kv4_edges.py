@@ -202,3 +202,24 @@ def test_spans_outside_the_sequence_in_front_of_others(cuda):
     got = call(cuda, q, cache, table, [100], spans=spans, status=status)
     assert status[0].item() == 5 and status[1].item() == 0
     kh.assert_decode(got, *kh.decode(q, cache, table, [100], 128 ** -0.5), "both spans")
+
+
+# ---- single rows ----------------------------------------------------------------------------------------------------------------------
+def test_a_single_row_of_any_stride(cuda):
+    """One token cut out of rows whose length is no multiple of eight: its own stride leads nowhere."""
+    g, hq, hkv, d = gen(1), 4, 2, 128
+    odd = torch.zeros(3, (hq + 2 * hkv) * d + 3, dtype=BF, device=cuda)
+    odd[0, :-3] = torch.randn((hq + 2 * hkv) * d, generator=g).to(BF)
+    q, k, v = (odd.as_strided((1, h, d), (odd.stride(0), d, 1), at * d) for h, at in ((hq, 0), (hkv, hq), (hkv, hq + hkv)))
+    assert q.stride(0) % 8 and q.shape == (1, hq, d)
+    slots, table, lens = torch.zeros(1, dtype=torch.int32, device=cuda), torch.zeros(1, 1, dtype=torch.int32, device=cuda), torch.ones(1, dtype=torch.int32, device=cuda)
+    pos, cos, ws = torch.ones(1, dtype=torch.int64, device=cuda), torch.randn(2, d, generator=g).to(cuda), ops.decode4_workspace(1, hq, hkv, d, cuda)
+    got = []
+    for rows in ((q, k, v), (q.contiguous().clone(), k.contiguous(), v.contiguous())):
+        cache = ops.KV4Cache.empty(1, 256, hkv, d, cuda)
+        out = ops.rotary_kv4_write(*rows, pos, cos, slots, cache, q_out=torch.empty_strided((1, hq, d), (hq * d + 1, d, 1), dtype=BF, device=cuda))
+        summaries = ops.kv4_summarise(cache, slots, ops.kv4_summaries(cache))
+        spans = ops.kv4_select(out, summaries, lens, table, 256, 2)
+        got.append((out, spans, ops.decode_attn4(out, cache, lens, table, 1.0, -1, ws, spans=spans), ops.rotary(rows[0], None, pos, cos)[0]))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
