@@ -1264,6 +1264,7 @@ def _need_shape(ok: bool, what: str) -> None:
 
 
 _BIG = 1 << 62
+_INT = (1 << 31) - 1                   # a C int, which a longer window or context would wrap around in
 
 
 def rotary(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tensor, cos_sin: torch.Tensor, interleaved: bool = False,
@@ -1461,7 +1462,7 @@ def decode_attn4(q: torch.Tensor, cache: KV4Cache, cache_seqlens: torch.Tensor, 
         spans_ptr = _dense(spans, i32, device, (B, hkv, budget), "spans")
     ws_ptr = _numbers(workspace, torch.uint8, device, 0, _BIG, "workspace")
     rc = _cabi.load().mvb_decode_attn4(q.data_ptr(), q_stride, cache.struct(device), lens_ptr, table_ptr, stride, width, spans_ptr, budget, B, hq,
-                                       float(scale), window_left, float(softcap), float(out_scale), out.data_ptr(), out_stride, ws_ptr, workspace.numel(),
+                                       float(scale), min(window_left, _INT), float(softcap), float(out_scale), out.data_ptr(), out_stride, ws_ptr, workspace.numel(),
                                        _status(status, device), _stream())
     if rc:
         _cabi.check(rc, "mvb_decode_attn4")
@@ -1507,7 +1508,7 @@ def kv4_select(q: torch.Tensor, summaries: torch.Tensor, cache_seqlens: torch.Te
     if out is None:
         out = torch.empty((B, hkv, max(budget, 0)), dtype=torch.int32, device=q.device)
     rc = _cabi.load().mvb_kv4_select(q.data_ptr(), q_stride, sum_ptr, blocks, block_size, lens_ptr, table_ptr, stride, width, B, hq, hkv, d,
-                                     width * block_size if max_context is None else max_context, budget,
+                                     min(width * block_size if max_context is None else max_context, _INT), budget,
                                      _dense(out, torch.int32, device, (B, hkv, max(budget, 0)), "out"), _status(status, device), _stream())
     if rc:
         _cabi.check(rc, "mvb_kv4_select")

@@ -223,3 +223,17 @@ def test_a_single_row_of_any_stride(cuda):
         got.append((out, spans, ops.decode_attn4(out, cache, lens, table, 1.0, -1, ws, spans=spans), ops.rotary(rows[0], None, pos, cos)[0]))
     for a, b in zip(*got):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("far", [2 ** 31 - 1, 2 ** 32 + 64, 2 ** 63 - 1])
+def test_windows_and_contexts_beyond_32_bits(cuda, far):
+    """As long as can be, not what is left of them in 32 bits."""
+    g, lens, hq, hkv, d = gen(5), [3000, 64, 2600], 4, 2, 128
+    table, blocks = kh.block_lists(g, lens, 256)
+    cache = kh.make_cache(g, blocks, hkv, 256, d)
+    q = torch.randn(3, hq, d, generator=g).to(BF)
+    assert torch.equal(call(cuda, q, cache, table, lens, window=far), call(cuda, q, cache, table, lens))
+    status, summaries = ops.new_status(cuda), torch.randn(blocks, hkv, 4, 2, d, generator=g).to(BF).sort(3).values
+    got = ops.kv4_select(q.to(cuda), summaries.to(cuda), torch.tensor(lens, dtype=torch.int32, device=cuda), table.to(cuda), 256, 5, status=status, max_context=far)
+    ops.check_status(status)
+    assert torch.equal(got.cpu(), kh.select(q, summaries, table, lens, 5))
