@@ -237,3 +237,53 @@ def test_windows_and_contexts_beyond_32_bits(cuda, far):
     got = ops.kv4_select(q.to(cuda), summaries.to(cuda), torch.tensor(lens, dtype=torch.int32, device=cuda), table.to(cuda), 256, 5, status=status, max_context=far)
     ops.check_status(status)
     assert torch.equal(got.cpu(), kh.select(q, summaries, table, lens, 5))
+
+
+# ---- every tile counts ------------------------------------------------------------------------------------------------------------------
+def tile_marks(cache, table, lens, size, d):
+    """Values that say where they come from: channel c is 1 in the tiles of 32 tokens whose number leaves c when divided by d, else 0."""
+    t = torch.arange(table.shape[1] * size)
+    one = torch.nn.functional.one_hot(t // 32 % d, d).to(BF)
+    codes, affine = kh.quantise(one, False)
+    for b, n in enumerate(lens):
+        for i in range(-(-n // size)):
+            cache[2][table[b, i]], cache[3][table[b, i]] = codes[i * size:(i + 1) * size], affine[i * size:(i + 1) * size]
+
+
+@pytest.mark.parametrize("lens,room", [([9000], None), ([9000], 2000), ([40000], None), ([40000], 2000), ([9000, 3, 700, 0, 4000, 31], None),
+                                       ([9000, 3, 700, 0, 4000, 31], 2000), ([2500 + 33 * i for i in range(12)], 2000)])
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 128), (16, 8, 128), (2, 1, 256), (2, 2, 64)])
+def test_every_tile_counts_once(cuda, hq, hkv, d, lens, room):
+    """A channel's output is the weight of its few tiles, and has to be right as a number of that size.  All values are 0 or 1, so each error is
+    relative: a weight's rounding 2^-11, scores good to 2^-14 twice (numerator and sum), the rounding of the output 2^-8."""
+    g, size = gen(len(lens)), 256
+    table, blocks = kh.block_lists(g, lens, size)
+    cache = kh.make_cache(g, blocks, hkv, size, d)
+    tile_marks(cache, table, lens, size, d)
+    kh.poison(cache, table, lens, size)
+    q = (torch.randn(len(lens), hq, d, generator=g) * 0.25).to(BF)
+    q[:, 0] = 0                                                     # a head whose weights are all alike
+    for window in (-1, 2600):
+        got, (want, _) = call(cuda, q, cache, table, lens, window=window, room=room), kh.decode(q, cache, table, lens, d ** -0.5, window)
+        worst = ((got - want).abs() / want.clamp(min=1e-300))[want > 0].max() / (2.0 ** -8 + 2.0 ** -10 + 2.0 ** -12)
+        assert worst <= 1.0 and (got[want == 0] == 0).all(), f"window {window}: {worst:.3f}"
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(16, 8, 128), (2, 1, 256), (2, 2, 64)])
+def test_every_tile_of_a_list_counts_once(cuda, hq, hkv, d):
+    g, lens, size, budget = gen(d), [9000, 64, 3000, 12000], 256, 70
+    table, blocks = kh.block_lists(g, lens, size)
+    cache = kh.make_cache(g, blocks, hkv, size, d)
+    tile_marks(cache, table, lens, size, d)
+    kh.poison(cache, table, lens, size)
+    spans = torch.full((len(lens), hkv, budget), -1, dtype=torch.int32)
+    for b, n in enumerate(lens):
+        for h in range(hkv):
+            chosen = torch.randperm(-(-n // 64), generator=g)[:budget - 9 * h % 20]
+            spans[b, h, torch.randperm(budget, generator=g)[:len(chosen)]] = chosen.int()
+    q = (torch.randn(len(lens), hq, d, generator=g) * 0.25).to(BF)
+    want, _ = kh.decode(q, cache, table, lens, d ** -0.5, spans=spans)
+    for room in (None, 2000):
+        got = call(cuda, q, cache, table, lens, spans=spans, room=room)
+        worst = ((got - want).abs() / want.clamp(min=1e-300))[want > 0].max() / (2.0 ** -8 + 2.0 ** -10 + 2.0 ** -12)
+        assert worst <= 1.0 and (got[want == 0] == 0).all(), f"{worst:.3f}"
