@@ -620,8 +620,9 @@ int mvb_row_norm_rope_kv_write(int dtype, void* q, int64_t q_row_stride, void* k
  *   [num_rows, num_kv_heads, head_dim] from row cu_seqlens_k[b] on; rows behind the last sequence stay as they are; a block id outside the
  *   pool is reported and reads as zeros.
  * mvb_decode_attn4: one query token per sequence over its cache_seqlens cached tokens, as mvb_decode_attn_capped; num_q_heads <= 8 *
- *   num_kv_heads.  spans (NULL: all tokens): int32 [num_seqs, num_kv_heads, budget], the 64-token spans that a head's queries read, each once;
- *   entries below 0, wherever they stand, and spans behind the sequence's last (reported) are skipped (not with a window).  A sequence of no tokens, or none that is read, gives zeros.  workspace of
+ *   num_kv_heads; q below 2^118 in size.  spans (NULL: all tokens): int32 [num_seqs, num_kv_heads, budget], the 64-token spans that a
+ *   head's queries read, each once (not with a window); entries below 0, wherever they stand, and spans behind the sequence's last
+ *   (reported) are skipped.  A sequence of no tokens, or none that is read, gives zeros.  workspace of
  *   mvb_decode_attn4_workspace_bytes, 256-byte aligned, zeroed once by the caller and left zeroed where it has to be; calls that share it
  *   must not overlap.  out lies apart from q.
  * mvb_kv4_summarise: bounds of the keys of the spans that a step's tokens were written to: summaries bf16 [num_blocks, num_kv_heads,

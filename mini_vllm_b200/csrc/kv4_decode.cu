@@ -495,6 +495,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const Decode4Para
           qf[j][e] = pack_f16(x * less, y * less);
         }
       }
+      // (a factor that fp32 holds: from 2^118 on, scores come out smaller than they are)
       const float f = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(min(127 + 24 - up, 254)) << 23);
 #pragma unroll
       for (int j = 0; j < GRP; ++j) {
