@@ -17,9 +17,10 @@
 // that a warp's sum of p m is finite too, for 16 K tokens of the largest values there are).  A rounding of p s meets the codes, up to 15 of them, while p m is exact: next to the plain form's error that is
 // 2^-11 sum p (15 s) more at most.
 //
-// On paper bound by memory: a tile of 32 tokens of a 128-wide head is 4608 bytes.  Its 655 warp instructions, most of them on the integer
-// pipe, bring instruction issue near: 240 sequences of 128-8192 tokens, 16 heads on 8, 0.51 GB in 114 us, 4.5 TB/s (0.69 of what a copy reaches),
-// 64 % of the issue slots, the integer pipe at 60 %.  A few rows are bound by the chain of dependent loads (lengths, block lists, tiles, parts):
+// On paper bound by memory: a tile of 32 tokens of a 128-wide head is 4608 bytes.  Its 650 warp instructions, most of them on the integer
+// pipe, bring instruction issue near: 240 sequences of 128-8192 tokens, 16 heads on 8, 0.51 GB in 115 us, 4.4 TB/s (0.68 of what a copy reaches),
+// 62 % of the issue slots, the integer pipe at 59 %.  Neither is at its limit: four warps a scheduler, at 128 registers with 156 bytes of them
+// spilled, do not cover each other's waits, and more do not fit.  A few rows are bound by the chain of dependent loads (lengths, block lists, tiles, parts):
 // one context of 700 tokens 10 us.
 //
 // Work is tiles of 32 tokens of one (sequence, head), numbered sequence by sequence and head by head.  Each CTA takes a contiguous range (all
@@ -45,7 +46,7 @@ template <int D, int W>
 struct Decode4Cfg {
   static constexpr int TOK = 32;                             // tokens of a tile
   static constexpr int NW = W;                               // warps of a CTA
-  static constexpr int NST = 2;                              // tiles in a warp's ring, one of them being computed (three: 113 us instead of 111 for the ragged batch)
+  static constexpr int NST = 2;                              // tiles in a warp's ring, one of them being computed (three: 113 us instead of 111 for the ragged batch, when that took 111)
   static constexpr int CODES = TOK * D / 2, AFF = TOK * D / 16;
   static constexpr int STAGE = 2 * CODES + 2 * AFF;          // key codes, value codes, key affine, value affine
   static constexpr int RING = NST * STAGE;
@@ -252,8 +253,8 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const Decode4Para
   }
   // Few rows: whole CTAs for each of them, in proportion to its tiles but one for a row of up to three tiles a warp, so that a CTA works on one
   // row and most need no other CTA.  Where some CTA would get much more than its share, or there are more rows than CTAs: the even cut.
-  // (Cut evenly and by rows: 8 rows of 22 tiles, sixteen warps, 15.4 and 11.8 us; 128 rows of up to 17 tiles of 256-wide heads 18.9 and 13.7; 8 rows
-  // of 1280, sixteen warps, 30.5 and 24.8.)
+  // (Cut evenly and by rows: 8 rows of 22 tiles 12.7 and 10.3 us, with sixteen warps 17.9 and 13.2; 128 rows of up to 17 tiles of 256-wide heads
+  // 17.3 and 14.4; 8 rows of 1280 25.3 and 22.1, with sixteen warps 30.2 and 26.6.)
   const int grid = gridDim.x, share = (total + grid - 1) / grid;
   const float part_of_grid = static_cast<float>(grid) / static_cast<float>(max(total, 1));
   auto ctas_of = [&](int v) -> int {                         // (a tile a warp at least: no CTA is left without one)
@@ -973,10 +974,10 @@ extern "C" int mvb_decode_attn4(const void* q, int64_t q_row_stride, const mvb_k
   const int grid = sm_count() < kDecode4MaxCtas ? sm_count() : kDecode4MaxCtas;
   // Sixteen warps keep an SM's pipes busier, eight have twice the registers and are quicker from the first load to the last part (and take a
   // shorter row by themselves): eight up to 200 tiles an SM (80 of 64-wide heads), as far as the call can tell; always eight for heads of 256,
-  // whose fragments need the registers.  8 heads of 128, sixteen and eight: 1 context of 700 tokens 11.7 and 9.4 us, of 40000 21.7 and 19.4, 32 of
-  // 1000 22.2 and 19.7, 32 of 4000 39.1 and 38.7, 4 of 40000 45.3 and 47.1, 64 of 4000 61 and 65.  2 heads of 64: 1 of 40000 16.8 and 13.8, 32 of
-  // 4000 16.6 and 16.3, 16 of 16000 20.2 and 21.1.  Lists of spans, a run of loads more for every two tiles, half of that: 8 heads of 128, 64 spans
-  // for 1 sequence 14.1 and 11.2, 16 for 48 27.4 and 25.5, 16 for 96 38.4 and 39.9, 64 for 64 73 and 81
+  // whose fragments need the registers.  8 heads of 128, sixteen and eight: 1 context of 700 tokens 12.9 and 10.2 us, of 40000 23.6 and 19.9, 32 of
+  // 1000 23.8 and 19.8, 32 of 4000 41.3 and 39.7, 4 of 40000 48.0 and 46.5, 16 of 16000 63 and 66, 64 of 4000 63 and 66.  2 heads of 64: 1 of 40000 17.0
+  // and 13.9, 32 of 4000 17.1 and 17.7, 16 of 16000 21.4 and 22.0.  Lists of spans, a run of loads more for every two tiles, half of that: 8 heads of
+  // 128, 64 spans for 1 sequence 16.1 and 11.8, 16 for 48 30.4 and 27.0, 16 for 96 41.4 and 41.8, 64 for 64 77 and 86
   int64_t most = longest * cache->block_size / 32 + 1;       // tiles of a row
   if (window_left >= 0 && (static_cast<int64_t>(window_left) + 1) / 32 + 2 < most) most = (static_cast<int64_t>(window_left) + 1) / 32 + 2;
   if (spans != nullptr && static_cast<int64_t>(budget) * (kKv4Span / 32) < most) most = static_cast<int64_t>(budget) * (kKv4Span / 32);
