@@ -102,11 +102,11 @@ __device__ __forceinline__ float fast_log2(float x) {
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Powers of two, as their exponents say: of a whole number (0 below 2^-126, at most 2^127; of one that is not a number 0), one over 2^-126 .. 2^126,
+// Powers of two, as their exponents say: of a whole number (0 below 2^-126, at most 2^127, and that of what is no number: nothing has been added up then), one over 2^-126 .. 2^126,
 // and what brings the greatest of a group's weights to 2^8 .. 2^9
 constexpr float kMostUp = 0x1p126f;
 __device__ __forceinline__ float pow2_whole(float x) {
-  return __uint_as_float(static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(x, -127.f), 127.f)) + 127) << 23);
+  return __uint_as_float(static_cast<uint32_t>(static_cast<int>(fmaxf(fminf(x, 127.f), -127.f)) + 127) << 23);
 }
 __device__ __forceinline__ float pow2_inverse(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
 __device__ __forceinline__ float up_for(float most) {

@@ -100,6 +100,23 @@ def test_groups_that_grow_and_shrink_along_a_row(cuda, up):
     check_groups(cuda, change, 1, 1, 128, [640], seed=4)
 
 
+@pytest.mark.parametrize("first", [32, 64, 300])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_a_head_whose_first_scores_pass_below_all_numbers(cuda, d, first):
+    """Keys of 2^126 that one head meets with zeros and the other with negative numbers: for that one they weigh nothing, and the rest is what it was."""
+    g, lens = gen(first), [700]
+    table, blocks = kh.block_lists(g, lens, 256)
+    cache = kh.make_cache(g, blocks, 1, 256, d)
+    for t in range(first):
+        cache[1][table[0, t // 256], 0, t % 256, :, 0], cache[1][table[0, t // 256], 0, t % 256, :, 1] = 0, 2.0 ** 126
+    q = torch.zeros(1, 2, d, dtype=BF)
+    q[0, 1] = -8.0
+    got, (want, _) = call(cuda, q, cache, table, lens), kh.decode(q, cache, table, lens, d ** -0.5)
+    bound = want.abs() * 2.0 ** -8 + group_bound(q, cache, table, lens).repeat_interleave(64, -1)
+    # (the second head's scores are sums of numbers of one sign, up to 2^7: good to 2^-14 as a difference, too)
+    assert torch.isfinite(got).all() and ((got - want).abs() <= bound).all()
+
+
 # ---- what is not a number -------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("bad", [NAN, -NAN, INF, -INF])
 @pytest.mark.parametrize("d", [64, 128, 256])
