@@ -102,7 +102,7 @@ def _reach(hf, max_model_len: int) -> None:
     """``max_position_embeddings`` as far as a scaled rotation goes: ``factor`` times the trained length.  Checkpoints with linear scaling mostly
     give the scaled length already, so there the factor counts only as far as ``max_model_len`` asks for it."""
     scaling, most = getattr(hf, "rope_scaling", None), getattr(hf, "max_position_embeddings", None)
-    if not isinstance(scaling, dict) or most is None or _rope_kind(scaling) == "default":
+    if most is None or _rope_kind(scaling) not in ("linear", "yarn", "llama3"):
         return
     if scaling.get("original_max_position_embeddings") is None:
         hf.rope_scaling = scaling = {**scaling, "original_max_position_embeddings": most}

@@ -33,11 +33,11 @@ def scaled_frequencies(rotary_dim: int, rope_theta: float, scaling: dict) -> tup
     freq = rope_theta ** (-torch.arange(0, rotary_dim, 2, dtype=torch.double, device="cpu") / max(rotary_dim, 1))
     if kind == "default":
         return freq, 1.0
+    if kind not in ("linear", "yarn", "llama3"):
+        raise ValueError(f"rope scaling of type {kind!r} is not supported (default, linear, yarn, llama3)")
     factor = float(scaling["factor"])
     if kind == "linear":
         return freq / factor, 1.0
-    if kind not in ("yarn", "llama3"):
-        raise ValueError(f"rope scaling of type {kind!r} is not supported (default, linear, yarn, llama3)")
     trained = float(scaling["original_max_position_embeddings"])
     if kind == "llama3":
         low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])

@@ -88,6 +88,15 @@ def test_tables_reach_as_far_as_the_scaling(scaling, most, model_len, want):
     assert torch.equal(table[:most], build_cos_sin_cache(16, most, 1e6, scaling=scaling))
 
 
+def test_a_scaling_that_is_not_known_is_the_models_matter():
+    from mini_vllm_b200.config import Config, qwen3_shape
+    from mini_vllm_b200.models.models.qwen3 import Qwen3ForCausalLM
+    cfg = Config(hf_config=qwen3_shape(rope_scaling={"rope_type": "longrope", "short_factor": [1.0]})).hf_config
+    assert cfg.max_position_embeddings == 40960
+    with pytest.raises(ValueError, match="not supported"):
+        Qwen3ForCausalLM(cfg)
+
+
 def test_requests_past_the_tables_are_refused():
     from types import SimpleNamespace
     from mini_vllm_b200.config import SamplingParams
