@@ -14,14 +14,14 @@
 // (16 times as large) have it divided by 16.  Scores, softmax statistics and outputs are fp32; the weights p s are rounded once, to fp16.  Every
 // group of channels and head has a power of two of its own on them, moved when the group's greatest weight would pass 2^14: they never
 // overflow, and a group keeps its bits whatever the sizes of other groups, tokens and heads (scales from 2^-120 on; p itself is at most 2^-14, so
-// that a warp's sum of p m is finite too, for 16 K tokens of the largest values there are).  A rounding of p s meets the codes, up to 15 of them, while p m is exact: next to the plain form's error that is
-// 2^-11 sum p (15 s) more at most.
+// that a warp's sum of p m is finite too, for 16 K tokens of the largest values there are).  A rounding of p s meets the codes, up to 15 of them,
+// while p m is exact: next to the plain form's error that is 2^-11 sum p (15 s) more at most.
 //
 // On paper bound by memory: a tile of 32 tokens of a 128-wide head is 4608 bytes.  Its 650 warp instructions, most of them on the integer
 // pipe, bring instruction issue near: 240 sequences of 128-8192 tokens, 16 heads on 8, 0.51 GB in 115 us, 4.4 TB/s (0.68 of what a copy reaches),
 // 62 % of the issue slots, the integer pipe at 59 %.  Neither is at its limit: four warps a scheduler, at 128 registers with 156 bytes of them
-// spilled, do not cover each other's waits, and more do not fit.  A few rows are bound by the chain of dependent loads (lengths, block lists, tiles, parts):
-// one context of 700 tokens 10 us.
+// spilled, do not cover each other's waits, and more do not fit.  A few rows are bound by the chain of dependent loads (lengths, block lists,
+// tiles, parts): one context of 700 tokens 10 us.
 //
 // Work is tiles of 32 tokens of one (sequence, head), numbered sequence by sequence and head by head.  Each CTA takes a contiguous range (all
 // alike, or, where there are few rows, a share of one of them), each of its warps a contiguous part of that.  A warp streams its tiles
@@ -102,8 +102,8 @@ __device__ __forceinline__ float fast_log2(float x) {
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Powers of two, as their exponents say: of a whole number (0 below 2^-126, at most 2^127, and that of what is no number: nothing has been added up then), one over 2^-126 .. 2^126,
-// and what brings the greatest of a group's weights to 2^8 .. 2^9
+// Powers of two, as their exponents say: of a whole number (0 below 2^-126, at most 2^127, and that of what is no number: nothing has been added up
+// then), one over 2^-126 .. 2^126, and what brings the greatest of a group's weights to 2^8 .. 2^9
 constexpr float kMostUp = 0x1p126f;
 __device__ __forceinline__ float pow2_whole(float x) {
   return __uint_as_float(static_cast<uint32_t>(static_cast<int>(fmaxf(fminf(x, 127.f), -127.f)) + 127) << 23);

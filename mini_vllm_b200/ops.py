@@ -1375,8 +1375,8 @@ def rotary_kv4_write(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, p
                      slot_mapping: torch.Tensor, cache: KV4Cache, interleaved: bool = False, q_out: torch.Tensor | None = None,
                      k_in_place: bool = False, status: torch.Tensor | None = None) -> torch.Tensor | None:
     """Turns ``q`` (in place or into ``q_out``) and ``k`` as ``rotary`` does, and writes ``k`` and ``v`` in 4 bits to their cache slots
-    (-1: none; each slot once); ``k_in_place``: the turned k also goes back to ``k``, and ``v`` lies apart from it.  ``cos_sin`` None: nothing is turned.  bf16; the rotated channels a
-    multiple of 16.  Returns the turned q."""
+    (-1: none; each slot once); ``k_in_place``: the turned k also goes back to ``k``, and ``v`` lies apart from it.  ``cos_sin`` None:
+    nothing is turned.  bf16; the rotated channels a multiple of 16.  Returns the turned q."""
     if q is None and q_out is not None:
         raise ValueError("q_out needs q")
     device, bf16 = _device() if k.is_cuda else -2, torch.bfloat16
@@ -1462,8 +1462,8 @@ def decode_attn4(q: torch.Tensor, cache: KV4Cache, cache_seqlens: torch.Tensor, 
         spans_ptr = _dense(spans, i32, device, (B, hkv, budget), "spans")
     ws_ptr = _numbers(workspace, torch.uint8, device, 0, _BIG, "workspace")
     rc = _cabi.load().mvb_decode_attn4(q.data_ptr(), q_stride, cache.struct(device), lens_ptr, table_ptr, stride, width, spans_ptr, budget, B, hq,
-                                       float(scale), min(window_left, _INT), float(softcap), float(out_scale), out.data_ptr(), out_stride, ws_ptr, workspace.numel(),
-                                       _status(status, device), _stream())
+                                       float(scale), min(window_left, _INT), float(softcap), float(out_scale), out.data_ptr(), out_stride, ws_ptr,
+                                       workspace.numel(), _status(status, device), _stream())
     if rc:
         _cabi.check(rc, "mvb_decode_attn4")
     LaunchCounter.total += 1 if B else 0

@@ -87,7 +87,8 @@ class Scheduler:
                 req = self.prefilling[len(picked)]
                 if not fits(req, req.num_cached_tokens):
                     break
-            elif self.waiting and fits(self.waiting[0], len(self.waiting[0].tokens) if bm.support_prefix_cache else 0) and bm.can_allocate_new_block(self.waiting[0]):
+            elif (self.waiting and fits(self.waiting[0], len(self.waiting[0].tokens) if bm.support_prefix_cache else 0) and
+                  bm.can_allocate_new_block(self.waiting[0])):
                 req = self.waiting.popleft()
                 bm.allocate_blocks_for_prefill(req)
                 req.state = Request.RUNNING
